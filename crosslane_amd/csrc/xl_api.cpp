@@ -1792,6 +1792,217 @@ int32_t xl_hc_post_async(xl_context* ctx, const float* d_y, const float* d_res, 
     });
 }
 
+// ---- a block of an 8-bit model around the routed experts ---------------------------
+namespace {
+
+bool float_type(int32_t t) { return t == XL_F32 || t == XL_F16 || t == XL_BF16; }
+// Bytes from a matrix's first value to behind its last.
+uint64_t extent(int64_t rows, int64_t cols, int64_t stride, int size) {
+    return (uint64_t(rows - 1) * uint64_t(stride) + uint64_t(cols)) * uint64_t(size);
+}
+void check_rows(const void* p, int64_t stride, int64_t cols, int size, const char* what) {
+    if (stride < cols || stride > (int64_t(1) << 31)) fail(XL_E_ARG, "%s: stride below the row's length or above 2^31", what);
+    if (reinterpret_cast<uintptr_t>(p) % uintptr_t(size)) fail(XL_E_ARG, "%s: not aligned to its element type", what);
+}
+void check_q(const void* p, int64_t stride, int64_t cols, const char* what) {
+    check_rows(p, stride, cols, 1, what);
+    if (reinterpret_cast<uintptr_t>(p) % 16 || stride % 16)
+        fail(XL_E_ARG, "%s: int8 rows must be 16-byte aligned, with a stride that is a multiple of 16", what);
+}
+struct Span {
+    const void* p;   // null: none
+    uint64_t bytes;
+};
+void check_apart(const Span& out, std::initializer_list<Span> others, const char* what) {
+    if (!out.p) return;
+    for (const Span& o : others)
+        if (o.p && !apart(out.p, out.bytes, o.p, o.bytes)) fail(XL_E_ARG, "%s overlaps another buffer of the call", what);
+}
+
+struct LinearWork {
+    uint64_t q = 0, scale = 0, bytes = 0;
+    int64_t stride = 0;
+};
+// x quantized by the call, and its scales.
+LinearWork linear_work(int32_t T, int32_t K) {
+    LinearWork w;
+    w.stride = (int64_t(K) + 15) / 16 * 16;
+    w.scale = xl::align256(uint64_t(T) * uint64_t(w.stride));
+    w.bytes = w.scale + xl::align256(uint64_t(T) * 4);
+    return w;
+}
+
+}  // namespace
+
+int32_t xl_route_scored_async(xl_context* ctx, const void* d_logits, int32_t logits_type, int32_t T, int64_t stride,
+                              const float* d_bias_or_null, int32_t n, int32_t score, int32_t n_groups,
+                              int32_t top_groups, int32_t group_keys, int32_t k, int32_t renorm, float scale,
+                              int32_t* d_ids, float* d_w, void* stream, xl_error* err) {
+    return guarded(ctx, err, [&] {
+        need(d_logits && d_ids && d_w, XL_E_ARG, "null device pointer");
+        need(float_type(logits_type), XL_E_ARG, "logits must be f32, f16 or bf16");
+        need(T >= 1 && T <= xl::kLinMaxT, XL_E_ARG, "T outside 1..2^19");
+        need(n >= 1 && n <= xl::kScoreMaxExperts, XL_E_ARG, "expert count outside 1..1024");
+        need(score == XL_SCORE_SOFTMAX || score == XL_SCORE_SIGMOID, XL_E_ARG, "unknown score");
+        need(n_groups >= 1 && n_groups <= n && n % n_groups == 0, XL_E_ARG, "groups must divide the experts");
+        need(top_groups >= 1 && top_groups <= n_groups, XL_E_ARG, "top_groups outside 1..n_groups");
+        need((group_keys == 1 || group_keys == 2) && (n_groups == 1 || group_keys <= n / n_groups), XL_E_ARG,
+             "group_keys must be 1 or 2, and at most a group's experts");
+        need(k >= 1 && k <= 16 && k <= top_groups * (n / n_groups), XL_E_ARG,
+             "pick count outside 1..min(16, top_groups * group size)");
+        need(std::isfinite(scale) && scale >= 0.0f, XL_E_ARG, "route scale must be finite and >= 0");
+        const int es = xl::act_bytes(logits_type);
+        check_rows(d_logits, stride, n, es, "logits");
+        const Span lg{d_logits, extent(T, n, stride, es)}, bias{d_bias_or_null, uint64_t(n) * 4};
+        const Span ids{d_ids, uint64_t(T) * k * 4}, w{d_w, uint64_t(T) * k * 4};
+        check_apart(ids, {lg, bias, w}, "ids");
+        check_apart(w, {lg, bias}, "weights");
+        ready(ctx, false);
+        hipStream_t s = pick_stream(ctx, stream);
+        Ordered ord(ctx, s);
+        const xl::ScoreArgs a{d_logits, d_bias_or_null, stride, logits_type, T, n, k, score == XL_SCORE_SIGMOID, n_groups,
+                              top_groups, group_keys, renorm != 0, scale, d_ids, d_w, ctx->err_flag};
+        hip_check(xl::dev::launch_score_route(a, s, ord.stop()), "scored route launch");
+        ord.carried_by_launch(true);   // the launch records the ordering event itself
+    });
+}
+
+int32_t xl_block_norm_async(xl_context* ctx, const void* d_y_or_null, int64_t y_stride, const void* d_res_or_null,
+                            int64_t res_stride, const void* d_gate_or_null, int64_t gate_stride,
+                            const float* d_post_w_or_null, const float* d_pre_w_or_null, int32_t T, int32_t D,
+                            int32_t type, int32_t res_type, float alpha, float eps, void* d_res_out_or_null,
+                            int64_t res_out_stride, void* d_x_or_null, int64_t x_stride, int8_t* d_q_or_null,
+                            int64_t q_stride, float* d_q_scale_or_null, void* stream, xl_error* err) {
+    return guarded(ctx, err, [&] {
+        need(d_y_or_null || d_res_or_null, XL_E_ARG, "neither a block output nor a residual");
+        need(d_y_or_null || (!d_gate_or_null && !d_post_w_or_null), XL_E_ARG, "gate and post norm need the block output");
+        need(d_res_out_or_null || d_x_or_null || d_q_or_null, XL_E_ARG, "no output");
+        need(d_pre_w_or_null || (!d_x_or_null && !d_q_or_null), XL_E_ARG, "x and q need the weights of the norm before the block");
+        need((d_q_or_null != nullptr) == (d_q_scale_or_null != nullptr), XL_E_ARG, "q and its scales come together");
+        need(T >= 1 && T <= xl::kLinMaxT && D >= 1 && D <= xl::kNormMaxDim, XL_E_ARG, "T outside 1..2^19 or D outside 1..32768");
+        need(float_type(type) && float_type(res_type), XL_E_ARG, "element types must be f32, f16 or bf16");
+        need(std::isfinite(alpha) && std::isfinite(eps) && eps > 0.0f, XL_E_ARG, "alpha must be finite, eps finite and positive");
+        const int es = xl::act_bytes(type), rs = xl::act_bytes(res_type);
+        Span y{}, res{}, gate{}, ro{}, x{}, q{}, qs{};
+        const Span pw{d_post_w_or_null, uint64_t(D) * 4}, nw{d_pre_w_or_null, uint64_t(D) * 4};
+        const auto rows = [&](const void* p, int64_t stride, int size, const char* what) {
+            if (!p) return Span{};
+            check_rows(p, stride, D, size, what);
+            return Span{p, extent(T, D, stride, size)};
+        };
+        y = rows(d_y_or_null, y_stride, es, "y");
+        res = rows(d_res_or_null, res_stride, rs, "res");
+        if (d_gate_or_null && gate_stride == 0) {
+            check_rows(d_gate_or_null, D, D, es, "gate");
+            gate = Span{d_gate_or_null, uint64_t(D) * es};
+        } else {
+            gate = rows(d_gate_or_null, gate_stride, es, "gate");
+        }
+        ro = rows(d_res_out_or_null, res_out_stride, rs, "res_out");
+        x = rows(d_x_or_null, x_stride, es, "x");
+        if (d_q_or_null) {
+            check_q(d_q_or_null, q_stride, D, "q");
+            q = Span{d_q_or_null, extent(T, (int64_t(D) + 15) / 16 * 16, q_stride, 1)};
+            qs = Span{d_q_scale_or_null, uint64_t(T) * 4};
+        }
+        // in place: a workgroup has read its whole row of res and y before it writes
+        const Span res_other = ro.p && ro.p == res.p && res_out_stride == res_stride ? Span{} : res;
+        const Span y_other = x.p && x.p == y.p && x_stride == y_stride ? Span{} : y;
+        check_apart(ro, {y, res_other, gate, pw, nw, x, q, qs}, "res_out");
+        check_apart(x, {y_other, res, gate, pw, nw, q, qs}, "x");
+        check_apart(q, {y, res, gate, pw, nw, qs}, "q");
+        check_apart(qs, {y, res, gate, pw, nw}, "q_scale");
+        ready(ctx, false);
+        hipStream_t s = pick_stream(ctx, stream);
+        Ordered ord(ctx, s);
+        const xl::BlockNormArgs a{d_y_or_null, d_res_or_null, d_gate_or_null, d_post_w_or_null, d_pre_w_or_null,
+                                  d_res_out_or_null, d_x_or_null, d_q_or_null, d_q_scale_or_null, y_stride, res_stride,
+                                  gate_stride, res_out_stride, x_stride, q_stride, T, D, type, res_type, alpha, eps,
+                                  ctx->err_flag};
+        hip_check(xl::dev::launch_block_norm(a, s, ord.stop()), "block norm launch");
+        ord.carried_by_launch(true);   // the launch records the ordering event itself
+    });
+}
+
+int32_t xl_quantize_rows_async(xl_context* ctx, const void* d_x, int32_t type, int32_t T, int32_t K, int64_t x_stride,
+                               int8_t* d_q, int64_t q_stride, float* d_scale, void* stream, xl_error* err) {
+    return guarded(ctx, err, [&] {
+        need(d_x && d_q && d_scale, XL_E_ARG, "null device pointer");
+        need(float_type(type), XL_E_ARG, "rows must be f32, f16 or bf16");
+        need(T >= 1 && T <= xl::kLinMaxT && K >= 1 && K <= xl::kLinMaxK, XL_E_ARG, "T outside 1..2^19 or K outside 1..65536");
+        const int es = xl::act_bytes(type);
+        check_rows(d_x, x_stride, K, es, "x");
+        check_q(d_q, q_stride, K, "q");
+        const Span x{d_x, extent(T, K, x_stride, es)}, scale{d_scale, uint64_t(T) * 4};
+        const Span q{d_q, extent(T, (int64_t(K) + 15) / 16 * 16, q_stride, 1)};
+        check_apart(q, {x, scale}, "q");
+        check_apart(scale, {x}, "scale");
+        ready(ctx, false);
+        hipStream_t s = pick_stream(ctx, stream);
+        Ordered ord(ctx, s);
+        hip_check(xl::dev::launch_quant_rows(d_x, type, x_stride, T, K, d_q, q_stride, d_scale, ctx->err_flag, s, ord.stop()),
+                  "row quantization launch");
+        ord.carried_by_launch(true);   // the launch records the ordering event itself
+    });
+}
+
+uint64_t xl_linear_i8_work_bytes(int32_t T, int32_t K, int32_t N, int32_t gated) {
+    (void)gated;
+    if (T < 1 || T > xl::kLinMaxT || K < 1 || K > xl::kLinMaxK || N < 1 || N > xl::kLinMaxT) return 0;
+    return linear_work(T, K).bytes;
+}
+
+int32_t xl_linear_i8_async(xl_context* ctx, const void* d_x, int32_t x_type, const float* d_x_scale_or_null,
+                           int64_t x_stride, int32_t T, int32_t K, const int8_t* d_w, const float* d_w_scale,
+                           const int8_t* d_up_or_null, const float* d_up_scale_or_null, int64_t w_stride, int32_t N,
+                           float limit, void* d_out, int32_t out_type, int64_t out_stride, void* d_work,
+                           uint64_t work_bytes, void* stream, xl_error* err) {
+    return guarded(ctx, err, [&] {
+        need(d_x && d_w && d_w_scale && d_out && d_work, XL_E_ARG, "null device pointer");
+        need((d_up_or_null != nullptr) == (d_up_scale_or_null != nullptr), XL_E_ARG, "up and its scales come together");
+        need(x_type == XL_I8 || float_type(x_type), XL_E_ARG, "x must be f32, f16, bf16 or int8");
+        need((x_type == XL_I8) == (d_x_scale_or_null != nullptr), XL_E_ARG, "x_scale goes with an int8 x, and with no other");
+        need(float_type(out_type), XL_E_ARG, "out must be f32, f16 or bf16");
+        need(T >= 1 && T <= xl::kLinMaxT && N >= 1 && N <= xl::kLinMaxT && K >= 1 && K <= xl::kLinMaxK, XL_E_ARG,
+             "T or N outside 1..2^19, or K outside 1..65536");
+        need(std::isfinite(limit), XL_E_ARG, "limit not finite");
+        const int64_t K16 = (int64_t(K) + 15) / 16 * 16;
+        const int xs = xl::act_bytes(x_type), os = xl::act_bytes(out_type);
+        if (x_type == XL_I8) check_q(d_x, x_stride, K, "x");
+        else check_rows(d_x, x_stride, K, xs, "x");
+        check_q(d_w, w_stride, K, "w");
+        if (d_up_or_null) check_q(d_up_or_null, w_stride, K, "up");
+        check_rows(d_out, out_stride, N, os, "out");
+        need(w_stride <= (int64_t(1) << 20) && (x_type != XL_I8 || x_stride <= (int64_t(1) << 20)), XL_E_ARG,
+             "int8 strides above 2^20");
+        const LinearWork lw = linear_work(T, K);
+        need(work_bytes >= lw.bytes, XL_E_ARG, "workspace smaller than xl_linear_i8_work_bytes(T, K, N, gated)");
+        need(reinterpret_cast<uintptr_t>(d_work) % 256 == 0, XL_E_ARG, "workspace not 256-byte aligned");
+        const Span x{d_x, extent(T, K, x_stride, xs)}, xsc{d_x_scale_or_null, uint64_t(T) * 4};
+        const Span w{d_w, extent(N, K16, w_stride, 1)}, ws{d_w_scale, uint64_t(N) * 4};
+        const Span up{d_up_or_null, extent(N, K16, w_stride, 1)}, us{d_up_scale_or_null, uint64_t(N) * 4};
+        const Span out{d_out, extent(T, N, out_stride, os)}, work{d_work, lw.bytes};
+        check_apart(out, {x, xsc, w, ws, up, us, work}, "out");
+        check_apart(work, {x, xsc, w, ws, up, us}, "workspace");
+        ready(ctx, false);
+        hipStream_t s = pick_stream(ctx, stream);
+        Ordered ord(ctx, s);
+        xl::Lin8Args a{static_cast<const int8_t*>(d_x), d_x_scale_or_null, d_w, d_w_scale, d_up_or_null,
+                       d_up_scale_or_null, d_out, x_stride, w_stride, out_stride, T, K, N, out_type, limit};
+        if (x_type != XL_I8) {
+            int8_t* q = static_cast<int8_t*>(d_work);
+            float* scale = reinterpret_cast<float*>(q + lw.scale);
+            hip_check(xl::dev::launch_quant_rows(d_x, x_type, x_stride, T, K, q, lw.stride, scale, ctx->err_flag, s, nullptr),
+                      "row quantization launch");
+            a.x = q;
+            a.x_scale = scale;
+            a.x_stride = lw.stride;
+        }
+        hip_check(xl::dev::launch_lin8(a, ctx->cus, s, ord.stop()), "int8 product launch");
+        ord.carried_by_launch(true);   // the launch records the ordering event itself
+    });
+}
+
 int32_t xl_sync(xl_context* ctx, void* stream, xl_error* err) {
     return guarded(ctx, err, [&] {
         need(ctx != nullptr, XL_E_ARG, "null context");

@@ -174,6 +174,56 @@ constexpr int kLayer3TableBytes = 24576;   // expanded codebooks of the single-l
 constexpr int kTableIQ1X = kLayer3TableBytes;
 constexpr int kTableBytes = kTableIQ1X + 4096 * 8;
 
+// Element types of activations (XL_F32 ... of the C ABI).
+enum : int { kActF32 = 0, kActF16 = 1, kActBF16 = 2, kActI8 = 3 };
+inline int act_bytes(int type) { return type == kActF32 ? 4 : type == kActI8 ? 1 : 2; }
+constexpr int kNormMaxDim = 32768;     // block norm: 1024 threads of 32 values
+constexpr int kScoreMaxExperts = 1024; // scored router: 16 keys per lane
+constexpr int kLinMaxK = 65536;        // int8 product: 65536 * 2^14 = 2^30 stays inside an int32
+constexpr int kLinMaxT = 1 << 19;      // ... at most this many tokens and channels
+// What lies between two blocks (xl_norm.hip); y, res, gate, post_w, pre_w, res_out, x
+// and q may be null, strides in elements.
+struct BlockNormArgs {
+    const void* y;
+    const void* res;
+    const void* gate;           // gate_stride 0: one row for every token
+    const float* post_w;
+    const float* pre_w;
+    void* res_out;
+    void* x;
+    int8_t* q;
+    float* q_scale;
+    int64_t y_stride, res_stride, gate_stride, res_out_stride, x_stride, q_stride;
+    int T, D, type, res_type;   // type: y, gate and x; res_type: res and res_out
+    float alpha, eps;
+    int* err;
+};
+// Router over softmax or sigmoid scores (xl_score.hip).
+struct ScoreArgs {
+    const void* logits;
+    const float* bias;          // or null
+    int64_t stride;
+    int type, T, n, k, sigmoid, groups, top_groups, group_keys, renorm;
+    float scale;
+    int32_t* ids;
+    float* w;
+    int* err;
+};
+// int8 product (xl_lin8.hip): out[t][r] = (sum_k x[t][k] w[r][k]) * x_scale[t] *
+// w_scale[r], or SwiGLU of two such products (up set).
+struct Lin8Args {
+    const int8_t* x;
+    const float* x_scale;
+    const int8_t* w;
+    const float* w_scale;
+    const int8_t* up;           // or null
+    const float* up_scale;
+    void* out;
+    int64_t x_stride, w_stride, out_stride;
+    int T, K, N, out_type;
+    float lim;
+};
+
 // Size of the no-allocation entry point's static device scratch (xl_noalloc.hip).
 constexpr uint64_t kNoAllocScratchBytes = uint64_t(8) << 20;
 
@@ -295,6 +345,13 @@ constexpr int kFfnTokensMin = 3;
 hipError_t launch_ffn_tokens(const MatRef& gate, const MatRef& up, const MatRef& down, int T, int dim, int ff,
                              const float* x, float* out, int8_t* xq, float* xd, int8_t* hq, float* hd, float lim,
                              int* err, int cus, hipStream_t s);
+hipError_t launch_block_norm(const BlockNormArgs& a, hipStream_t s, hipEvent_t stop);
+// Rows of x (type f32, f16 or bf16) to int8 with a scale each; the bytes from K
+// to the next multiple of 16 are zeroed.
+hipError_t launch_quant_rows(const void* x, int type, int64_t x_stride, int T, int K, int8_t* q, int64_t q_stride,
+                             float* scale, int* err, hipStream_t s, hipEvent_t stop);
+hipError_t launch_score_route(const ScoreArgs& a, hipStream_t s, hipEvent_t stop);
+hipError_t launch_lin8(const Lin8Args& a, int cus, hipStream_t s, hipEvent_t stop);
 // h = SwiGLU(g, u) elementwise over n values, with the limit (lim <= 0: none).
 hipError_t launch_swiglu(const float* g, const float* u, int n, float lim, float* h, hipStream_t s);
 // Seeded generation of one planar matrix (role 0 gate, 1 up, 2 down).

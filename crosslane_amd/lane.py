@@ -110,6 +110,14 @@ _SIGNATURES = {
     "xl_layer_forward_post_async": (_I32, [_P, _I32, _P, _P, _I32, _P, _P, _P, _P, _P, _P, _I32, _P, _P, _ErrP]),
     "xl_moe_block_async": (_I32, [_P, _I32, _P, _P, _I32, _P, _I32, _P, _I32, _P, _I32, _P, _I32, _P, C.c_uint64,
                                   _P, _P, _P, _I32, _P, _P, _P, _ErrP]),
+    "xl_route_scored_async": (_I32, [_P, _P, _I32, _I32, C.c_int64, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32,
+                                     C.c_float, _P, _P, _P, _ErrP]),
+    "xl_block_norm_async": (_I32, [_P, _P, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P, _P, _I32, _I32, _I32, _I32,
+                                   C.c_float, C.c_float, _P, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P, _P, _ErrP]),
+    "xl_quantize_rows_async": (_I32, [_P, _P, _I32, _I32, _I32, C.c_int64, _P, C.c_int64, _P, _P, _ErrP]),
+    "xl_linear_i8_work_bytes": (C.c_uint64, [_I32, _I32, _I32, _I32]),
+    "xl_linear_i8_async": (_I32, [_P, _P, _I32, _P, C.c_int64, _I32, _I32, _P, _P, _P, _P, C.c_int64, _I32, C.c_float,
+                                  _P, _I32, C.c_int64, _P, C.c_uint64, _P, _ErrP]),
     "xl_profile_begin": (_I32, [_P, _I32, _ErrP]),
     "xl_profile_end": (_I32, [_P, _f32p, _I32, C.POINTER(_I32), C.POINTER(_I32), C.c_char_p, _I32, _ErrP]),
     "xl_profile_timeline": (_I32, [_P, _u64p, _I32, C.POINTER(_I32), _ErrP]),
@@ -206,6 +214,43 @@ def pack_meta(pack_dir: str) -> dict:
 def shared_work_bytes(dim: int, ff: int, T: int = 1) -> int:
     """Workspace bytes xl_shared_forward_async needs for T tokens."""
     return int(lib().xl_shared_work_bytes(dim, ff, T))
+
+
+def linear_i8_work_bytes(T: int, K: int, N: int, gated: bool = False) -> int:
+    """Workspace bytes xl_linear_i8_async needs for T tokens of K values and N output channels."""
+    return int(lib().xl_linear_i8_work_bytes(T, K, N, int(gated)))
+
+
+# Element types of the calls around a block (XL_F32 ... by the tensor's dtype)
+_ACT = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2, "torch.int8": 3}
+SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def _arg(ok: bool, message: str) -> None:
+    if not ok:
+        raise XLError(1, message)
+
+
+def _act(t, what: str, allowed=(0, 1, 2)) -> int:
+    a = _ACT.get(str(t.dtype), -1)
+    _arg(a in allowed, f"{what}: element type {t.dtype} not taken here")
+    return a
+
+
+def _rows(t, what: str, shape=None) -> int:
+    """A [T, n] matrix of contiguous rows on the GPU; returns its row stride."""
+    _arg(t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1), f"{what}: a matrix of contiguous rows is wanted")
+    _arg(t.is_cuda, f"{what}: not on the GPU")
+    _arg(shape is None or tuple(t.shape) == tuple(shape), f"{what}: shape {tuple(t.shape)} where {shape} is wanted")
+    return int(t.stride(0)) if t.shape[0] > 1 else max(int(t.stride(0)), int(t.shape[1]))
+
+
+def _vec(t, n: int, what: str, dtype: str = "torch.float32"):
+    """A contiguous GPU vector of n values (None passes)."""
+    if t is not None:
+        _arg(t.is_cuda and t.is_contiguous() and t.numel() == n and str(t.dtype) == dtype,
+             f"{what}: {n} contiguous {dtype} values on the GPU are wanted")
+    return t
 
 
 def pack_types(pack_dir: str, first_layer: int, n_layers: int, n_experts: int) -> np.ndarray:
@@ -528,6 +573,79 @@ class Lane:
         T, H, D = (int(v) for v in res.shape)
         self._call("xl_hc_post_async", _ptr(y), _ptr(res), _ptr(post), _ptr(comb), D, H, T, _ptr(out),
                    None if stream is None else int(stream))
+
+    def route_scored_async(self, logits, k: int, ids, w, score: str = "softmax", bias=None, groups: int = 1,
+                           top_groups: int = 1, group_keys: int = 1, renorm: bool = True, scale: float = 1.0,
+                           stream=None) -> None:
+        """Router over softmax or sigmoid scores: logits [T, n] (f32, f16 or bf16; -inf
+        masks an expert), bias [n] float32 added to the scores for the choice only,
+        `top_groups` of `groups` expert groups by the sum of their `group_keys`
+        largest keys; ids (int32) and w [T, k]."""
+        _arg(score in SCORES, f"score must be one of {sorted(SCORES)}")
+        stride = _rows(logits, "logits")
+        T, n = (int(v) for v in logits.shape)
+        _vec(ids, T * k, "ids", "torch.int32"), _vec(w, T * k, "w"), _vec(bias, n, "bias")
+        self._call("xl_route_scored_async", _ptr(logits), _act(logits, "logits"), T, stride, _ptr(bias), n, SCORES[score],
+                   groups, top_groups, group_keys, k, int(renorm), float(scale), _ptr(ids), _ptr(w),
+                   None if stream is None else int(stream))
+
+    def block_norm_async(self, res, y=None, post_w=None, gate=None, alpha: float = 1.0, pre_w=None, eps: float = 1e-6,
+                         res_out=None, x=None, q=None, q_scale=None, stream=None) -> None:
+        """Between two blocks: a = y (RMS-normed with post_w [D]); r = alpha * res +
+        gate * a; x = RMS norm of r with pre_w [D]. res, y [T, D] (one may be None),
+        gate [T, D], [D] or None; outputs res_out (r, as res), x (as y) [T, D], and q
+        int8 [T, D] with q_scale [T]: x quantized, for linear_i8_async."""
+        some = y if res is None else res
+        _arg(some is not None, "res or y is wanted")
+        T, D = (int(v) for v in some.shape)
+        shape = (T, D)
+        st = {n: 0 if t is None else _rows(t, n, shape)
+              for n, t in (("y", y), ("res", res), ("res_out", res_out), ("x", x), ("q", q))}
+        gs = 0
+        if gate is not None and gate.dim() == 1:
+            _vec(gate, D, "gate", str(gate.dtype))
+        elif gate is not None:
+            gs = _rows(gate, "gate", shape)
+        act = [t for t in (y, x, gate) if t is not None]
+        streams = [t for t in (res, res_out) if t is not None]
+        kinds = {_act(t, "y, x and gate") for t in act}, {_act(t, "res and res_out") for t in streams}
+        _arg(len(kinds[0]) <= 1 and len(kinds[1]) <= 1, "y, x and gate have one element type, res and res_out one")
+        _arg(q is None or str(q.dtype) == "torch.int8", "q must be int8")
+        _vec(post_w, D, "post_w"), _vec(pre_w, D, "pre_w"), _vec(q_scale, T, "q_scale")
+        rt = kinds[1].pop() if kinds[1] else 0
+        self._call("xl_block_norm_async", _ptr(y), st["y"], _ptr(res), st["res"], _ptr(gate), gs, _ptr(post_w),
+                   _ptr(pre_w), T, D, kinds[0].pop() if kinds[0] else rt, rt, float(alpha), float(eps), _ptr(res_out),
+                   st["res_out"], _ptr(x), st["x"], _ptr(q), st["q"], _ptr(q_scale),
+                   None if stream is None else int(stream))
+
+    def quantize_rows_async(self, x, q, scale, stream=None) -> None:
+        """x [T, K] (f32, f16 or bf16) to int8 q [T, K] (16-byte aligned rows) with scale [T]."""
+        stride = _rows(x, "x")
+        T, K = (int(v) for v in x.shape)
+        qs = _rows(q, "q", (T, K))
+        _arg(str(q.dtype) == "torch.int8", "q must be int8")
+        _vec(scale, T, "scale")
+        self._call("xl_quantize_rows_async", _ptr(x), _act(x, "x"), T, K, stride, _ptr(q), qs, _ptr(scale),
+                   None if stream is None else int(stream))
+
+    def linear_i8_async(self, x, w, w_scale, out, x_scale=None, up=None, up_scale=None, limit: float = 0.0, work=None,
+                        stream=None) -> None:
+        """out [T, N] = x [T, K] times int8 w [N, K] (16-byte aligned rows) with a scale
+        for each token and channel; x int8 with x_scale [T], or float (quantized by
+        the call). With up, up_scale: SwiGLU of the products with w (gate) and up.
+        work: linear_i8_work_bytes(T, K, N, gated) bytes."""
+        xs, ws = _rows(x, "x"), _rows(w, "w")
+        T, K = (int(v) for v in x.shape)
+        N = int(w.shape[0])
+        _arg(int(w.shape[1]) == K and str(w.dtype) == "torch.int8", "w: int8 [N, K] is wanted")
+        os_ = _rows(out, "out", (T, N))
+        if up is not None:
+            _arg(str(up.dtype) == "torch.int8" and _rows(up, "up", (N, K)) == ws, "up: int8 with w's shape and stride is wanted")
+        _vec(x_scale, T, "x_scale"), _vec(w_scale, N, "w_scale"), _vec(up_scale, N, "up_scale")
+        _arg(work is not None and work.is_cuda and work.is_contiguous(), "work: a contiguous GPU buffer is wanted")
+        self._call("xl_linear_i8_async", _ptr(x), _act(x, "x", (0, 1, 2, 3)), _ptr(x_scale), xs, T, K, _ptr(w),
+                   _ptr(w_scale), _ptr(up), _ptr(up_scale), ws, N, float(limit), _ptr(out), _act(out, "out"), os_,
+                   _ptr(work), int(work.numel() * work.element_size()), None if stream is None else int(stream))
 
     def swiglu_async(self, g, u, h, limit: float = 0.0, stream=None) -> None:
         self._call("xl_swiglu_async", _ptr(g), _ptr(u), int(g.numel()), float(limit), _ptr(h),

@@ -396,6 +396,82 @@ int32_t xl_moe_block_async(xl_context* ctx, int32_t layer, const int32_t* d_ids,
                            const float* d_res, const float* d_post, const float* d_comb, int32_t H, float* d_out,
                            float* d_post_out, void* stream, xl_error* err);
 
+/* ---- a block of an 8-bit model around the routed experts (device pointers) ----
+ * What a MoE block has around the lane's calls in models with an ordinary
+ * residual stream and int8 weights: the norms between blocks, a router over
+ * softmax or sigmoid scores, and the int8 product of the dense projections and
+ * the shared expert. No counterpart in the reference (its model has the
+ * hyper-connection forms and route_cpu above). The calls use neither the bank nor
+ * the context's workspace. Element types of activations: XL_F32, XL_F16,
+ * XL_BF16 (XL_I8 where a call says so); every stride is in elements, from one
+ * token's first value to the next's. Sums and scales are float32 or more. */
+enum { XL_F32 = 0, XL_F16 = 1, XL_BF16 = 2, XL_I8 = 3 };
+enum { XL_SCORE_SOFTMAX = 0, XL_SCORE_SIGMOID = 1 };
+
+/* Router over scores, per token: s = softmax(logits) or sigmoid(logits); key = s +
+ * bias (null: zeros). With n_groups > 1 the experts are n_groups equal groups of
+ * consecutive ids, a group is worth the sum of its group_keys (1 or 2) largest
+ * keys, and only the top_groups of largest value stay. The k largest keys of what
+ * stays are picked, in descending order; all ties go to the lower index. weight =
+ * s (without the bias), with renorm divided by (sum of the picked s + 1e-20),
+ * times scale. Scores and keys are doubles, the weight rounds to float once.
+ * A logit of -inf masks its expert: s = 0, key below every other, so it is picked
+ * only where fewer than k others stay, with weight 0 (a row of -inf alone: the
+ * lowest ids, weights 0). NaN, +inf or a non-finite bias set the device flag.
+ * logits T x stride of type logits_type (n used, n <= 1024); ids and w T x k (k <= 16,
+ * k <= top_groups * n / n_groups); T <= 2^19. ids, w go to the layer and grouped
+ * calls as they are. */
+int32_t xl_route_scored_async(xl_context* ctx, const void* d_logits, int32_t logits_type, int32_t T, int64_t stride,
+                              const float* d_bias_or_null, int32_t n, int32_t score, int32_t n_groups,
+                              int32_t top_groups, int32_t group_keys, int32_t k, int32_t renorm, float scale,
+                              int32_t* d_ids, float* d_w, void* stream, xl_error* err);
+
+/* What lies between two blocks, for T tokens of D values (D <= 32768), one launch:
+ *   a = y;  post_w: a = a / sqrt(mean(a^2) + eps) * post_w    (norm after the block)
+ *   r = alpha * res + gate * a                                (residual scale, gate)
+ *   pre_w: x = r / sqrt(mean(r^2) + eps) * pre_w              (norm before the next)
+ * float32 throughout, x from the unrounded r. y null: r = alpha * res (gate and
+ * post_w null too); res null: r = gate * a. gate: T x D, or one row for all tokens
+ * (gate_stride 0), or null (1). y, gate and x have element type `type`, res and
+ * res_out `res_type`. Outputs, each optional but one needed: res_out (r), x, and q
+ * with q_scale: x quantized as xl_quantize_rows_async would quantize it unrounded
+ * (q 16-byte aligned, q_stride a multiple of 16). x and q need pre_w. res_out may be
+ * res and x may be y (same stride); every other overlap of an output is rejected. */
+int32_t xl_block_norm_async(xl_context* ctx, const void* d_y_or_null, int64_t y_stride, const void* d_res_or_null,
+                            int64_t res_stride, const void* d_gate_or_null, int64_t gate_stride,
+                            const float* d_post_w_or_null, const float* d_pre_w_or_null, int32_t T, int32_t D,
+                            int32_t type, int32_t res_type, float alpha, float eps, void* d_res_out_or_null,
+                            int64_t res_out_stride, void* d_x_or_null, int64_t x_stride, int8_t* d_q_or_null,
+                            int64_t q_stride, float* d_q_scale_or_null, void* stream, xl_error* err);
+
+/* T rows of K values to int8 with a scale each (tokens of activations, or the
+ * output channels of a weight matrix): scale = max|x| / 127, q =
+ * round-half-even(x / scale), -127..127, separate float roundings. A row of zeros
+ * has scale 0. A row with an infinity or NaN sets the device flag and has scale
+ * NaN and q = 0. q 16-byte aligned, q_stride a multiple of 16 (the bytes from K to
+ * the next multiple of 16 are zeroed); K <= 65536, T <= 2^19. */
+int32_t xl_quantize_rows_async(xl_context* ctx, const void* d_x, int32_t type, int32_t T, int32_t K, int64_t x_stride,
+                               int8_t* d_q, int64_t q_stride, float* d_scale, void* stream, xl_error* err);
+
+/* Product with int8 weights: out[t][r] = (sum_k x[t][k] * w[r][k]) * x_scale[t] *
+ * w_scale[r], the sum exact in int32. x: int8 (x_type XL_I8, with d_x_scale; 16-byte
+ * aligned, x_stride a multiple of 16) or float (d_x_scale null): then the call
+ * quantizes it as xl_quantize_rows_async does. w: N rows of K, 16-byte aligned,
+ * w_stride a multiple of 16 (each row readable up to the next multiple of 16; what
+ * lies between is not used). With d_up (as w, same stride) and d_up_scale: SwiGLU
+ * of the two products, limit > 0 clamping g to <= limit and u to [-limit, limit],
+ * out = g / (1 + exp(-g)) * u (the gate and up of a shared expert; its output is
+ * the row that the layer and grouped calls take as `shared`). out: XL_F32, XL_F16 or
+ * XL_BF16, one rounding. K <= 65536, N and T <= 2^19. d_work: 256-byte aligned,
+ * xl_linear_i8_work_bytes(T, K, N, gated) bytes (needed whatever x_type is), used
+ * during the call only. out and work overlap nothing else. */
+uint64_t xl_linear_i8_work_bytes(int32_t T, int32_t K, int32_t N, int32_t gated);
+int32_t xl_linear_i8_async(xl_context* ctx, const void* d_x, int32_t x_type, const float* d_x_scale_or_null,
+                           int64_t x_stride, int32_t T, int32_t K, const int8_t* d_w, const float* d_w_scale,
+                           const int8_t* d_up_or_null, const float* d_up_scale_or_null, int64_t w_stride, int32_t N,
+                           float limit, void* d_out, int32_t out_type, int64_t out_stride, void* d_work,
+                           uint64_t work_bytes, void* stream, xl_error* err);
+
 /* ---- stage profiling --------------------------------------------------------
  * Between xl_profile_begin and xl_profile_end, the first max_calls layer calls
  * record a HIP event before and after each kernel on the stream it runs on
