@@ -53,6 +53,21 @@ __device__ __forceinline__ T rounded(float v) {
     return T(v);
 }
 
+// store8 of float32 products, in two roundings (see `rounded`).
+template <class T>
+__device__ __forceinline__ void store8_rounded(T* p, int n, const float (&v)[8]) {
+    if (n >= 8) {
+        T t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = rounded<T>(v[i]);
+        __builtin_memcpy(p, t, sizeof t);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = rounded<T>(v[i]);
+    }
+}
+
 template <int CTRL, int MASK = 0xF>
 __device__ __forceinline__ float dpp_or(float id, float v) {   // lanes that the pattern leaves out get `id`
     return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(id), __float_as_int(v), CTRL, MASK, 0xF, false));
