@@ -53,17 +53,17 @@ __device__ __forceinline__ T rounded(float v) {
     return T(v);
 }
 
-// store8 of float32 products, in two roundings (see `rounded`).
-template <class T>
-__device__ __forceinline__ void store8_rounded(T* p, int n, const float (&v)[8]) {
-    if (n >= 8) {
-        T t[8];
+// N (4 or 8) float32 products to memory, `n` of them in the row, in two roundings each (see `rounded`).
+template <class T, int N>
+__device__ __forceinline__ void store_rounded(T* p, int n, const float (&v)[N]) {
+    if (n >= N) {
+        T t[N];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) t[i] = rounded<T>(v[i]);
+        for (int i = 0; i < N; ++i) t[i] = rounded<T>(v[i]);
         __builtin_memcpy(p, t, sizeof t);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < N - 1; ++i)
             if (i < n) p[i] = rounded<T>(v[i]);
     }
 }
@@ -103,6 +103,12 @@ __device__ __forceinline__ float group_join(float v, float* red) {
 // rows give equal quants on any path. A row of zeros: d = 0, q = 0. A row with
 // an infinity or a NaN: the device flag, q = 0 and d = NaN (its products are
 // NaN, no finite wrong number).
+//
+// The quotient x / d of each value costs a dozen instructions; x times 1 / d rounds
+// to the same whole number unless it lies within 2^-14 of a half: it is off by 127.5
+// times 3 half steps at most (1 / d, the product, and the quotient's own rounding),
+// 2.3e-5. So only groups of eight with such a value, and rows with a scale so small that
+// 1 / d leaves the normal range, divide.
 __device__ __forceinline__ uint32_t quant4(const float* v, float d) {
     uint32_t r = 0;
 #pragma unroll
@@ -111,6 +117,46 @@ __device__ __forceinline__ uint32_t quant4(const float* v, float d) {
         r |= (uint32_t(int(q)) & 0xffu) << (8 * i);
     }
     return d > 0.0f ? r : 0u;
+}
+// Eight quants at q[0..7]; those past the row (n..7) are zeros, written up to
+// the next multiple of 16 bytes by whichever thread owns them.
+__device__ __forceinline__ void store_quants(int8_t* q, const float (&v)[8], float d) {
+    uint32_t o[2];
+    const float inv = 1.0f / d;
+    bool far = d >= 0x1p-100f;
+    uint32_t n[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float t = v[i] * inv, m = t + 12582912.0f;   // 1.5 * 2^23: t rounded to a whole number, in the low bits
+        n[i] = __float_as_uint(m);
+        far = far && fabsf(t - (m - 12582912.0f)) < 0.5f - 0x1p-14f;
+    }
+    if (far) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            o[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(n[4 * i + 3], n[4 * i + 2], 0x0c0c0400u),
+                                         __builtin_amdgcn_perm(n[4 * i + 1], n[4 * i], 0x0c0c0400u), 0x05040100u);
+    } else {
+        o[0] = quant4(v, d);
+        o[1] = quant4(v + 4, d);
+    }
+    __builtin_memcpy(q, o, 8);
+}
+
+// A row's scale from its largest magnitude (infinite where a value is not
+// finite: the device flag, and a NaN).
+__device__ __forceinline__ float row_scale(float amax, int* err) {
+    if (amax <= 3.402823466e38f) return __fdiv_rn(amax, 127.0f);
+    if (threadIdx.x == 0) atomicOr(err, kDevErrNonFinite);
+    return __int_as_float(0x7fc00000);
+}
+__device__ __forceinline__ float amax8(const float (&v)[8], float m) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float a = fabsf(v[i]);
+        m = a <= 3.402823466e38f ? fmaxf(m, a) : __int_as_float(0x7f800000);   // a NaN fails the comparison too
+    }
+    return m;
 }
 
 }  // namespace xl::dev

@@ -1988,8 +1988,9 @@ int32_t xl_linear_i8_async(xl_context* ctx, const void* d_x, int32_t x_type, con
         hipStream_t s = pick_stream(ctx, stream);
         Ordered ord(ctx, s);
         xl::Lin8Args a{static_cast<const int8_t*>(d_x), d_x_scale_or_null, d_w, d_w_scale, d_up_or_null,
-                       d_up_scale_or_null, d_out, x_stride, w_stride, out_stride, T, K, N, out_type, limit};
-        if (x_type != XL_I8) {
+                       d_up_scale_or_null, d_out, x_stride, w_stride, out_stride, T, K, N, x_type, out_type, limit,
+                       ctx->err_flag};
+        if (x_type != XL_I8 && !xl::lin8_quantizes(T, K)) {
             int8_t* q = static_cast<int8_t*>(d_work);
             float* scale = reinterpret_cast<float*>(q + lw.scale);
             hip_check(xl::dev::launch_quant_rows(d_x, x_type, x_stride, T, K, q, lw.stride, scale, ctx->err_flag, s, nullptr),
@@ -1997,6 +1998,7 @@ int32_t xl_linear_i8_async(xl_context* ctx, const void* d_x, int32_t x_type, con
             a.x = q;
             a.x_scale = scale;
             a.x_stride = lw.stride;
+            a.x_type = XL_I8;
         }
         hip_check(xl::dev::launch_lin8(a, ctx->cus, s, ord.stop()), "int8 product launch");
         ord.carried_by_launch(true);   // the launch records the ordering event itself

@@ -181,6 +181,9 @@ constexpr int kNormMaxDim = 32768;     // block norm: 1024 threads of 32 values
 constexpr int kScoreMaxExperts = 1024; // scored router: 16 keys per lane
 constexpr int kLinMaxK = 65536;        // int8 product: 65536 * 2^14 = 2^30 stays inside an int32
 constexpr int kLinMaxT = 1 << 19;      // ... at most this many tokens and channels
+// Whether the int8 product quantizes a float x itself (one row: each workgroup holds
+// its quants in LDS) or takes the quantizer's.
+inline bool lin8_quantizes(int T, int K) { return T == 1 && K <= 16384; }
 // What lies between two blocks (xl_norm.hip); y, res, gate, post_w, pre_w, res_out, x
 // and q may be null, strides in elements.
 struct BlockNormArgs {
@@ -220,8 +223,9 @@ struct Lin8Args {
     const float* up_scale;
     void* out;
     int64_t x_stride, w_stride, out_stride;
-    int T, K, N, out_type;
+    int T, K, N, x_type, out_type;   // x_type other than int8: x float, x_scale unused (lin8_quantizes)
     float lim;
+    int* err;
 };
 
 // Size of the no-allocation entry point's static device scratch (xl_noalloc.hip).

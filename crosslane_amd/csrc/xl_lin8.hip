@@ -11,7 +11,14 @@
 // Tokens are the result's rows, channels its columns.
 #include <hip/hip_ext.h>
 
+#include <algorithm>
+#include <cmath>
+#include <iterator>
+#include <type_traits>
+#include <utility>
+
 #include "xl_act.hpp"
+#include "xl_dev.hpp"
 
 namespace xl::dev {
 namespace {
@@ -58,97 +65,157 @@ __device__ __forceinline__ void tile_of(int b, int tm, int tn, int& m, int& n) {
 // the first operand: a lane's results are channels 4 q + i of one token. Row m of a
 // wave's tile i is channel 4 NI (m / 4) + 4 i + m % 4 of the wave's, so that a lane has
 // 4 NI consecutive channels and a token's are stored in runs of 16 NI.
-template <class OT, bool GATED, int TT, int TC, int WT, int WC>
-__global__ __launch_bounds__(64 * WT * WC, TT >= 256 ? 2 : 1) void lin8_tile_kernel(Lin8Args a, int tm, int tn) {
+template <int I>
+using index = std::integral_constant<int, I>;
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f) {   // f(0), ... f(N - 1) with compile-time arguments
+    [&]<int... I>(std::integer_sequence<int, I...>) { (f(index<I>{}), ...); }(std::make_integer_sequence<int, N>{});
+}
+
+// `n` rows of K bytes from row `first`, as a buffer whose range ends with the last
+// row's last 16 bytes (nothing behind it is read).
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const int8_t* p, int64_t stride, int64_t first, int64_t n, int K) {
+    const uint32_t bytes = uint32_t((n - 1) * stride) + uint32_t((K + 15) & ~15);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p + first * stride), 0, bytes, 0x00020000);
+}
+// Its 16 bytes at voff + soff straight to LDS, lane by lane from `lds` on.
+__device__ __forceinline__ void buffer16_lds(__amdgpu_buffer_rsrc_t r, int8_t* lds, uint32_t voff, int soff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, voff, soff, 0, 0);
+}
+// A mask of 16 bytes, the first n kept.
+__device__ __forceinline__ v4i bytes_below(int n) {
+    v4i m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int left = n - 4 * i;
+        m[i] = left >= 4 ? -1 : left <= 0 ? 0 : (1 << (8 * left)) - 1;
+    }
+    return m;
+}
+
+template <class OT, bool GATED, int TT, int TC, int WT, int WC, int S, int R, int OCC>
+__global__ __launch_bounds__(64 * WT * WC, OCC) void lin8_tile_kernel(Lin8Args a, int tm, int tn) {
     constexpr int BK = 128, NT = 64 * WT * WC, M = GATED ? 2 : 1;
     constexpr int WTT = TT / WT, WTC = TC / WC;            // a wave's tokens and channels
     constexpr int NJ = WTT / 16, NI = WTC / 16;
-    constexpr int LT = TT * BK / 16 / NT, LC = TC * BK / 16 / NT;   // 16-byte loads of a thread
     constexpr int RPL = NT / 8;                            // rows of one load of all threads
-    __shared__ alignas(16) int8_t lds[2][(TT + M * TC) * BK];
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    constexpr int LT = (TT + RPL - 1) / RPL, LC = (TC + RPL - 1) / RPL;   // 16-byte loads of a thread
+    constexpr bool SPARE = TT % RPL || TC % RPL;           // the last ones of some waves bring nothing
+    static_assert(R <= NJ && NJ % R == 0 && S >= 2 && S <= 4);
+    // a variable for each stage: the compiler then sees that loads into one do not touch another
+    constexpr int STAGE = (TT + M * TC) * BK;
+    __shared__ alignas(16) int8_t lds0[STAGE], lds1[STAGE], lds2[S > 2 ? STAGE : 16], lds3[S > 3 ? STAGE : 16], spare[SPARE ? 1024 : 16];
+    const auto stage = [&](auto si) -> int8_t* {
+        constexpr int i = decltype(si)::value % S;
+        if constexpr (i == 0) return lds0;
+        else if constexpr (i == 1) return lds1;
+        else if constexpr (i == 2) return lds2;
+        else return lds3;
+    };
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, q = lane >> 4;
     const int wt = wv / WC, wc = wv % WC;
     int bm, bn;
     tile_of(blockIdx.x, tm, tn, bm, bn);
     const int64_t t0 = int64_t(bm) * TT, n0 = int64_t(bn) * TC;
-    const int8_t* xb = a.x + t0 * a.x_stride;
-    const int8_t* wb = a.w + n0 * a.w_stride;
-    const int8_t* ub = GATED ? a.up + n0 * a.w_stride : nullptr;
-    const int row = tid >> 3, chunk = tid & 7;
-    const int k16 = 16 * chunk;
+    // rows behind the last one are out of the buffers' range
+    const auto xr = rows_of(a.x, a.x_stride, t0, min(int64_t(TT), a.T - t0), a.K);
+    const auto wr = rows_of(a.w, a.w_stride, n0, min(int64_t(TC), a.N - n0), a.K);
+    const auto ur = rows_of(GATED ? a.up : a.w, a.w_stride, n0, min(int64_t(TC), a.N - n0), a.K);
+    // A load brings 8 rows of 128 bytes, lane by lane one behind the other in LDS; chunk p
+    // of row r lies at p ^ (r & 7), so that 16 rows of one chunk meet no bank twice.
+    const int row = tid >> 3, k16 = 16 * ((tid ^ row) & 7);
     uint32_t offt[LT], offc[LC];
 #pragma unroll
-    for (int i = 0; i < LT; ++i)
-        offt[i] = uint32_t(min(int64_t(row + i * RPL), int64_t(a.T) - 1 - t0)) * uint32_t(a.x_stride) + k16;
+    for (int i = 0; i < LT; ++i) offt[i] = uint32_t(row + i * RPL) * uint32_t(a.x_stride) + k16;
 #pragma unroll
     for (int i = 0; i < LC; ++i) {
         const int r = row + i * RPL, in = r % WTC, m = in & 15;   // LDS row r: tile in / 16 of wave r / WTC, row m
-        const int ch = r / WTC * WTC + 4 * NI * (m >> 2) + 4 * (in >> 4) + (m & 3);
-        offc[i] = uint32_t(min(int64_t(ch), int64_t(a.N) - 1 - n0)) * uint32_t(a.w_stride) + k16;
+        offc[i] = uint32_t(r / WTC * WTC + 4 * NI * (m >> 2) + 4 * (in >> 4) + (m & 3)) * uint32_t(a.w_stride) + k16;
     }
-    // chunk p of row r lies at p ^ (r & 7): 16 rows of one chunk meet no bank twice
-    const uint32_t put = uint32_t(row * BK + 16 * (chunk ^ (row & 7)));
-    v4i gt[LT], gc[LC], gu[M == 2 ? LC : 1];
-    const auto load = [&](int k) {
-        if (k + BK <= a.K) {
-#pragma unroll
-            for (int i = 0; i < LT; ++i) gt[i] = *reinterpret_cast<const v4i*>(xb + k + offt[i]);
-#pragma unroll
-            for (int i = 0; i < LC; ++i) gc[i] = *reinterpret_cast<const v4i*>(wb + k + offc[i]);
-            if constexpr (GATED)
-#pragma unroll
-                for (int i = 0; i < LC; ++i) gu[i] = *reinterpret_cast<const v4i*>(ub + k + offc[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < LT; ++i) gt[i] = row16(xb + offt[i] - k16, k + k16, a.K, true);
-#pragma unroll
-            for (int i = 0; i < LC; ++i) gc[i] = row16(wb + offc[i] - k16, k + k16, a.K, true);
-            if constexpr (GATED)
-#pragma unroll
-                for (int i = 0; i < LC; ++i) gu[i] = row16(ub + offc[i] - k16, k + k16, a.K, true);
-        }
-    };
-    const auto stage = [&](int8_t* b) {
-#pragma unroll
-        for (int i = 0; i < LT; ++i) *reinterpret_cast<v4i*>(b + put + i * RPL * BK) = gt[i];
-#pragma unroll
-        for (int i = 0; i < LC; ++i) *reinterpret_cast<v4i*>(b + TT * BK + put + i * RPL * BK) = gc[i];
-        if constexpr (GATED)
-#pragma unroll
-            for (int i = 0; i < LC; ++i) *reinterpret_cast<v4i*>(b + (TT + TC) * BK + put + i * RPL * BK) = gu[i];
+    const int steps = (a.K + BK - 1) / BK;
+    constexpr int L = LT + M * LC;
+    // Load i of stage `si`; behind the rows' end nothing is read, but the count stays.
+    const auto load = [&](auto si, auto ii, int s) {
+        constexpr int i = decltype(ii)::value, j = i < LT ? i : (i - LT) % LC, rows = i < LT ? TT : TC;
+        constexpr int part = i < LT ? 0 : i < LT + LC ? TT : TT + TC;
+        int8_t* b = stage(si) + (part + j * RPL + wv * 8) * BK;
+        const int k = s * BK;
+        uint32_t out = k + k16 < a.K ? 0u : 0x80000000u;
+        if constexpr ((j + 1) * RPL > rows)
+            if (j * RPL + wv * 8 >= rows) {
+                b = spare;
+                out = 0x80000000u;
+            }
+        if constexpr (i < LT) buffer16_lds(xr, b, offt[j] | out, k);
+        else if constexpr (i < LT + LC) buffer16_lds(wr, b, offc[j] | out, k);
+        else buffer16_lds(ur, b, offc[j] | out, k);
     };
     v4i acc[M][NI][NJ] = {};
+    v4i fw[2][M][NI], ft[R];
     const uint32_t gett = uint32_t((wt * WTT + c) * BK), getc = uint32_t((TT + wc * WTC + c) * BK);
-    const int steps = (a.K + BK - 1) / BK;
-    load(0);
-    stage(lds[0]);
-    if (steps > 1) load(BK);
-    __syncthreads();
-    for (int s = 0; s < steps; ++s) {
-        if (s + 1 < steps) stage(lds[(s + 1) & 1]);
-        if (s + 2 < steps) load((s + 2) * BK);
-        const int8_t* b = lds[s & 1];
+    const uint32_t at[2] = {uint32_t(16 * (q ^ (c & 7))), uint32_t(16 * ((4 + q) ^ (c & 7)))};
+    const auto weights = [&](auto hi, const int8_t* b) {   // of the step's half h
+        constexpr int h = decltype(hi)::value;
 #pragma unroll
-        for (int h = 0; h < BK / 64; ++h) {
-            const uint32_t at = 16 * ((4 * h + q) ^ (c & 7));
-            v4i fw[M][NI];
+        for (int m = 0; m < M; ++m)
 #pragma unroll
-            for (int m = 0; m < M; ++m)
+            for (int i = 0; i < NI; ++i) fw[h][m][i] = *reinterpret_cast<const v4i*>(b + getc + (m * TC + 16 * i) * BK + at[h]);
+    };
+    const auto tokens = [&](auto pi, const int8_t* b) {    // piece p: half p / NJ, token tile p % NJ
+        constexpr int p = decltype(pi)::value;
+        ft[p % R] = *reinterpret_cast<const v4i*>(b + gett + 16 * (p % NJ) * BK + at[p / NJ]);
+    };
+    const auto multiply = [&](auto pi) {
+        constexpr int p = decltype(pi)::value, h = p / NJ, j = p % NJ;
 #pragma unroll
-                for (int i = 0; i < NI; ++i) fw[m][i] = *reinterpret_cast<const v4i*>(b + getc + (m * TC + 16 * i) * BK + at);
+        for (int m = 0; m < M; ++m)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const v4i ft = *reinterpret_cast<const v4i*>(b + gett + 16 * j * BK + at);
+            for (int i = 0; i < NI; ++i)
+                acc[m][i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[h][m][i], ft[p % R], acc[m][i][j], 0, 0, 0);
+    };
+    // A step reads its 2 NJ pieces R ahead of their products; the last R products run
+    // after the barrier, over the next step's first reads. Its stage is loaded S - 1 steps
+    // ahead, into the one that every wave has read when the barrier before lets it pass;
+    // the loads lie between the products, as a wave that issues them in a row stands still
+    // until the memory pipeline has taken them.
+    const auto piece = [&](auto si, auto xi, int s) {
+        constexpr int x = decltype(xi)::value;
+        constexpr int from = std::min(L, x * L / NJ), to = std::min(L, (x + 1) * L / NJ);   // in the step's first half
+        each<to - from>([&](auto i) { load(index<si + S - 1>{}, index<from + i>{}, s + S - 1); });
+        __builtin_amdgcn_sched_barrier(0);   // the compiler would move each read to its use
+    };
+    const auto step = [&](auto si, int s) {
+        int8_t* b = stage(si);
+        if (s == steps - 1 && (a.K & (BK - 1))) {   // what lies behind a token's row counts as zeros
+            const v4i keep = bytes_below(a.K - s * BK - k16);
 #pragma unroll
-                for (int m = 0; m < M; ++m)
-#pragma unroll
-                    for (int i = 0; i < NI; ++i)
-                        acc[m][i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[m][i], ft, acc[m][i][j], 0, 0, 0);
-            }
+            for (int i = 0; i < LT; ++i)
+                if (TT % RPL == 0 || row + i * RPL < TT) *reinterpret_cast<v4i*>(b + tid * 16 + i * RPL * BK) &= keep;
+            lds_barrier();
         }
-        __syncthreads();
-    }
+        weights(index<0>{}, b);
+        each<R>([&](auto r) {
+            if (s > 0) multiply(index<2 * NJ - R + r>{});
+            tokens(index<r>{}, b);
+            piece(si, r, s);
+        });
+        each<2 * NJ - R>([&](auto p) {
+            if constexpr (p == NJ - R) weights(index<1>{}, b);
+            multiply(p);
+            tokens(index<p + R>{}, b);
+            piece(si, index<p + R>{}, s);
+        });
+        // this wave's part of the next stage is here, and its reads of this one are done
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm((S - 2) * L) & kLgkm0);
+        asm volatile("s_barrier" ::: "memory");
+    };
+    each<S - 1>([&](auto si) { each<L>([&](auto i) { load(si, i, si); }); });
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm((S - 2) * L));
+    asm volatile("s_barrier" ::: "memory");
+    for (int s = 0; s < steps; s += S) each<S>([&](auto si) { if (s + si < steps) step(si, s + si); });
+    each<R>([&](auto r) { multiply(index<2 * NJ - R + r>{}); });
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // no load writes LDS behind the workgroup's end
     const int64_t n = n0 + wc * WTC + 4 * NI * q;
     const int left = int(min(int64_t(4 * NI), int64_t(a.N) - n));
     float ws[M][4 * NI];
@@ -163,43 +230,294 @@ __global__ __launch_bounds__(64 * WT * WC, TT >= 256 ? 2 : 1) void lin8_tile_ker
         if (t >= a.T) continue;
         const float xs = a.x_scale[t];
         OT* o = static_cast<OT*>(a.out) + t * a.out_stride + n;
+        const auto put = [&](auto ei, auto ni) {   // channels e0 .. e0 + N - 1
+            constexpr int e0 = decltype(ei)::value, N = decltype(ni)::value;
+            float y[N];
 #pragma unroll
-        for (int i = 0; i < NI; i += 2) {
-            float y[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                y[e] = float(acc[0][i + e / 4][j][e & 3]) * xs * ws[0][4 * i + e];
-                if constexpr (GATED) y[e] = swiglu1(y[e], float(acc[1][i + e / 4][j][e & 3]) * xs * ws[1][4 * i + e], a.lim);
+            for (int e = 0; e < N; ++e) {
+                const int i = (e0 + e) / 4;
+                y[e] = float(acc[0][i][j][e & 3]) * xs * ws[0][e0 + e];
+                if constexpr (GATED) y[e] = swiglu1(y[e], float(acc[1][i][j][e & 3]) * xs * ws[1][e0 + e], a.lim);
             }
-            if (left > 4 * i) store8_rounded(o + 4 * i, left - 4 * i, y);
-        }
+            if (left > e0) store_rounded<OT, N>(o + e0, left - e0, y);
+        };
+        each<NI / 2>([&](auto i) { put(index<8 * i>{}, index<8>{}); });
+        if constexpr (NI % 2) put(index<4 * NI - 4>{}, index<4>{});
     }
 }
 
-template <class OT, bool GATED, int TT, int TC, int WT, int WC>
+// Four results of a token to an output of any type.
+__device__ __forceinline__ void store4(const Lin8Args& a, int64_t t, int64_t n, int left, const float (&y)[4]) {
+    const auto put = [&](auto* o) {
+        using OT = std::remove_pointer_t<decltype(o)>;
+        o += t * a.out_stride + n;
+        OT v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = rounded<OT>(y[e]);
+        if (left >= 4) {
+            __builtin_memcpy(o, v, sizeof v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+                if (e < left) o[e] = v[e];
+        }
+    };
+    if (a.out_type == kActF32) put(static_cast<float*>(a.out));
+    else if (a.out_type == kActF16) put(static_cast<f16*>(a.out));
+    else put(static_cast<bf16*>(a.out));
+}
+
+// Few tokens: 16 NJ of them and 16 NI channels (of each matrix) per workgroup. The
+// waves take the rows' 128-byte pieces in turn, each through a ring of U stages of its
+// own in LDS (no barrier; loads of whole 128-byte lines go straight there, as in the
+// tile kernel), and their sums are added in LDS at the end.
+// XT: type of x; other than int8, the one row of x is quantized into LDS by every
+// workgroup, while its first weights are on their way.
+template <int NI, int NJ, bool GATED, int XT, int NW, int U>
+__global__ __launch_bounds__(64 * NW) void lin8_rows_kernel(Lin8Args a) {
+    constexpr int M = GATED ? 2 : 1, NT = 64 * NW, BK = 128;
+    constexpr bool FUSED = XT != kActI8;
+    static_assert(!FUSED || NJ == 1);
+    static_assert(U >= 2 && U <= 4);
+    constexpr int XR = FUSED ? 0 : 16 * NJ;                     // rows of x in a stage, ahead of the weights'
+    constexpr int STAGE = (XR + M * NI * 16) * BK, L = STAGE / 1024;
+    __shared__ alignas(16) int8_t lds0[NW][STAGE], lds1[NW][STAGE], lds2[U > 2 ? NW : 1][U > 2 ? STAGE : 16], lds3[U > 3 ? NW : 1][U > 3 ? STAGE : 16];
+    static_assert(sizeof(lds0) >= size_t(NW) * M * NI * NJ * 1024, "the sums take the first stage's place");
+    extern __shared__ int8_t xq[];                              // FUSED: K rounded up to 128
+    __shared__ float red[16], scale1;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, q = lane >> 4;
+    const auto stage = [&](auto ui) -> int8_t* {
+        constexpr int u = decltype(ui)::value;
+        if constexpr (u == 0) return lds0[wv];
+        else if constexpr (u == 1) return lds1[wv];
+        else if constexpr (u == 2) return lds2[wv];
+        else return lds3[wv];
+    };
+    const int64_t t0 = int64_t(blockIdx.y) * (16 * NJ), n0 = int64_t(blockIdx.x) * (16 * NI);
+    const auto xr = rows_of(FUSED ? a.w : a.x, FUSED ? 16 : a.x_stride, FUSED ? 0 : t0, FUSED ? 1 : min(int64_t(16 * NJ), a.T - t0), FUSED ? 16 : a.K);
+    const auto wr = rows_of(a.w, a.w_stride, n0, min(int64_t(16 * NI), a.N - n0), a.K);
+    const auto ur = rows_of(GATED ? a.up : a.w, a.w_stride, n0, min(int64_t(16 * NI), a.N - n0), a.K);
+    // a load: 8 rows, chunk p of row r at p ^ (r & 7)
+    const int row = lane >> 3, k16 = 16 * ((lane ^ row) & 7);
+    const uint32_t offx = uint32_t(row) * uint32_t(a.x_stride) + k16, offw = uint32_t(row) * uint32_t(a.w_stride) + k16;
+    const auto load = [&](auto ui, int p) {   // behind the rows' end nothing is read, but the count stays
+        int8_t* b = stage(ui);
+        const int k = min(p * BK, a.K);
+        const uint32_t out = p * BK + k16 < a.K ? 0u : 0x80000000u;
+        if constexpr (!FUSED)
+#pragma unroll
+            for (int j = 0; j < 2 * NJ; ++j) buffer16_lds(xr, b + j * 1024, (offx + 8 * j * uint32_t(a.x_stride)) | out, k);
+#pragma unroll
+        for (int i = 0; i < 2 * NI; ++i) buffer16_lds(wr, b + XR * BK + i * 1024, (offw + 8 * i * uint32_t(a.w_stride)) | out, k);
+        if constexpr (GATED)
+#pragma unroll
+            for (int i = 0; i < 2 * NI; ++i) buffer16_lds(ur, b + (XR + 16 * NI) * BK + i * 1024, (offw + 8 * i * uint32_t(a.w_stride)) | out, k);
+    };
+    using XF = std::conditional_t<XT == kActF32, float, std::conditional_t<XT == kActF16, f16, bf16>>;
+    const XF* x = reinterpret_cast<const XF*>(a.x);
+    constexpr int FIRST = FUSED ? 2 : 1;
+    float first[FIRST][8];
+    if constexpr (FUSED)   // ahead of the weights, as loads are waited for in their order
+#pragma unroll
+        for (int i = 0; i < FIRST; ++i) load8(x + 8 * (tid + i * NT), a.K - 8 * (tid + i * NT), first[i]);
+    each<U>([&](auto u) { load(u, wv + u * NW); });
+    if constexpr (FUSED) {
+        float v[8], m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < FIRST; ++i) m = amax8(first[i], m);
+        for (int at = 8 * (tid + FIRST * NT); at < a.K; at += 8 * NT) {
+            load8(x + at, a.K - at, v);
+            m = amax8(v, m);
+        }
+        const float d = row_scale(group_join<true>(m, red), a.err);
+        if (tid == 0) scale1 = d;
+        const int end = (a.K + BK - 1) / BK * BK;
+#pragma unroll
+        for (int i = 0; i < FIRST; ++i)
+            if (8 * (tid + i * NT) < end) store_quants(xq + 8 * (tid + i * NT), first[i], d);
+        for (int at = 8 * (tid + FIRST * NT); at < end; at += 8 * NT) {
+            load8(x + at, a.K - at, v);
+            store_quants(xq + at, v, d);
+        }
+        lds_barrier();
+    }
+    v4i acc[M][NI][NJ] = {};
+    const int pieces = (a.K + BK - 1) / BK;
+    const uint32_t at[2] = {uint32_t(c * BK + 16 * (q ^ (c & 7))), uint32_t(c * BK + 16 * ((4 + q) ^ (c & 7)))};
+    const auto work = [&](auto ui, int p) {
+        const int8_t* b = stage(ui);
+        v4i fw[2][M][NI], fx[2][NJ];
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm((U - 1) * L));
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+                fx[h][j] = FUSED ? *reinterpret_cast<const v4i*>(xq + p * BK + 64 * h + 16 * q) : *reinterpret_cast<const v4i*>(b + 16 * j * BK + at[h]);
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+#pragma unroll
+                for (int i = 0; i < NI; ++i) fw[h][m][i] = *reinterpret_cast<const v4i*>(b + (XR + 16 * (m * NI + i)) * BK + at[h]);
+        }
+        __builtin_amdgcn_s_waitcnt(kLgkm0);   // read: the stage is free
+        asm volatile("" ::: "memory");
+        load(ui, p + U * NW);
+        if (!FUSED && p == pieces - 1 && (a.K & (BK - 1))) {   // what lies behind a token's row counts as zeros
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const v4i keep = bytes_below(a.K - p * BK - 64 * h - 16 * q);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) fx[h][j] &= keep;
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int m = 0; m < M; ++m)
+#pragma unroll
+                    for (int i = 0; i < NI; ++i)
+                        acc[m][i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[h][m][i], fx[h][j], acc[m][i][j], 0, 0, 0);
+    };
+    for (int p = wv; p < pieces; p += U * NW) each<U>([&](auto u) { if (p + u * NW < pieces) work(u, p + u * NW); });
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // no load is left to write into a stage
+    __syncthreads();
+    v4i* sums = reinterpret_cast<v4i*>(&lds0[0][0]);   // [wave][tile][lane]
+    constexpr int TILES = M * NI * NJ;
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) sums[(wv * TILES + (m * NI + i) * NJ + j) * 64 + lane] = acc[m][i][j];
+    __syncthreads();
+    // item: tile i, j and lane of its results
+    for (int it = tid; it < NI * NJ * 64; it += NT) {
+        const int tile = it >> 6, i = tile / NJ, j = tile % NJ;
+        const int64_t t = t0 + 16 * j + c, n = n0 + 16 * i + 4 * q;
+        if (t >= a.T || n >= a.N) continue;
+        v4i s[M];
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            s[m] = sums[(m * NI * NJ + tile) * 64 + lane];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) s[m] += sums[(w * TILES + m * NI * NJ + tile) * 64 + lane];
+        }
+        const int left = int(min(int64_t(4), int64_t(a.N) - n));
+        float xs;
+        if constexpr (FUSED) xs = scale1;
+        else xs = a.x_scale[t];
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int64_t r = n + min(e, left - 1);
+            y[e] = float(s[0][e]) * xs * a.w_scale[r];
+            if constexpr (GATED) y[e] = swiglu1(y[e], float(s[M - 1][e]) * xs * a.up_scale[r], a.lim);
+        }
+        store4(a, t, n, left, y);
+    }
+}
+
+template <class OT, bool GATED, int TT, int TC, int WT, int WC, int S, int R, int OCC>
 void lin8_tiles(const Lin8Args& a, hipStream_t s, hipEvent_t stop) {
     const int tm = (a.T + TT - 1) / TT, tn = (a.N + TC - 1) / TC;
-    hipExtLaunchKernelGGL((lin8_tile_kernel<OT, GATED, TT, TC, WT, WC>), dim3(tm * tn), dim3(64 * WT * WC), 0, s, nullptr, stop, 0, a, tm, tn);
+    hipExtLaunchKernelGGL((lin8_tile_kernel<OT, GATED, TT, TC, WT, WC, S, R, OCC>), dim3(tm * tn), dim3(64 * WT * WC), 0, s, nullptr, stop, 0, a, tm, tn);
+}
+
+template <int NI, int NJ, bool GATED, int XT, int NW, int U>
+void lin8_rows(const Lin8Args& a, hipStream_t s, hipEvent_t stop) {
+    const size_t lds = XT == kActI8 ? 0 : size_t((a.K + 127) & ~127);
+    hipExtLaunchKernelGGL((lin8_rows_kernel<NI, NJ, GATED, XT, NW, U>), dim3((a.N + 16 * NI - 1) / (16 * NI), (a.T + 16 * NJ - 1) / (16 * NJ)),
+                          dim3(64 * NW), lds, s, nullptr, stop, 0, a);
+}
+// The ways to run a call, in order of their tiles: tokens, channels (of each of one or
+// two matrices), workgroups that one CU holds, and the microseconds that they take:
+// fixed, and for each 128-byte step of K with the chip mostly idle and with a workgroup
+// on every CU. Fitted to 500 calls of 1 to 8192 tokens, 256 to 8192 k, 300 to 9216
+// channels, one and two matrices: the way of the least estimate is within 0.7 % of the
+// fastest one on average, 12 % at most (96 tokens, 5120 x (2 x 2304): 11.8 for 10.5 us).
+struct Way {
+    int tokens, one, two, per_cu;
+    float fixed, idle, busy;
+    bool rounds;   // workgroups run in whole rounds over the CUs; else they overlap
+};
+constexpr Way kWays[] = {
+    {16, 16, 16, 1, 3.1f, 0.040f, 0.089f, false},    // lin8_rows_kernel
+    {32, 16, 16, 1, 3.2f, 0.081f, 0.102f, false},
+    {32, 32, 16, 1, 3.3f, 0.098f, 0.158f, false},
+    {32, 64, 32, 1, 4.0f, 0.142f, 0.253f, false},
+    {64, 64, 32, 2, 3.9f, 0.255f, 0.605f, true},     // lin8_tile_kernel
+    {64, 128, 64, 1, 4.0f, 0.337f, 0.463f, true},
+    {128, 128, 64, 1, 5.4f, 0.431f, 0.626f, true},
+    {128, 160, 96, 1, 5.7f, 0.621f, 0.790f, true},
+    {128, 256, 128, 1, 5.7f, 0.790f, 1.006f, true},
+    {256, 160, 96, 1, 12.9f, 0.623f, 1.242f, true},
+    {256, 192, 96, 1, 5.8f, 1.239f, 1.247f, true},
+    {256, 256, 128, 1, 8.5f, 1.208f, 1.647f, true},
+};
+int lin8_way(const Lin8Args& a, int cus) {
+    if (a.x_type != kActI8) return 0;
+    int best = 0;
+    float least = 0.0f;
+    for (int i = 0; i < int(std::size(kWays)); ++i) {
+        const Way& w = kWays[i];
+        const int64_t ch = a.up ? w.two : w.one;
+        const float per = float(((a.T + w.tokens - 1) / w.tokens) * ((a.N + ch - 1) / ch)) / float(cus * w.per_cu);
+        const float step = std::max((w.rounds ? std::ceil(per) : std::max(per, 1.0f)) * w.idle, per * w.busy);
+        const float us = w.fixed + float((a.K + 127) / 128) * step;
+        if (i == 0 || us < least) {
+            best = i;
+            least = us;
+        }
+    }
+    return best;
 }
 
 template <class OT, bool GATED>
-void lin8_out(const Lin8Args& a, hipStream_t s, hipEvent_t stop) {
-    if (int64_t(a.T) * a.N >= 1024 * 1024 * 8) lin8_tiles<OT, GATED, 256, GATED ? 128 : 256, 2, 4>(a, s, stop);
-    else lin8_tiles<OT, GATED, 128, GATED ? 64 : 128, 2, 2>(a, s, stop);
+void lin8_tiled(const Lin8Args& a, int way, hipStream_t s, hipEvent_t stop) {
+    constexpr int G = GATED ? 2 : 1;
+    switch (way) {
+    case 4: return lin8_tiles<OT, GATED, 64, 64 / G, 4, 1, 4, 1, 2>(a, s, stop);
+    case 5: return lin8_tiles<OT, GATED, 64, 128 / G, 2, 4, 4, 2, 2>(a, s, stop);
+    case 6: return lin8_tiles<OT, GATED, 128, 128 / G, 4, 2, 4, 2, 2>(a, s, stop);
+    case 7: return lin8_tiles<OT, GATED, 128, GATED ? 96 : 160, 4, 2, GATED ? 3 : 4, 2, 2>(a, s, stop);
+    case 8: return lin8_tiles<OT, GATED, 128, 256 / G, 2, 4, 3, 4, 2>(a, s, stop);
+    case 9:
+        if constexpr (!GATED) return lin8_tiles<OT, GATED, 256, 160, 4, 2, 3, 4, 2>(a, s, stop);
+        else [[fallthrough]];   // 96 channels of each matrix either way
+    case 10: return lin8_tiles<OT, GATED, 256, 192 / G, 4, 2, 2, 4, 2>(a, s, stop);
+    default: return lin8_tiles<OT, GATED, 256, 256 / G, 2, 4, 2, 4, 2>(a, s, stop);
+    }
+}
+template <bool GATED>
+void lin8_run(const Lin8Args& a, int way, hipStream_t s, hipEvent_t stop) {
+    if (a.x_type == kActF32) return lin8_rows<1, 1, GATED, kActF32, 8, 2>(a, s, stop);
+    if (a.x_type == kActF16) return lin8_rows<1, 1, GATED, kActF16, 8, 2>(a, s, stop);
+    if (a.x_type == kActBF16) return lin8_rows<1, 1, GATED, kActBF16, 8, 2>(a, s, stop);
+    switch (way) {
+    case 0: return lin8_rows<1, 1, GATED, kActI8, 8, 2>(a, s, stop);
+    case 1: return lin8_rows<1, 2, GATED, kActI8, 4, GATED ? 2 : 3>(a, s, stop);
+    case 2: return lin8_rows<GATED ? 1 : 2, 2, GATED, kActI8, 8, 2>(a, s, stop);
+    case 3: return lin8_rows<GATED ? 2 : 4, 2, GATED, kActI8, 4, 3>(a, s, stop);
+    default: break;
+    }
+    if (a.out_type == kActF32) lin8_tiled<float, GATED>(a, way, s, stop);
+    else if (a.out_type == kActF16) lin8_tiled<f16, GATED>(a, way, s, stop);
+    else lin8_tiled<bf16, GATED>(a, way, s, stop);
 }
 
 }  // namespace
 
 hipError_t launch_lin8(const Lin8Args& a, int cus, hipStream_t s, hipEvent_t stop) {
-    if (a.T < 1 || a.T > kLinMaxT || a.N < 1 || a.K < 1 || a.K > kLinMaxK || a.x_stride % 16 || a.w_stride % 16)
+    if (a.T < 1 || a.T > kLinMaxT || a.N < 1 || a.K < 1 || a.K > kLinMaxK || a.w_stride % 16 ||
+        (a.x_type == kActI8 ? a.x_stride % 16 != 0 : !lin8_quantizes(a.T, a.K)))
         return hipErrorInvalidValue;
-    (void)cus;
-    switch (a.out_type) {
-    case kActF32: a.up ? lin8_out<float, true>(a, s, stop) : lin8_out<float, false>(a, s, stop); break;
-    case kActF16: a.up ? lin8_out<f16, true>(a, s, stop) : lin8_out<f16, false>(a, s, stop); break;
-    case kActBF16: a.up ? lin8_out<bf16, true>(a, s, stop) : lin8_out<bf16, false>(a, s, stop); break;
-    default: return hipErrorInvalidValue;
-    }
+    if (a.out_type < kActF32 || a.out_type > kActBF16) return hipErrorInvalidValue;
+    const int way = lin8_way(a, cus);
+    if (a.up) lin8_run<true>(a, way, s, stop);
+    else lin8_run<false>(a, way, s, stop);
     return hipGetLastError();
 }
 

@@ -21,28 +21,6 @@
 namespace xl::dev {
 namespace {
 
-// A row's scale from its largest magnitude (infinite where a value is not
-// finite: the device flag, and a NaN).
-__device__ __forceinline__ float row_scale(float amax, int* err) {
-    if (amax <= 3.402823466e38f) return __fdiv_rn(amax, 127.0f);
-    if (threadIdx.x == 0) atomicOr(err, kDevErrNonFinite);
-    return __int_as_float(0x7fc00000);
-}
-__device__ __forceinline__ float amax8(const float (&v)[8], float m) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float a = fabsf(v[i]);
-        m = a <= 3.402823466e38f ? fmaxf(m, a) : __int_as_float(0x7f800000);   // a NaN fails the comparison too
-    }
-    return m;
-}
-// Eight quants at q[0..7]; those past the row (n..7) are zeros, written up to
-// the next multiple of 16 bytes by whichever thread owns them.
-__device__ __forceinline__ void store_quants(int8_t* q, const float (&v)[8], float d) {
-    uint32_t o[2] = {quant4(v, d), quant4(v + 4, d)};
-    __builtin_memcpy(q, o, 8);
-}
-
 template <class T, class RT, int R>
 __global__ __launch_bounds__(1024) void block_norm_kernel(BlockNormArgs a) {
     __shared__ float red[4][16];

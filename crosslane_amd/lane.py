@@ -221,36 +221,55 @@ def linear_i8_work_bytes(T: int, K: int, N: int, gated: bool = False) -> int:
     return int(lib().xl_linear_i8_work_bytes(T, K, N, int(gated)))
 
 
-# Element types of the calls around a block (XL_F32 ... by the tensor's dtype)
-_ACT = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2, "torch.int8": 3}
 SCORES = {"softmax": 0, "sigmoid": 1}
 
 
-def _arg(ok: bool, message: str) -> None:
-    if not ok:
-        raise XLError(1, message)
+class _Kinds(dict):
+    """Element types of the calls around a block (XL_F32 ..., 4: int32 vectors) by
+    torch dtype; looked up by name once each, torch itself is not imported here."""
+    NAMES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2, "torch.int8": 3, "torch.int32": 4}
+
+    def __missing__(self, dtype) -> int:
+        kind = self[dtype] = self.NAMES.get(str(dtype), -1)
+        return kind
 
 
-def _act(t, what: str, allowed=(0, 1, 2)) -> int:
-    a = _ACT.get(str(t.dtype), -1)
-    _arg(a in allowed, f"{what}: element type {t.dtype} not taken here")
-    return a
+_KINDS = _Kinds()
+_INT8, _INT32 = 3, 4
+
+
+# The checks below run before every launch of a decode loop: no message is built
+# and no attribute read that a passing call does not need.
+def _refuse(message: str):
+    raise XLError(1, message)
+
+
+def _act(t, what: str) -> int:
+    kind = _KINDS[t.dtype]
+    if not 0 <= kind < _INT8:
+        _refuse(f"{what}: element type {t.dtype} not taken here")
+    return kind
 
 
 def _rows(t, what: str, shape=None) -> int:
     """A [T, n] matrix of contiguous rows on the GPU; returns its row stride."""
-    _arg(t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1), f"{what}: a matrix of contiguous rows is wanted")
-    _arg(t.is_cuda, f"{what}: not on the GPU")
-    _arg(shape is None or tuple(t.shape) == tuple(shape), f"{what}: shape {tuple(t.shape)} where {shape} is wanted")
-    return int(t.stride(0)) if t.shape[0] > 1 else max(int(t.stride(0)), int(t.shape[1]))
+    sh, st = t.shape, t.stride()
+    if len(sh) != 2 or (st[1] != 1 and sh[1] != 1):
+        _refuse(f"{what}: a matrix of contiguous rows is wanted")
+    if not t.is_cuda:
+        _refuse(f"{what}: not on the GPU")
+    if shape is not None and sh != shape:
+        _refuse(f"{what}: shape {tuple(sh)} where {tuple(shape)} is wanted")
+    return st[0] if sh[0] > 1 else max(st[0], sh[1])
 
 
-def _vec(t, n: int, what: str, dtype: str = "torch.float32"):
-    """A contiguous GPU vector of n values (None passes)."""
-    if t is not None:
-        _arg(t.is_cuda and t.is_contiguous() and t.numel() == n and str(t.dtype) == dtype,
-             f"{what}: {n} contiguous {dtype} values on the GPU are wanted")
-    return t
+def _vec(t, n: int, what: str, kind: int = 0):
+    """The address of a contiguous GPU vector of n values (None passes)."""
+    if t is None:
+        return None
+    if not (t.is_cuda and t.is_contiguous() and t.numel() == n and _KINDS[t.dtype] == kind):
+        _refuse(f"{what}: {n} contiguous values of the right type on the GPU are wanted")
+    return t.data_ptr()
 
 
 def pack_types(pack_dir: str, first_layer: int, n_layers: int, n_experts: int) -> np.ndarray:
@@ -581,13 +600,13 @@ class Lane:
         masks an expert), bias [n] float32 added to the scores for the choice only,
         `top_groups` of `groups` expert groups by the sum of their `group_keys`
         largest keys; ids (int32) and w [T, k]."""
-        _arg(score in SCORES, f"score must be one of {sorted(SCORES)}")
+        if score not in SCORES:
+            _refuse(f"score must be one of {sorted(SCORES)}")
         stride = _rows(logits, "logits")
-        T, n = (int(v) for v in logits.shape)
-        _vec(ids, T * k, "ids", "torch.int32"), _vec(w, T * k, "w"), _vec(bias, n, "bias")
-        self._call("xl_route_scored_async", _ptr(logits), _act(logits, "logits"), T, stride, _ptr(bias), n, SCORES[score],
-                   groups, top_groups, group_keys, k, int(renorm), float(scale), _ptr(ids), _ptr(w),
-                   None if stream is None else int(stream))
+        T, n = logits.shape
+        self._call("xl_route_scored_async", logits.data_ptr(), _act(logits, "logits"), T, stride, _vec(bias, n, "bias"), n,
+                   SCORES[score], groups, top_groups, group_keys, int(k), bool(renorm), float(scale), _vec(ids, T * k, "ids", _INT32),
+                   _vec(w, T * k, "w"), None if stream is None else int(stream))
 
     def block_norm_async(self, res, y=None, post_w=None, gate=None, alpha: float = 1.0, pre_w=None, eps: float = 1e-6,
                          res_out=None, x=None, q=None, q_scale=None, stream=None) -> None:
@@ -596,37 +615,60 @@ class Lane:
         gate [T, D], [D] or None; outputs res_out (r, as res), x (as y) [T, D], and q
         int8 [T, D] with q_scale [T]: x quantized, for linear_i8_async."""
         some = y if res is None else res
-        _arg(some is not None, "res or y is wanted")
-        T, D = (int(v) for v in some.shape)
-        shape = (T, D)
-        st = {n: 0 if t is None else _rows(t, n, shape)
-              for n, t in (("y", y), ("res", res), ("res_out", res_out), ("x", x), ("q", q))}
-        gs = 0
-        if gate is not None and gate.dim() == 1:
-            _vec(gate, D, "gate", str(gate.dtype))
-        elif gate is not None:
-            gs = _rows(gate, "gate", shape)
-        act = [t for t in (y, x, gate) if t is not None]
-        streams = [t for t in (res, res_out) if t is not None]
-        kinds = {_act(t, "y, x and gate") for t in act}, {_act(t, "res and res_out") for t in streams}
-        _arg(len(kinds[0]) <= 1 and len(kinds[1]) <= 1, "y, x and gate have one element type, res and res_out one")
-        _arg(q is None or str(q.dtype) == "torch.int8", "q must be int8")
-        _vec(post_w, D, "post_w"), _vec(pre_w, D, "pre_w"), _vec(q_scale, T, "q_scale")
-        rt = kinds[1].pop() if kinds[1] else 0
-        self._call("xl_block_norm_async", _ptr(y), st["y"], _ptr(res), st["res"], _ptr(gate), gs, _ptr(post_w),
-                   _ptr(pre_w), T, D, kinds[0].pop() if kinds[0] else rt, rt, float(alpha), float(eps), _ptr(res_out),
-                   st["res_out"], _ptr(x), st["x"], _ptr(q), st["q"], _ptr(q_scale),
-                   None if stream is None else int(stream))
+        if some is None:
+            _refuse("res or y is wanted")
+        shape = some.shape
+        if len(shape) != 2:
+            _refuse("res and y: a matrix of contiguous rows is wanted")
+        T, D = shape
+        kind = rkind = -1
+        at = []   # address and row stride of each matrix
+        for t, what in ((y, "y"), (x, "x")):
+            if t is None:
+                at += (None, 0)
+                continue
+            at += (t.data_ptr(), _rows(t, what, shape))
+            k = _act(t, what)
+            if kind not in (-1, k):
+                _refuse("y, x and gate have one element type, res and res_out one")
+            kind = k
+        for t, what in ((res, "res"), (res_out, "res_out")):
+            if t is None:
+                at += (None, 0)
+                continue
+            at += (t.data_ptr(), _rows(t, what, shape))
+            k = _act(t, what)
+            if rkind not in (-1, k):
+                _refuse("y, x and gate have one element type, res and res_out one")
+            rkind = k
+        gp, gs = None, 0
+        if gate is not None:
+            k = _act(gate, "gate")
+            if kind not in (-1, k):
+                _refuse("y, x and gate have one element type, res and res_out one")
+            kind = k
+            if gate.dim() == 1:
+                gp = _vec(gate, D, "gate", k)
+            else:
+                gp, gs = gate.data_ptr(), _rows(gate, "gate", shape)
+        qp, qs = None, 0
+        if q is not None:
+            if _KINDS[q.dtype] != _INT8:
+                _refuse("q must be int8")
+            qp, qs = q.data_ptr(), _rows(q, "q", shape)
+        rkind = max(rkind, 0)
+        self._call("xl_block_norm_async", at[0], at[1], at[4], at[5], gp, gs, _vec(post_w, D, "post_w"),
+                   _vec(pre_w, D, "pre_w"), T, D, kind if kind >= 0 else rkind, rkind, float(alpha), float(eps), at[6], at[7], at[2], at[3],
+                   qp, qs, _vec(q_scale, T, "q_scale"), None if stream is None else int(stream))
 
     def quantize_rows_async(self, x, q, scale, stream=None) -> None:
         """x [T, K] (f32, f16 or bf16) to int8 q [T, K] (16-byte aligned rows) with scale [T]."""
-        stride = _rows(x, "x")
-        T, K = (int(v) for v in x.shape)
-        qs = _rows(q, "q", (T, K))
-        _arg(str(q.dtype) == "torch.int8", "q must be int8")
-        _vec(scale, T, "scale")
-        self._call("xl_quantize_rows_async", _ptr(x), _act(x, "x"), T, K, stride, _ptr(q), qs, _ptr(scale),
-                   None if stream is None else int(stream))
+        stride, shape = _rows(x, "x"), x.shape
+        qs = _rows(q, "q", shape)
+        if _KINDS[q.dtype] != _INT8:
+            _refuse("q must be int8")
+        self._call("xl_quantize_rows_async", x.data_ptr(), _act(x, "x"), shape[0], shape[1], stride, q.data_ptr(), qs,
+                   _vec(scale, shape[0], "scale"), None if stream is None else int(stream))
 
     def linear_i8_async(self, x, w, w_scale, out, x_scale=None, up=None, up_scale=None, limit: float = 0.0, work=None,
                         stream=None) -> None:
@@ -635,17 +677,23 @@ class Lane:
         the call). With up, up_scale: SwiGLU of the products with w (gate) and up.
         work: linear_i8_work_bytes(T, K, N, gated) bytes."""
         xs, ws = _rows(x, "x"), _rows(w, "w")
-        T, K = (int(v) for v in x.shape)
-        N = int(w.shape[0])
-        _arg(int(w.shape[1]) == K and str(w.dtype) == "torch.int8", "w: int8 [N, K] is wanted")
+        T, K = x.shape
+        shape = w.shape
+        N = shape[0]
+        if shape[1] != K or _KINDS[w.dtype] != _INT8:
+            _refuse("w: int8 [N, K] is wanted")
         os_ = _rows(out, "out", (T, N))
-        if up is not None:
-            _arg(str(up.dtype) == "torch.int8" and _rows(up, "up", (N, K)) == ws, "up: int8 with w's shape and stride is wanted")
-        _vec(x_scale, T, "x_scale"), _vec(w_scale, N, "w_scale"), _vec(up_scale, N, "up_scale")
-        _arg(work is not None and work.is_cuda and work.is_contiguous(), "work: a contiguous GPU buffer is wanted")
-        self._call("xl_linear_i8_async", _ptr(x), _act(x, "x", (0, 1, 2, 3)), _ptr(x_scale), xs, T, K, _ptr(w),
-                   _ptr(w_scale), _ptr(up), _ptr(up_scale), ws, N, float(limit), _ptr(out), _act(out, "out"), os_,
-                   _ptr(work), int(work.numel() * work.element_size()), None if stream is None else int(stream))
+        if up is not None and (_KINDS[up.dtype] != _INT8 or _rows(up, "up", shape) != ws):
+            _refuse("up: int8 with w's shape and stride is wanted")
+        if work is None or not (work.is_cuda and work.is_contiguous()):
+            _refuse("work: a contiguous GPU buffer is wanted")
+        kind = _KINDS[x.dtype]
+        if not 0 <= kind <= _INT8:
+            _refuse(f"x: element type {x.dtype} not taken here")
+        self._call("xl_linear_i8_async", x.data_ptr(), kind, _vec(x_scale, T, "x_scale"), xs, T, K, w.data_ptr(),
+                   _vec(w_scale, N, "w_scale"), None if up is None else up.data_ptr(), _vec(up_scale, N, "up_scale"), ws, N,
+                   float(limit), out.data_ptr(), _act(out, "out"), os_, work.data_ptr(), work.numel() * work.element_size(),
+                   None if stream is None else int(stream))
 
     def swiglu_async(self, g, u, h, limit: float = 0.0, stream=None) -> None:
         self._call("xl_swiglu_async", _ptr(g), _ptr(u), int(g.numel()), float(limit), _ptr(h),
