@@ -13,21 +13,29 @@ namespace xl::dev {
 typedef _Float16 f16;
 typedef __bf16 bf16;
 
-// Eight consecutive values of a row as float32, `n` of them in the row (the
-// others 0). Rows start at any element: the loads are wide and unaligned (the
-// hardware takes dword loads at any byte), so odd widths and strides go the
-// same way as aligned ones.
+// Eight consecutive values of a row, `n` of them in the row (the others 0). Rows start
+// at any element: the loads are wide and unaligned (the hardware takes dword loads at
+// any byte), so odd widths and strides go the same way as aligned ones.
 template <class T>
-__device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
+struct Eight {
+    T v[8];
+};
+template <class T>
+__device__ __forceinline__ Eight<T> eight(const T* p, int n) {
+    Eight<T> r;
     if (n >= 8) {
-        T t[8];
-        __builtin_memcpy(t, p, sizeof t);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = float(t[i]);
+        __builtin_memcpy(&r, p, sizeof r);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? float(p[i]) : 0.0f;
+        for (int i = 0; i < 8; ++i) r.v[i] = i < n ? p[i] : T(0.0f);
     }
+    return r;
+}
+template <class T>
+__device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
+    const Eight<T> r = eight(p, n);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = float(r.v[i]);
 }
 // The same to memory, each value rounded once (to nearest, ties to even).
 template <class T>

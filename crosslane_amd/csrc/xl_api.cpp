@@ -1861,7 +1861,7 @@ int32_t xl_route_scored_async(xl_context* ctx, const void* d_logits, int32_t log
         hipStream_t s = pick_stream(ctx, stream);
         Ordered ord(ctx, s);
         const xl::ScoreArgs a{d_logits, d_bias_or_null, stride, logits_type, T, n, k, score == XL_SCORE_SIGMOID, n_groups,
-                              top_groups, group_keys, renorm != 0, scale, d_ids, d_w, ctx->err_flag};
+                              top_groups, group_keys, renorm != 0, scale, d_ids, d_w, ctx->err_flag, 0, 0};
         hip_check(xl::dev::launch_score_route(a, s, ord.stop()), "scored route launch");
         ord.carried_by_launch(true);   // the launch records the ordering event itself
     });
@@ -1919,7 +1919,7 @@ int32_t xl_block_norm_async(xl_context* ctx, const void* d_y_or_null, int64_t y_
                                   d_res_out_or_null, d_x_or_null, d_q_or_null, d_q_scale_or_null, y_stride, res_stride,
                                   gate_stride, res_out_stride, x_stride, q_stride, T, D, type, res_type, alpha, eps,
                                   ctx->err_flag};
-        hip_check(xl::dev::launch_block_norm(a, s, ord.stop()), "block norm launch");
+        hip_check(xl::dev::launch_block_norm(a, ctx->cus, s, ord.stop()), "block norm launch");
         ord.carried_by_launch(true);   // the launch records the ordering event itself
     });
 }
@@ -1993,7 +1993,8 @@ int32_t xl_linear_i8_async(xl_context* ctx, const void* d_x, int32_t x_type, con
         if (x_type != XL_I8 && !xl::lin8_quantizes(T, K)) {
             int8_t* q = static_cast<int8_t*>(d_work);
             float* scale = reinterpret_cast<float*>(q + lw.scale);
-            hip_check(xl::dev::launch_quant_rows(d_x, x_type, x_stride, T, K, q, lw.stride, scale, ctx->err_flag, s, nullptr),
+            // both launches carry the event: a launch without one after it costs 2 us more
+            hip_check(xl::dev::launch_quant_rows(d_x, x_type, x_stride, T, K, q, lw.stride, scale, ctx->err_flag, s, ord.stop()),
                       "row quantization launch");
             a.x = q;
             a.x_scale = scale;

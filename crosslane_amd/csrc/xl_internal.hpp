@@ -211,6 +211,7 @@ struct ScoreArgs {
     int32_t* ids;
     float* w;
     int* err;
+    int size, run;              // a group's experts; log2 of its lanes (set by the launch)
 };
 // int8 product (xl_lin8.hip): out[t][r] = (sum_k x[t][k] w[r][k]) * x_scale[t] *
 // w_scale[r], or SwiGLU of two such products (up set).
@@ -349,7 +350,7 @@ constexpr int kFfnTokensMin = 3;
 hipError_t launch_ffn_tokens(const MatRef& gate, const MatRef& up, const MatRef& down, int T, int dim, int ff,
                              const float* x, float* out, int8_t* xq, float* xd, int8_t* hq, float* hd, float lim,
                              int* err, int cus, hipStream_t s);
-hipError_t launch_block_norm(const BlockNormArgs& a, hipStream_t s, hipEvent_t stop);
+hipError_t launch_block_norm(const BlockNormArgs& a, int cus, hipStream_t s, hipEvent_t stop);
 // Rows of x (type f32, f16 or bf16) to int8 with a scale each; the bytes from K
 // to the next multiple of 16 are zeroed.
 hipError_t launch_quant_rows(const void* x, int type, int64_t x_stride, int T, int K, int8_t* q, int64_t q_stride,

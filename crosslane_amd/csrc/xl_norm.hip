@@ -21,92 +21,117 @@
 namespace xl::dev {
 namespace {
 
-template <class T, class RT, int R>
+// A workgroup takes rows blockIdx.x, + gridDim.x, ...: with a row for each (few rows)
+// or with several, the next row's loads on their way while this one is reduced and
+// stored, and the vectors over the channels (post_w, pre_w, a gate for all) kept in
+// registers, where one row for each workgroup would read as many bytes of them from L2
+// as of the row itself. KEEP: registers allow that (rows of up to 8192 values, of 16384
+// in 16 bits); else a row's loads follow the row before.
+template <class T, class RT, int R, bool KEEP>
 __global__ __launch_bounds__(1024) void block_norm_kernel(BlockNormArgs a) {
-    __shared__ float red[4][16];
-    const int64_t t = blockIdx.x;
+    __shared__ float red[2][3][16];
     const int NT = blockDim.x, D = a.D;
-    float v[R][8], r[R][8];
     int at[R];
 #pragma unroll
     for (int j = 0; j < R; ++j) at[j] = 8 * (int(threadIdx.x) + j * NT);
-    const T* y = static_cast<const T*>(a.y) + t * a.y_stride;
-    const RT* res = static_cast<const RT*>(a.res) + t * a.res_stride;
-    const T* gate = static_cast<const T*>(a.gate) + t * a.gate_stride;
+    const bool one_gate = a.gate && a.gate_stride == 0;
+    float post[KEEP ? R : 1][8], pre[KEEP ? R : 1][8];
+    Eight<T> gate[R], y[R];
+    Eight<RT> res[R];
+    const auto fetch = [&](int64_t t) {
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
-        if (a.res) load8(res + at[j], D - at[j], r[j]);
-        else
-            for (int i = 0; i < 8; ++i) r[j][i] = 0.0f;
-        if (a.y) load8(y + at[j], D - at[j], v[j]);
+        for (int j = 0; j < R; ++j) {
+            if (a.y) y[j] = eight(static_cast<const T*>(a.y) + t * a.y_stride + at[j], D - at[j]);
+            if (a.res) res[j] = eight(static_cast<const RT*>(a.res) + t * a.res_stride + at[j], D - at[j]);
+            if (a.gate && !one_gate) gate[j] = eight(static_cast<const T*>(a.gate) + t * a.gate_stride + at[j], D - at[j]);
+        }
+    };
+    int64_t t = blockIdx.x;
+    const auto of_channels = [&](int j) {
+        if (a.post_w) load8(a.post_w + at[j], D - at[j], post[KEEP ? j : 0]);
+        if (one_gate) gate[j] = eight(static_cast<const T*>(a.gate) + at[j], D - at[j]);
+    };
+    const auto before_next = [&](int j) { load8(a.pre_w + at[j], D - at[j], pre[KEEP ? j : 0]); };
+    if (KEEP) {
+        fetch(t);
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            of_channels(j);
+            if (a.pre_w) before_next(j);
+        }
     }
-    if (a.y) {
-        float inv = 1.0f;
-        if (a.post_w) {
-            float ss = 0.0f;
+    for (int turn = 0; t < a.T; turn ^= 1) {
+        if (!KEEP) fetch(t);
+        float r[R][8];
+        if (a.y) {
+            float v[R][8], inv = 1.0f;
 #pragma unroll
             for (int j = 0; j < R; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) ss = fmaf(v[j][i], v[j][i], ss);
-            inv = 1.0f / sqrtf(group_join<false>(ss, red[0]) / float(D) + a.eps);
-        }
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            float w[8];
+                for (int i = 0; i < 8; ++i) v[j][i] = float(y[j].v[i]);
             if (a.post_w) {
-                load8(a.post_w + at[j], D - at[j], w);
+                float ss = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[j][i] = v[j][i] * inv * w[i];
-            }
-            if (a.gate) {
-                load8(gate + at[j], D - at[j], w);
+                for (int j = 0; j < R; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[j][i] *= w[i];
+                    for (int i = 0; i < 8; ++i) ss = fmaf(v[j][i], v[j][i], ss);
+                inv = 1.0f / sqrtf(group_join<false>(ss, red[turn][0]) / float(D) + a.eps);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) r[j][i] = fmaf(a.alpha, r[j][i], v[j][i]);
+            for (int j = 0; j < R; ++j) {
+                if (!KEEP) of_channels(j);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float w = v[j][i];
+                    if (a.post_w) w = w * inv * post[KEEP ? j : 0][i];
+                    if (a.gate) w *= float(gate[j].v[i]);
+                    r[j][i] = a.res ? fmaf(a.alpha, float(res[j].v[i]), w) : w;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < R; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) r[j][i] = a.alpha * float(res[j].v[i]);
         }
-    } else {
+        const int64_t now = t;
+        t += gridDim.x;
+        if (KEEP && t < a.T) fetch(t);
+        if (a.res_out) {
+            RT* o = static_cast<RT*>(a.res_out) + now * a.res_out_stride;
+#pragma unroll
+            for (int j = 0; j < R; ++j) store8(o + at[j], D - at[j], r[j]);
+        }
+        if (!a.pre_w) continue;
+        float ss = 0.0f;
 #pragma unroll
         for (int j = 0; j < R; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) r[j][i] *= a.alpha;
+            for (int i = 0; i < 8; ++i) ss = fmaf(r[j][i], r[j][i], ss);
+        const float inv = 1.0f / sqrtf(group_join<false>(ss, red[turn][1]) / float(D) + a.eps);
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            if (!KEEP) before_next(j);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r[j][i] = r[j][i] * inv * pre[KEEP ? j : 0][i];
+        }
+        if (a.x) {
+            T* o = static_cast<T*>(a.x) + now * a.x_stride;
+#pragma unroll
+            for (int j = 0; j < R; ++j) store8(o + at[j], D - at[j], r[j]);
+        }
+        if (!a.q) continue;
+        float m = 0.0f;
+#pragma unroll
+        for (int j = 0; j < R; ++j) m = amax8(r[j], m);
+        const float d = row_scale(group_join<true>(m, red[turn][2]), a.err);
+        if (threadIdx.x == 0) a.q_scale[now] = d;
+        int8_t* q = a.q + now * a.q_stride;
+        const int end = (D + 15) & ~15;   // the quants' row ends with zeros to a multiple of 16
+#pragma unroll
+        for (int j = 0; j < R; ++j)
+            if (at[j] < end) store_quants(q + at[j], r[j], d);
     }
-    if (a.res_out) {
-        RT* o = static_cast<RT*>(a.res_out) + t * a.res_out_stride;
-#pragma unroll
-        for (int j = 0; j < R; ++j) store8(o + at[j], D - at[j], r[j]);
-    }
-    if (!a.pre_w) return;
-    float ss = 0.0f;
-#pragma unroll
-    for (int j = 0; j < R; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(r[j][i], r[j][i], ss);
-    const float inv = 1.0f / sqrtf(group_join<false>(ss, red[1]) / float(D) + a.eps);
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-        float w[8];
-        load8(a.pre_w + at[j], D - at[j], w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r[j][i] = r[j][i] * inv * w[i];
-    }
-    if (a.x) {
-        T* o = static_cast<T*>(a.x) + t * a.x_stride;
-#pragma unroll
-        for (int j = 0; j < R; ++j) store8(o + at[j], D - at[j], r[j]);
-    }
-    if (!a.q) return;
-    float m = 0.0f;
-#pragma unroll
-    for (int j = 0; j < R; ++j) m = amax8(r[j], m);
-    const float d = row_scale(group_join<true>(m, red[2]), a.err);
-    if (threadIdx.x == 0) a.q_scale[t] = d;
-    int8_t* q = a.q + t * a.q_stride;
-    const int end = (D + 15) & ~15;   // the quants' row ends with zeros to a multiple of 16
-#pragma unroll
-    for (int j = 0; j < R; ++j)
-        if (at[j] < end) store_quants(q + at[j], r[j], d);
 }
 
 // Rows to int8 with a scale each. R > 0: the row in registers; R == 0: rows of
@@ -157,22 +182,26 @@ __global__ __launch_bounds__(1024) void quant_rows_kernel(const T* __restrict__ 
 int row_threads(int n, int per) { return std::min(1024, ((n + per - 1) / per + 63) / 64 * 64); }
 
 template <class T, class RT>
-hipError_t norm_types(const BlockNormArgs& a, hipStream_t s, hipEvent_t stop) {
+hipError_t norm_types(const BlockNormArgs& a, int cus, hipStream_t s, hipEvent_t stop) {
     const int chunks = (a.D + 7) / 8;   // at most 4096
     const auto go = [&](auto kernel, int per) {
-        hipExtLaunchKernelGGL(kernel, dim3(a.T), dim3(row_threads(chunks, per)), 0, s, nullptr, stop, 0, a);
+        const int threads = row_threads(chunks, per);
+        // as many workgroups as the CUs hold at a time (24 waves of up to 81 registers): 8192 x
+        // 5120 bf16 in 77 us, with 16 waves 109, with a workgroup for each row 106
+        const int many = cus * std::max(1, 24 * 64 / threads);
+        hipExtLaunchKernelGGL(kernel, dim3(std::min(a.T, many)), dim3(threads), 0, s, nullptr, stop, 0, a);
     };
-    if (chunks <= 1024) go(block_norm_kernel<T, RT, 1>, 1);
-    else if (chunks <= 2048) go(block_norm_kernel<T, RT, 2>, 2);
-    else go(block_norm_kernel<T, RT, 4>, 4);
+    if (chunks <= 1024) go(block_norm_kernel<T, RT, 1, true>, 1);
+    else if (chunks <= 2048) go(block_norm_kernel<T, RT, 2, sizeof(T) + sizeof(RT) <= 4>, 2);
+    else go(block_norm_kernel<T, RT, 4, false>, 4);
     return hipGetLastError();
 }
 template <class T>
-hipError_t norm_type(const BlockNormArgs& a, hipStream_t s, hipEvent_t stop) {
+hipError_t norm_type(const BlockNormArgs& a, int cus, hipStream_t s, hipEvent_t stop) {
     switch (a.res_type) {
-    case kActF32: return norm_types<T, float>(a, s, stop);
-    case kActF16: return norm_types<T, f16>(a, s, stop);
-    case kActBF16: return norm_types<T, bf16>(a, s, stop);
+    case kActF32: return norm_types<T, float>(a, cus, s, stop);
+    case kActF16: return norm_types<T, f16>(a, cus, s, stop);
+    case kActBF16: return norm_types<T, bf16>(a, cus, s, stop);
     default: return hipErrorInvalidValue;
     }
 }
@@ -192,13 +221,13 @@ hipError_t quant_type(const void* x, int64_t x_stride, int T_, int K, int8_t* q,
 
 }  // namespace
 
-hipError_t launch_block_norm(const BlockNormArgs& a, hipStream_t s, hipEvent_t stop) {
+hipError_t launch_block_norm(const BlockNormArgs& a, int cus, hipStream_t s, hipEvent_t stop) {
     if (a.D < 1 || a.D > kNormMaxDim || a.T < 1 || (a.res_out && !a.y && !a.res) || (a.q && !a.pre_w) || (a.x && !a.pre_w))
         return hipErrorInvalidValue;
     switch (a.type) {
-    case kActF32: return norm_type<float>(a, s, stop);
-    case kActF16: return norm_type<f16>(a, s, stop);
-    case kActBF16: return norm_type<bf16>(a, s, stop);
+    case kActF32: return norm_type<float>(a, cus, s, stop);
+    case kActF16: return norm_type<f16>(a, cus, s, stop);
+    case kActBF16: return norm_type<bf16>(a, cus, s, stop);
     default: return hipErrorInvalidValue;
     }
 }

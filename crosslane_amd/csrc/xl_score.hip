@@ -23,6 +23,7 @@ namespace xl::dev {
 namespace {
 
 constexpr double kMaskedKey = -1e300;
+constexpr float kMaxFloat = 3.402823466e38f;
 
 // Keys as unsigned integers that order as the doubles do; 0 for what is out.
 __device__ __forceinline__ uint64_t ordered64(double d) {
@@ -43,124 +44,174 @@ __device__ __forceinline__ uint64_t readlane64(uint64_t v, int lane) {
     const uint32_t hi = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v >> 32)), lane));
     return uint64_t(lo) | (uint64_t(hi) << 32);
 }
-template <class F>
-__device__ __forceinline__ uint64_t wave_fold64(uint64_t v, F f) {   // identity 0
-    v = f(v, dpp64<0xB1>(v));
-    v = f(v, dpp64<0x4E>(v));
-    v = f(v, dpp64<0x141>(v));
-    v = f(v, dpp64<0x140>(v));
-    v = f(v, dpp64<0x142, 0xA>(v));
-    v = f(v, dpp64<0x143, 0xC>(v));
-    return readlane64(v, 63);
+__device__ __forceinline__ double readlane_f64(double v, int lane) {
+    return __longlong_as_double(int64_t(readlane64(uint64_t(__double_as_longlong(v)), lane)));
 }
-__device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
-    return wave_fold64(v, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+__device__ __forceinline__ double wave_sum64(double x) {
+    const auto add = [](double v, uint64_t o) { return v + __longlong_as_double(int64_t(o)); };
+    const auto bits = [](double v) { return uint64_t(__double_as_longlong(v)); };
+    x = add(x, dpp64<0xB1>(bits(x)));
+    x = add(x, dpp64<0x4E>(bits(x)));
+    x = add(x, dpp64<0x141>(bits(x)));
+    x = add(x, dpp64<0x140>(bits(x)));
+    x = add(x, dpp64<0x142, 0xA>(bits(x)));
+    x = add(x, dpp64<0x143, 0xC>(bits(x)));
+    return readlane_f64(x, 63);
 }
-__device__ __forceinline__ double wave_sum64(double v) {
-    return __longlong_as_double(int64_t(wave_fold64(uint64_t(__double_as_longlong(v)), [](uint64_t a, uint64_t b) {
-        return uint64_t(__double_as_longlong(__longlong_as_double(int64_t(a)) + __longlong_as_double(int64_t(b))));
-    })));
+__device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint64_t min64(uint64_t a, uint64_t b) { return a > b ? b : a; }
+
+// The two largest keys of each aligned run of `lanes` (1, 2, ... 64) lanes, in all of
+// them, from each lane's two.
+__device__ __forceinline__ void top_two(uint64_t& m1, uint64_t& m2, int lanes) {
+    const auto join = [&](uint64_t o1, uint64_t o2) {
+        m2 = max64(min64(m1, o1), max64(m2, o2));
+        m1 = max64(m1, o1);
+    };
+    if (lanes >= 2) join(dpp64<0xB1>(m1), dpp64<0xB1>(m2));
+    if (lanes >= 4) join(dpp64<0x4E>(m1), dpp64<0x4E>(m2));
+    if (lanes >= 8) join(dpp64<0x141>(m1), dpp64<0x141>(m2));
+    if (lanes >= 16) join(dpp64<0x140>(m1), dpp64<0x140>(m2));
+    if (lanes >= 32) join(__shfl_xor(static_cast<unsigned long long>(m1), 16), __shfl_xor(static_cast<unsigned long long>(m2), 16));
 }
 
-// One wave per token, expert lane + 64 j in slot j of each lane. Group values
-// through LDS: lane g reads group g's keys.
-template <class T, int NPL>
+// One wave per token. Up to 64 groups: each has a run of 64 / (groups rounded up to a
+// power of two) lanes, its experts going round them (one group: all 64), so that its
+// value is a few lane steps away and ranks come from lanes' values as scalars. MANY
+// (more groups): experts go round all lanes, and groups' keys and values through LDS.
+//
+// Bound by instructions: about 600 for 256 experts in 8 groups, a third of them the
+// scores' (exp and a quotient in double). A pick is a maximum of the keys' upper words
+// over the wave; only where two lanes have the same do lower words and indexes decide.
+template <class T, int NPL, bool MANY>
 __global__ __launch_bounds__(256) void score_route_kernel(ScoreArgs a) {
     constexpr int WAVES = 4;
-    __shared__ uint64_t keys[WAVES][NPL * 64];
-    __shared__ double values[WAVES][NPL * 64];
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    __shared__ uint64_t keys[MANY ? WAVES : 1][MANY ? NPL * 64 : 1];
+    __shared__ double values[MANY ? WAVES : 1][MANY ? NPL * 64 : 1];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t t = int64_t(blockIdx.x) * WAVES + wv;
-    const bool here = t < a.T;   // every wave reaches the barriers
+    const bool here = t < a.T;
+    if (!MANY && !here) return;   // MANY: every wave reaches the barriers
     const T* lg = static_cast<const T*>(a.logits) + (here ? t : 0) * a.stride;
+    const int size = a.size, run = MANY ? 64 : 1 << a.run;   // a group's experts and lanes
+    const int g = MANY ? 0 : lane >> a.run, r = lane & (run - 1);
+    const int first = MANY ? r : g < a.groups ? g * size + r : a.n;   // the lane's experts: first, first + run, ...
+    const int end = MANY ? a.n : g < a.groups ? (g + 1) * size : 0;   // ... below end
     float l[NPL];
+    float b[NPL];
     float top = -__int_as_float(0x7f800000);
     bool bad = false;
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {
-        const int e = lane + 64 * j;
-        l[j] = e < a.n ? float(lg[e]) : -__int_as_float(0x7f800000);
-        bad |= !(l[j] <= 3.402823466e38f);
-        top = fmaxf(top, l[j]);
+        const int e = first + run * j;
+        l[j] = e < end ? float(lg[e]) : -__int_as_float(0x7f800000);
+        b[j] = a.bias && e < end ? a.bias[e] : 0.0f;
     }
-    // the largest logit, by integers that order as floats do
-    const uint32_t ot = wave_ext<true>(ordered(top));
-    top = __uint_as_float((ot & 0x80000000u) ? (ot ^ 0x80000000u) : ~ot);
-    const double dtop = top >= -3.402823466e38f ? double(top) : 0.0;
-    double p[NPL], total = 0.0;
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {
-        const double x = double(l[j]);
-        const bool on = l[j] >= -3.402823466e38f;
-        p[j] = !on ? 0.0 : a.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - dtop);
-        total += p[j];
+        const bool no = !(l[j] <= kMaxFloat) || !(fabsf(b[j]) <= kMaxFloat);
+        bad |= no;
+        l[j] = no ? 0.0f : l[j];   // picks stay indexes of experts
+        b[j] = no ? 0.0f : b[j];
+        top = fmaxf(top, l[j]);
     }
-    double denom = 1.0;
-    if (!a.sigmoid) {
+    if (__any(bad) && here && lane == 0) atomicOr(a.err, kDevErrNonFinite);
+    double p[NPL], denom = 1.0;
+    if (a.sigmoid) {
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) p[j] = l[j] >= -kMaxFloat ? 1.0 / (1.0 + exp(-double(l[j]))) : 0.0;
+    } else {
+        // the largest logit, by integers that order as floats do
+        const uint32_t ot = wave_ext<true>(ordered(top));
+        top = __uint_as_float((ot & 0x80000000u) ? (ot ^ 0x80000000u) : ~ot);
+        double total = 0.0;
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) {
+            p[j] = l[j] >= -kMaxFloat ? exp(double(l[j]) - double(top)) : 0.0;
+            total += p[j];
+        }
         denom = wave_sum64(total);
         denom = denom > 0.0 ? denom : 1.0;
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) p[j] = p[j] / denom;
     }
     uint64_t key[NPL];
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) {
-        const int e = lane + 64 * j;
-        const float b = a.bias && e < a.n ? a.bias[e] : 0.0f;
-        const bool on = l[j] >= -3.402823466e38f;
-        bad |= !(fabsf(b) <= 3.402823466e38f);
-        const double s = a.sigmoid ? p[j] : p[j] / denom;
-        key[j] = e < a.n ? ordered64(on ? s + double(b) : kMaskedKey) : 0;
-    }
-    if (__any(bad) && here && lane == 0) atomicOr(a.err, kDevErrNonFinite);
-    if (a.groups > 1) {
-        const int size = a.n / a.groups;
+    for (int j = 0; j < NPL; ++j)
+        key[j] = first + run * j < end ? ordered64(l[j] >= -kMaxFloat ? p[j] + double(b[j]) : kMaskedKey) : 0;
+    if constexpr (MANY) {
 #pragma unroll
         for (int j = 0; j < NPL; ++j) keys[wv][lane + 64 * j] = key[j];
         __syncthreads();
-        for (int g = lane; g < a.groups; g += 64) {
+        for (int i = lane; i < a.groups; i += 64) {
             uint64_t m1 = 0, m2 = 0;
-            for (int i = 0; i < size; ++i) {
-                const uint64_t v = keys[wv][g * size + i];
-                if (v > m1) { m2 = m1; m1 = v; }
-                else if (v > m2) m2 = v;
+            for (int e = i * size; e < (i + 1) * size; ++e) {
+                const uint64_t v = keys[wv][e];
+                m2 = max64(m2, min64(m1, v));
+                m1 = max64(m1, v);
             }
-            values[wv][g] = unordered64(m1) + (a.group_keys == 2 ? unordered64(m2) : 0.0);
+            values[wv][i] = unordered64(m1) + (a.group_keys == 2 ? unordered64(m2) : 0.0);
         }
         __syncthreads();
-        // a group stays if fewer than top_groups are ahead of it
 #pragma unroll
         for (int j = 0; j < NPL; ++j) {
-            const int g = (lane + 64 * j) / size;
             if (lane + 64 * j >= a.n) continue;
-            const double mine = values[wv][g];
+            const int mine = (lane + 64 * j) / size;
             int ahead = 0;
-            for (int i = 0; i < a.groups; ++i) {
-                const double v = values[wv][i];
-                ahead += (v > mine || (v == mine && i < g)) ? 1 : 0;
-            }
+            for (int i = 0; i < a.groups; ++i)
+                ahead += values[wv][i] > values[wv][mine] || (values[wv][i] == values[wv][mine] && i < mine) ? 1 : 0;
             if (ahead >= a.top_groups) key[j] = 0;
         }
+    } else if (a.top_groups < a.groups) {
+        uint64_t m1 = 0, m2 = 0;
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) {
+            m2 = max64(m2, min64(m1, key[j]));
+            m1 = max64(m1, key[j]);
+        }
+        top_two(m1, m2, run);
+        const double value = unordered64(m1) + (a.group_keys == 2 ? unordered64(m2) : 0.0);
+        int ahead = 0;   // a group stays if fewer than top_groups are ahead of it
+        for (int i = 0; i < a.groups; ++i) {
+            const double v = readlane_f64(value, i * run);
+            ahead += v > value || (v == value && i < g) ? 1 : 0;
+        }
+        if (ahead >= a.top_groups)
+#pragma unroll
+            for (int j = 0; j < NPL; ++j) key[j] = 0;
     }
     double sum = 0.0, mine = 0.0;
     int myid = 0;
     for (int i = 0; i < a.k; ++i) {
         uint64_t bk = 0;
-        int bj = 0;
+        int be = 0;
+        double bs = 0.0;
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) {
+            const bool more = key[j] > bk;
+            bk = more ? key[j] : bk;
+            be = more ? first + run * j : be;
+            bs = more ? p[j] : bs;
+        }
+        const uint32_t hi = uint32_t(bk >> 32), best = wave_ext<true>(hi);
+        uint64_t who = __ballot(hi == best);
+        if (who & (who - 1)) {
+            const uint32_t lo = wave_ext<true>(hi == best ? uint32_t(bk) : 0u);
+            const bool in = hi == best && uint32_t(bk) == lo;
+            const uint32_t e = wave_ext<false>(in ? uint32_t(be) : 0xffffffffu);
+            who = __ballot(in && uint32_t(be) == e);
+        }
+        const int from = __builtin_ctzll(who);
+        const int e = __builtin_amdgcn_readlane(be, from);
+        const double s = readlane_f64(bs, from);
 #pragma unroll
         for (int j = 0; j < NPL; ++j)
-            if (key[j] > bk) { bk = key[j]; bj = j; }
-        const uint64_t best = wave_max64(bk);
-        const int e = int(wave_ext<false>(bk == best ? uint32_t(lane + 64 * bj) : 0xffffffffu));
-        double s = 0.0;
-#pragma unroll
-        for (int j = 0; j < NPL; ++j)
-            if (lane + 64 * j == e) {
-                s = p[j];
-                key[j] = 0;
-            }
-        s = __longlong_as_double(int64_t(readlane64(uint64_t(__double_as_longlong(s)), e & 63)));
-        if (!a.sigmoid) s = s / denom;
+            if (lane == from && first + run * j == e) key[j] = 0;
         sum += s;
-        if (lane == i) { mine = s; myid = e; }
+        if (lane == i) {
+            mine = s;
+            myid = e;
+        }
     }
     if (here && lane < a.k) {
         const double w = a.renorm ? mine / (sum + 1e-20) : mine;
@@ -170,15 +221,21 @@ __global__ __launch_bounds__(256) void score_route_kernel(ScoreArgs a) {
 }
 
 template <class T>
-void score_type(const ScoreArgs& a, hipStream_t s, hipEvent_t stop) {
+void score_type(ScoreArgs a, hipStream_t s, hipEvent_t stop) {
     const auto go = [&](auto kernel) {
         hipExtLaunchKernelGGL(kernel, dim3((a.T + 3) / 4), dim3(256), 0, s, nullptr, stop, 0, a);
     };
-    if (a.n <= 64) go(score_route_kernel<T, 1>);
-    else if (a.n <= 128) go(score_route_kernel<T, 2>);
-    else if (a.n <= 256) go(score_route_kernel<T, 4>);
-    else if (a.n <= 512) go(score_route_kernel<T, 8>);
-    else go(score_route_kernel<T, 16>);
+    a.size = a.n / a.groups;
+    if (a.groups > 64) return go(score_route_kernel<T, 16, true>);
+    for (a.run = 6; a.groups << a.run > 64;) --a.run;
+    const int slots = (a.size + (1 << a.run) - 1) >> a.run;
+    if (slots <= 1) go(score_route_kernel<T, 1, false>);
+    else if (slots <= 2) go(score_route_kernel<T, 2, false>);
+    else if (slots <= 4) go(score_route_kernel<T, 4, false>);
+    else if (slots <= 6) go(score_route_kernel<T, 6, false>);
+    else if (slots <= 8) go(score_route_kernel<T, 8, false>);
+    else if (slots <= 16) go(score_route_kernel<T, 16, false>);
+    else go(score_route_kernel<T, 32, false>);   // a number of groups far from a power of two
 }
 
 }  // namespace

@@ -229,8 +229,8 @@ class _Kinds(dict):
     torch dtype; looked up by name once each, torch itself is not imported here."""
     NAMES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2, "torch.int8": 3, "torch.int32": 4}
 
-    def __missing__(self, dtype) -> int:
-        kind = self[dtype] = self.NAMES.get(str(dtype), -1)
+    def __missing__(self, dtype) -> int:   # other types: -2 (-1 stands for a matrix that is not given)
+        kind = self[dtype] = self.NAMES.get(str(dtype), -2)
         return kind
 
 
@@ -251,8 +251,10 @@ def _act(t, what: str) -> int:
     return kind
 
 
-def _rows(t, what: str, shape=None) -> int:
-    """A [T, n] matrix of contiguous rows on the GPU; returns its row stride."""
+def _mat(t, what: str, shape=None):
+    """A [T, n] matrix of contiguous rows on the GPU: address, row stride, element type (None: null)."""
+    if t is None:
+        return None, 0, -1
     sh, st = t.shape, t.stride()
     if len(sh) != 2 or (st[1] != 1 and sh[1] != 1):
         _refuse(f"{what}: a matrix of contiguous rows is wanted")
@@ -260,7 +262,10 @@ def _rows(t, what: str, shape=None) -> int:
         _refuse(f"{what}: not on the GPU")
     if shape is not None and sh != shape:
         _refuse(f"{what}: shape {tuple(sh)} where {tuple(shape)} is wanted")
-    return st[0] if sh[0] > 1 else max(st[0], sh[1])
+    row = st[0]
+    if sh[0] <= 1 and row < sh[1]:
+        row = sh[1]
+    return t.data_ptr(), row, _KINDS[t.dtype]
 
 
 def _vec(t, n: int, what: str, kind: int = 0):
@@ -304,6 +309,8 @@ class Lane:
         err = _Err()
         _check(L.xl_open(ABI_VERSION, C.byref(cfg), C.byref(ctx), C.byref(err)), err)
         self._ctx = ctx
+        self._err = _Err()   # of the calls that a decode loop makes many of (a context has one caller at a time)
+        self._errp = C.byref(self._err)
         self.dim, self.ff, self.n_layers, self.n_experts, self.max_picks = dim, ff, n_layers, n_experts, max_picks
         types = np.ascontiguousarray(types, dtype=np.int32).reshape(n_layers, n_experts, 3)
         self.types = types
@@ -602,11 +609,12 @@ class Lane:
         largest keys; ids (int32) and w [T, k]."""
         if score not in SCORES:
             _refuse(f"score must be one of {sorted(SCORES)}")
-        stride = _rows(logits, "logits")
+        lp, stride, _ = _mat(logits, "logits")
         T, n = logits.shape
-        self._call("xl_route_scored_async", logits.data_ptr(), _act(logits, "logits"), T, stride, _vec(bias, n, "bias"), n,
-                   SCORES[score], groups, top_groups, group_keys, int(k), bool(renorm), float(scale), _vec(ids, T * k, "ids", _INT32),
-                   _vec(w, T * k, "w"), None if stream is None else int(stream))
+        _check(lib().xl_route_scored_async(
+            self._ctx, lp, _act(logits, "logits"), T, stride, _vec(bias, n, "bias"), n, SCORES[score], groups, top_groups,
+            group_keys, int(k), bool(renorm), float(scale), _vec(ids, T * k, "ids", _INT32), _vec(w, T * k, "w"),
+            None if stream is None else int(stream), self._errp), self._err)
 
     def block_norm_async(self, res, y=None, post_w=None, gate=None, alpha: float = 1.0, pre_w=None, eps: float = 1e-6,
                          res_out=None, x=None, q=None, q_scale=None, stream=None) -> None:
@@ -618,57 +626,45 @@ class Lane:
         if some is None:
             _refuse("res or y is wanted")
         shape = some.shape
-        if len(shape) != 2:
-            _refuse("res and y: a matrix of contiguous rows is wanted")
+        yp, ys, yk = _mat(y, "y", shape)
+        rp, rs, rk = _mat(res, "res", shape)
+        op, os_, ok = _mat(res_out, "res_out", shape)
+        xp, xs, xk = _mat(x, "x", shape)
+        qp, qs, qk = _mat(q, "q", shape)
         T, D = shape
-        kind = rkind = -1
-        at = []   # address and row stride of each matrix
-        for t, what in ((y, "y"), (x, "x")):
-            if t is None:
-                at += (None, 0)
-                continue
-            at += (t.data_ptr(), _rows(t, what, shape))
-            k = _act(t, what)
-            if kind not in (-1, k):
-                _refuse("y, x and gate have one element type, res and res_out one")
-            kind = k
-        for t, what in ((res, "res"), (res_out, "res_out")):
-            if t is None:
-                at += (None, 0)
-                continue
-            at += (t.data_ptr(), _rows(t, what, shape))
-            k = _act(t, what)
-            if rkind not in (-1, k):
-                _refuse("y, x and gate have one element type, res and res_out one")
-            rkind = k
-        gp, gs = None, 0
+        gp, gs, gk = None, 0, -1
         if gate is not None:
-            k = _act(gate, "gate")
-            if kind not in (-1, k):
-                _refuse("y, x and gate have one element type, res and res_out one")
-            kind = k
             if gate.dim() == 1:
-                gp = _vec(gate, D, "gate", k)
+                gk = _KINDS[gate.dtype]
+                gp = _vec(gate, D, "gate", gk)
             else:
-                gp, gs = gate.data_ptr(), _rows(gate, "gate", shape)
-        qp, qs = None, 0
-        if q is not None:
-            if _KINDS[q.dtype] != _INT8:
-                _refuse("q must be int8")
-            qp, qs = q.data_ptr(), _rows(q, "q", shape)
-        rkind = max(rkind, 0)
-        self._call("xl_block_norm_async", at[0], at[1], at[4], at[5], gp, gs, _vec(post_w, D, "post_w"),
-                   _vec(pre_w, D, "pre_w"), T, D, kind if kind >= 0 else rkind, rkind, float(alpha), float(eps), at[6], at[7], at[2], at[3],
-                   qp, qs, _vec(q_scale, T, "q_scale"), None if stream is None else int(stream))
+                gp, gs, gk = _mat(gate, "gate", shape)
+        # -1: not given
+        kind = yk if yk >= 0 else xk if xk >= 0 else gk
+        rkind = rk if rk >= 0 else ok
+        if kind not in (yk, xk, gk) or (yk >= 0 and yk != kind) or (xk >= 0 and xk != kind) or (gk >= 0 and gk != kind) \
+                or (ok >= 0 and ok != rkind):
+            _refuse("y, x and gate have one element type, res and res_out one")
+        if kind >= _INT8 or rkind >= _INT8 or min(yk, xk, gk, rk, ok) < -1:
+            _refuse("y, x, gate, res and res_out: element type not taken here")
+        if q is not None and qk != _INT8:
+            _refuse("q must be int8")
+        if rkind < 0:
+            rkind = 0
+        _check(lib().xl_block_norm_async(
+            self._ctx, yp, ys, rp, rs, gp, gs, _vec(post_w, D, "post_w"), _vec(pre_w, D, "pre_w"), T, D,
+            kind if kind >= 0 else rkind, rkind, float(alpha), float(eps), op, os_, xp, xs, qp, qs,
+            _vec(q_scale, T, "q_scale"), None if stream is None else int(stream), self._errp), self._err)
 
     def quantize_rows_async(self, x, q, scale, stream=None) -> None:
         """x [T, K] (f32, f16 or bf16) to int8 q [T, K] (16-byte aligned rows) with scale [T]."""
-        stride, shape = _rows(x, "x"), x.shape
-        qs = _rows(q, "q", shape)
-        if _KINDS[q.dtype] != _INT8:
+        xp, xs, _ = _mat(x, "x")
+        T, K = shape = x.shape
+        qp, qs, qk = _mat(q, "q", shape)
+        if qk != _INT8:
             _refuse("q must be int8")
-        self._call("xl_quantize_rows_async", x.data_ptr(), _act(x, "x"), shape[0], shape[1], stride, q.data_ptr(), qs,
-                   _vec(scale, shape[0], "scale"), None if stream is None else int(stream))
+        _check(lib().xl_quantize_rows_async(self._ctx, xp, _act(x, "x"), T, K, xs, qp, qs, _vec(scale, T, "scale"),
+                                            None if stream is None else int(stream), self._errp), self._err)
 
     def linear_i8_async(self, x, w, w_scale, out, x_scale=None, up=None, up_scale=None, limit: float = 0.0, work=None,
                         stream=None) -> None:
@@ -676,24 +672,25 @@ class Lane:
         for each token and channel; x int8 with x_scale [T], or float (quantized by
         the call). With up, up_scale: SwiGLU of the products with w (gate) and up.
         work: linear_i8_work_bytes(T, K, N, gated) bytes."""
-        xs, ws = _rows(x, "x"), _rows(w, "w")
+        xp, xs, kind = _mat(x, "x")
+        wp, ws, wk = _mat(w, "w")
         T, K = x.shape
         shape = w.shape
         N = shape[0]
-        if shape[1] != K or _KINDS[w.dtype] != _INT8:
+        if shape[1] != K or wk != _INT8:
             _refuse("w: int8 [N, K] is wanted")
-        os_ = _rows(out, "out", (T, N))
-        if up is not None and (_KINDS[up.dtype] != _INT8 or _rows(up, "up", shape) != ws):
+        op, os_, _ = _mat(out, "out", (T, N))
+        up_, us, uk = _mat(up, "up", shape)
+        if up is not None and (uk != _INT8 or us != ws):
             _refuse("up: int8 with w's shape and stride is wanted")
         if work is None or not (work.is_cuda and work.is_contiguous()):
             _refuse("work: a contiguous GPU buffer is wanted")
-        kind = _KINDS[x.dtype]
         if not 0 <= kind <= _INT8:
             _refuse(f"x: element type {x.dtype} not taken here")
-        self._call("xl_linear_i8_async", x.data_ptr(), kind, _vec(x_scale, T, "x_scale"), xs, T, K, w.data_ptr(),
-                   _vec(w_scale, N, "w_scale"), None if up is None else up.data_ptr(), _vec(up_scale, N, "up_scale"), ws, N,
-                   float(limit), out.data_ptr(), _act(out, "out"), os_, work.data_ptr(), work.numel() * work.element_size(),
-                   None if stream is None else int(stream))
+        _check(lib().xl_linear_i8_async(
+            self._ctx, xp, kind, _vec(x_scale, T, "x_scale"), xs, T, K, wp, _vec(w_scale, N, "w_scale"), up_,
+            _vec(up_scale, N, "up_scale"), ws, N, float(limit), op, _act(out, "out"), os_, work.data_ptr(), work.nbytes,
+            None if stream is None else int(stream), self._errp), self._err)
 
     def swiglu_async(self, g, u, h, limit: float = 0.0, stream=None) -> None:
         self._call("xl_swiglu_async", _ptr(g), _ptr(u), int(g.numel()), float(limit), _ptr(h),
