@@ -74,14 +74,28 @@ __device__ __forceinline__ void each(F&& f) {   // f(0), ... f(N - 1) with compi
 
 // `n` rows of K bytes from row `first`, as a buffer whose range ends with the last
 // row's last 16 bytes (nothing behind it is read).
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const int8_t* p, int64_t stride, int64_t first, int64_t n, int K) {
+__device__ __forceinline__ v4i rows_of(const int8_t* p, int64_t stride, int64_t first, int64_t n, int K) {
+    const uint64_t at = reinterpret_cast<uint64_t>(p + first * stride);
     const uint32_t bytes = uint32_t((n - 1) * stride) + uint32_t((K + 15) & ~15);
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p + first * stride), 0, bytes, 0x00020000);
+    return v4i{__builtin_amdgcn_readfirstlane(int(uint32_t(at))), __builtin_amdgcn_readfirstlane(int(uint32_t(at >> 32) & 0xffffu)),
+               __builtin_amdgcn_readfirstlane(int(bytes)), 0x00020000};
 }
-// Its 16 bytes at voff + soff straight to LDS, lane by lane from `lds` on.
-__device__ __forceinline__ void buffer16_lds(__amdgpu_buffer_rsrc_t r, int8_t* lds, uint32_t voff, int soff) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, voff, soff, 0, 0);
+// Its 16 bytes at voff + soff straight to LDS, lane by lane from `lds` on. Neither a
+// register's value nor, for the compiler, an access to LDS: left to it, every read of
+// LDS behind such a load waits for all of them. wait_loads and the barriers here order
+// loads and reads instead; with the "memory" that each names nothing moves across them.
+// (m0 is nobody else's here, and a register that a statement cannot name.)
+__device__ __forceinline__ void buffer16_lds(v4i r, const int8_t* lds, uint32_t voff, int soff) {
+    const uint32_t at = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const int8_t*)lds));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :: "s"(__builtin_amdgcn_readfirstlane(int(at))), "v"(voff), "s"(r), "s"(soff) : "memory");
 }
+// All but the last N of the wave's loads to LDS are there.
+template <int N>
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
+// The wave's reads of LDS are done; then the workgroup's barrier.
+__device__ __forceinline__ void reads_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // A mask of 16 bytes, the first n kept.
 __device__ __forceinline__ v4i bytes_below(int n) {
     v4i m;
@@ -101,8 +115,8 @@ __global__ __launch_bounds__(64 * WT * WC, OCC) void lin8_tile_kernel(Lin8Args a
     constexpr int RPL = NT / 8;                            // rows of one load of all threads
     constexpr int LT = (TT + RPL - 1) / RPL, LC = (TC + RPL - 1) / RPL;   // 16-byte loads of a thread
     constexpr bool SPARE = TT % RPL || TC % RPL;           // the last ones of some waves bring nothing
-    static_assert(R <= NJ && NJ % R == 0 && S >= 2 && S <= 4);
-    // a variable for each stage: the compiler then sees that loads into one do not touch another
+    constexpr int PARTS = S == 2 ? 2 : 1;                  // parts of a stage's tokens that are given back by themselves
+    static_assert(R <= NJ && NJ % R == 0 && S >= 2 && S <= 4 && LT % PARTS == 0 && NJ % PARTS == 0);
     constexpr int STAGE = (TT + M * TC) * BK;
     __shared__ alignas(16) int8_t lds0[STAGE], lds1[STAGE], lds2[S > 2 ? STAGE : 16], lds3[S > 3 ? STAGE : 16], spare[SPARE ? 1024 : 16];
     const auto stage = [&](auto si) -> int8_t* {
@@ -127,7 +141,10 @@ __global__ __launch_bounds__(64 * WT * WC, OCC) void lin8_tile_kernel(Lin8Args a
     const int row = tid >> 3, k16 = 16 * ((tid ^ row) & 7);
     uint32_t offt[LT], offc[LC];
 #pragma unroll
-    for (int i = 0; i < LT; ++i) offt[i] = uint32_t(row + i * RPL) * uint32_t(a.x_stride) + k16;
+    for (int i = 0; i < LT; ++i) {
+        const int r = row + i * RPL, in = r % (TT / PARTS);   // PARTS 2: the waves' first tiles in the first half of the rows
+        offt[i] = uint32_t(in / (WTT / PARTS) * WTT + r / (TT / PARTS) * (WTT / PARTS) + in % (WTT / PARTS)) * uint32_t(a.x_stride) + k16;
+    }
 #pragma unroll
     for (int i = 0; i < LC; ++i) {
         const int r = row + i * RPL, in = r % WTC, m = in & 15;   // LDS row r: tile in / 16 of wave r / WTC, row m
@@ -140,8 +157,8 @@ __global__ __launch_bounds__(64 * WT * WC, OCC) void lin8_tile_kernel(Lin8Args a
         constexpr int i = decltype(ii)::value, j = i < LT ? i : (i - LT) % LC, rows = i < LT ? TT : TC;
         constexpr int part = i < LT ? 0 : i < LT + LC ? TT : TT + TC;
         int8_t* b = stage(si) + (part + j * RPL + wv * 8) * BK;
-        const int k = s * BK;
-        uint32_t out = k + k16 < a.K ? 0u : 0x80000000u;
+        const int k = min(s * BK, a.K);   // never behind the buffer's range
+        uint32_t out = s * BK + k16 < a.K ? 0u : 0x80000000u;
         if constexpr ((j + 1) * RPL > rows)
             if (j * RPL + wv * 8 >= rows) {
                 b = spare;
@@ -153,7 +170,7 @@ __global__ __launch_bounds__(64 * WT * WC, OCC) void lin8_tile_kernel(Lin8Args a
     };
     v4i acc[M][NI][NJ] = {};
     v4i fw[2][M][NI], ft[R];
-    const uint32_t gett = uint32_t((wt * WTT + c) * BK), getc = uint32_t((TT + wc * WTC + c) * BK);
+    const uint32_t gett = uint32_t((wt * (WTT / PARTS) + c) * BK), getc = uint32_t((TT + wc * WTC + c) * BK);
     const uint32_t at[2] = {uint32_t(16 * (q ^ (c & 7))), uint32_t(16 * ((4 + q) ^ (c & 7)))};
     const auto weights = [&](auto hi, const int8_t* b) {   // of the step's half h
         constexpr int h = decltype(hi)::value;
@@ -164,7 +181,8 @@ __global__ __launch_bounds__(64 * WT * WC, OCC) void lin8_tile_kernel(Lin8Args a
     };
     const auto tokens = [&](auto pi, const int8_t* b) {    // piece p: half p / NJ, token tile p % NJ
         constexpr int p = decltype(pi)::value;
-        ft[p % R] = *reinterpret_cast<const v4i*>(b + gett + 16 * (p % NJ) * BK + at[p / NJ]);
+        constexpr int j = p % NJ, JP = NJ / PARTS;
+        ft[p % R] = *reinterpret_cast<const v4i*>(b + gett + (j / JP * (TT / PARTS) + 16 * (j % JP)) * BK + at[p / NJ]);
     };
     const auto multiply = [&](auto pi) {
         constexpr int p = decltype(pi)::value, h = p / NJ, j = p % NJ;
@@ -175,14 +193,34 @@ __global__ __launch_bounds__(64 * WT * WC, OCC) void lin8_tile_kernel(Lin8Args a
                 acc[m][i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[h][m][i], ft[p % R], acc[m][i][j], 0, 0, 0);
     };
     // A step reads its 2 NJ pieces R ahead of their products; the last R products run
-    // after the barrier, over the next step's first reads. Its stage is loaded S - 1 steps
-    // ahead, into the one that every wave has read when the barrier before lets it pass;
-    // the loads lie between the products, as a wave that issues them in a row stands still
-    // until the memory pipeline has taken them.
-    const auto piece = [&](auto si, auto xi, int s) {
+    // after the barrier, over the next step's first reads. The loads lie between the
+    // products, as a wave that issues them in a row stands still until the memory pipeline
+    // has taken them.
+    //
+    // S > 2: a step loads the stage S - 1 ahead, into the one that every wave has read when
+    // the barrier before lets it pass. S == 2: each part of a stage is given back by a
+    // barrier of its own as soon as it has been read, and loaded for two steps on: the
+    // weights after the first products, the first half of the tokens where the second
+    // half's last reads are left, the second half at the next step's start. So every load
+    // has a whole step to arrive.
+    constexpr int WEIGHTS = M * LC, AHEAD = S == 2 ? WEIGHTS + LT / 2 : (S - 2) * L;   // loads on their way at a step's end
+    constexpr int GIVE_T = NJ + NJ / 2 - R, GIVE_W = std::min(2, GIVE_T);               // pieces before which parts are given back
+    const auto some = [&](auto si, auto fi, auto ti, int s) {   // loads from .. to - 1
+        constexpr int from = decltype(fi)::value, n = std::max(0, decltype(ti)::value - from);
+        each<n>([&](auto i) { load(si, index<from + i>{}, s); });
+    };
+    const auto piece = [&](auto si, auto xi, int s) {   // x of 2 NJ: what is loaded behind it
         constexpr int x = decltype(xi)::value;
-        constexpr int from = std::min(L, x * L / NJ), to = std::min(L, (x + 1) * L / NJ);   // in the step's first half
-        each<to - from>([&](auto i) { load(index<si + S - 1>{}, index<from + i>{}, s + S - 1); });
+        if constexpr (S > 2) {   // in the step's first half
+            some(index<si + S - 1>{}, index<std::min(L, x * L / NJ)>{}, index<std::min(L, (x + 1) * L / NJ)>{}, s + S - 1);
+        } else if constexpr (x < R) {
+            some(index<si + 1>{}, index<LT / 2 + x * (LT / 2) / R>{}, index<LT / 2 + (x + 1) * (LT / 2) / R>{}, s + 1);
+        } else {
+            constexpr int p = x - R, w = p - GIVE_W, t = p - GIVE_T;
+            constexpr int over = std::min(4, 2 * NJ - R - GIVE_W), per = (WEIGHTS + over - 1) / over;   // pieces that they lie behind
+            if constexpr (w >= 0 && w < over) some(si, index<LT + std::min(WEIGHTS, w * per)>{}, index<LT + std::min(WEIGHTS, (w + 1) * per)>{}, s + 2);
+            if constexpr (t >= 0 && t < 2) some(si, index<t * (LT / 2) / 2>{}, index<(t + 1) * (LT / 2) / 2>{}, s + 2);
+        }
         __builtin_amdgcn_sched_barrier(0);   // the compiler would move each read to its use
     };
     const auto step = [&](auto si, int s) {
@@ -201,21 +239,28 @@ __global__ __launch_bounds__(64 * WT * WC, OCC) void lin8_tile_kernel(Lin8Args a
             piece(si, r, s);
         });
         each<2 * NJ - R>([&](auto p) {
-            if constexpr (p == NJ - R) weights(index<1>{}, b);
+            if constexpr (p == (S == 2 ? 0 : NJ - R)) weights(index<1>{}, b);
             multiply(p);
+            if constexpr (S == 2 && (p == GIVE_W || p == GIVE_T)) reads_barrier();
             tokens(index<p + R>{}, b);
             piece(si, index<p + R>{}, s);
         });
         // this wave's part of the next stage is here, and its reads of this one are done
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm((S - 2) * L) & kLgkm0);
-        asm volatile("s_barrier" ::: "memory");
+        wait_loads<AHEAD>();
+        reads_barrier();
     };
-    each<S - 1>([&](auto si) { each<L>([&](auto i) { load(si, i, si); }); });
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm((S - 2) * L));
-    asm volatile("s_barrier" ::: "memory");
+    if constexpr (S == 2) {
+        some(index<0>{}, index<0>{}, index<L>{}, 0);
+        some(index<1>{}, index<LT>{}, index<L>{}, 1);
+        some(index<1>{}, index<0>{}, index<LT / 2>{}, 1);
+    } else {
+        each<S - 1>([&](auto si) { some(si, index<0>{}, index<L>{}, si); });
+    }
+    wait_loads<AHEAD>();
+    reads_barrier();
     for (int s = 0; s < steps; s += S) each<S>([&](auto si) { if (s + si < steps) step(si, s + si); });
     each<R>([&](auto r) { multiply(index<2 * NJ - R + r>{}); });
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // no load writes LDS behind the workgroup's end
+    wait_loads<0>();   // none writes LDS behind the workgroup's end
     const int64_t n = n0 + wc * WTC + 4 * NI * q;
     const int left = int(min(int64_t(4 * NI), int64_t(a.N) - n));
     float ws[M][4 * NI];
@@ -348,8 +393,7 @@ __global__ __launch_bounds__(64 * NW) void lin8_rows_kernel(Lin8Args a) {
     const auto work = [&](auto ui, int p) {
         const int8_t* b = stage(ui);
         v4i fw[2][M][NI], fx[2][NJ];
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm((U - 1) * L));
-        asm volatile("" ::: "memory");
+        wait_loads<(U - 1) * L>();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -360,8 +404,7 @@ __global__ __launch_bounds__(64 * NW) void lin8_rows_kernel(Lin8Args a) {
 #pragma unroll
                 for (int i = 0; i < NI; ++i) fw[h][m][i] = *reinterpret_cast<const v4i*>(b + (XR + 16 * (m * NI + i)) * BK + at[h]);
         }
-        __builtin_amdgcn_s_waitcnt(kLgkm0);   // read: the stage is free
-        asm volatile("" ::: "memory");
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read: the stage is free
         load(ui, p + U * NW);
         if (!FUSED && p == pieces - 1 && (a.K & (BK - 1))) {   // what lies behind a token's row counts as zeros
 #pragma unroll
@@ -382,7 +425,7 @@ __global__ __launch_bounds__(64 * NW) void lin8_rows_kernel(Lin8Args a) {
                         acc[m][i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[h][m][i], fx[h][j], acc[m][i][j], 0, 0, 0);
     };
     for (int p = wv; p < pieces; p += U * NW) each<U>([&](auto u) { if (p + u * NW < pieces) work(u, p + u * NW); });
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // no load is left to write into a stage
+    wait_loads<0>();   // none is left to write into a stage
     __syncthreads();
     v4i* sums = reinterpret_cast<v4i*>(&lds0[0][0]);   // [wave][tile][lane]
     constexpr int TILES = M * NI * NJ;
@@ -435,28 +478,23 @@ void lin8_rows(const Lin8Args& a, hipStream_t s, hipEvent_t stop) {
 // The ways to run a call, in order of their tiles: tokens, channels (of each of one or
 // two matrices), workgroups that one CU holds, and the microseconds that they take:
 // fixed, and for each 128-byte step of K with the chip mostly idle and with a workgroup
-// on every CU. Fitted to 500 calls of 1 to 8192 tokens, 256 to 8192 k, 300 to 9216
-// channels, one and two matrices: the way of the least estimate is within 0.7 % of the
-// fastest one on average, 12 % at most (96 tokens, 5120 x (2 x 2304): 11.8 for 10.5 us).
+// on every CU. Fitted to 285 calls of 1 to 8192 tokens, 64 to 8192 k, 100 to 9216
+// channels, one and two matrices, each run all ways: the way of the least estimate is
+// within 0.3 % of the fastest on average and 16 % at most (7.5 for 6.7 us).
 struct Way {
-    int tokens, one, two, per_cu;
+    int tokens, one, two, per_cu;   // two 0: one matrix only
     float fixed, idle, busy;
-    bool rounds;   // workgroups run in whole rounds over the CUs; else they overlap
+    bool rows;   // lin8_rows_kernel, whose workgroups overlap; else lin8_tile_kernel, in rounds over the CUs
 };
 constexpr Way kWays[] = {
-    {16, 16, 16, 1, 3.1f, 0.040f, 0.089f, false},    // lin8_rows_kernel
-    {32, 16, 16, 1, 3.2f, 0.081f, 0.102f, false},
-    {32, 32, 16, 1, 3.3f, 0.098f, 0.158f, false},
-    {32, 64, 32, 1, 4.0f, 0.142f, 0.253f, false},
-    {64, 64, 32, 2, 3.9f, 0.255f, 0.605f, true},     // lin8_tile_kernel
-    {64, 128, 64, 1, 4.0f, 0.337f, 0.463f, true},
-    {128, 128, 64, 1, 5.4f, 0.431f, 0.626f, true},
-    {128, 160, 96, 1, 5.7f, 0.621f, 0.790f, true},
-    {128, 256, 128, 1, 5.7f, 0.790f, 1.006f, true},
-    {256, 160, 96, 1, 12.9f, 0.623f, 1.242f, true},
-    {256, 192, 96, 1, 5.8f, 1.239f, 1.247f, true},
-    {256, 256, 128, 1, 8.5f, 1.208f, 1.647f, true},
+    {16, 16, 16, 1, 3.4f, 0.047f, 0.078f, true},    {32, 16, 16, 1, 3.4f, 0.077f, 0.110f, true},
+    {32, 32, 0, 1, 3.6f, 0.086f, 0.152f, true},     {32, 64, 32, 1, 4.6f, 0.135f, 0.213f, true},
+    {64, 64, 32, 2, 3.3f, 0.250f, 0.609f, false},   {64, 128, 64, 1, 3.3f, 0.309f, 0.323f, false},
+    {128, 128, 64, 1, 4.9f, 0.442f, 0.551f, false}, {128, 160, 96, 1, 6.0f, 0.576f, 0.742f, false},
+    {128, 256, 128, 1, 7.8f, 0.685f, 1.005f, false}, {256, 160, 0, 1, 9.1f, 0.752f, 1.258f, false},
+    {256, 192, 96, 1, 9.1f, 1.145f, 1.415f, false}, {256, 256, 128, 1, 11.6f, 1.124f, 1.871f, false},
 };
+constexpr float kRowsRound = 0.8f, kTilesRound = 4.2f;   // ... for each further round
 int lin8_way(const Lin8Args& a, int cus) {
     if (a.x_type != kActI8) return 0;
     int best = 0;
@@ -464,9 +502,11 @@ int lin8_way(const Lin8Args& a, int cus) {
     for (int i = 0; i < int(std::size(kWays)); ++i) {
         const Way& w = kWays[i];
         const int64_t ch = a.up ? w.two : w.one;
+        if (ch == 0) continue;
         const float per = float(((a.T + w.tokens - 1) / w.tokens) * ((a.N + ch - 1) / ch)) / float(cus * w.per_cu);
-        const float step = std::max((w.rounds ? std::ceil(per) : std::max(per, 1.0f)) * w.idle, per * w.busy);
-        const float us = w.fixed + float((a.K + 127) / 128) * step;
+        const float rounds = w.rows ? std::max(per, 1.0f) : std::ceil(per);
+        const float us = w.fixed + (w.rows ? kRowsRound : kTilesRound) * (rounds - 1.0f) +
+                         float((a.K + 127) / 128) * std::max((w.rows ? 1.0f : rounds) * w.idle, per * w.busy);
         if (i == 0 || us < least) {
             best = i;
             least = us;
@@ -486,10 +526,11 @@ void lin8_tiled(const Lin8Args& a, int way, hipStream_t s, hipEvent_t stop) {
     case 8: return lin8_tiles<OT, GATED, 128, 256 / G, 2, 4, 3, 4, 2>(a, s, stop);
     case 9:
         if constexpr (!GATED) return lin8_tiles<OT, GATED, 256, 160, 4, 2, 3, 4, 2>(a, s, stop);
-        else [[fallthrough]];   // 96 channels of each matrix either way
+        break;
     case 10: return lin8_tiles<OT, GATED, 256, 192 / G, 4, 2, 2, 4, 2>(a, s, stop);
-    default: return lin8_tiles<OT, GATED, 256, 256 / G, 2, 4, 2, 4, 2>(a, s, stop);
+    default: break;
     }
+    lin8_tiles<OT, GATED, 256, 256 / G, 2, 4, 2, 4, 2>(a, s, stop);
 }
 template <bool GATED>
 void lin8_run(const Lin8Args& a, int way, hipStream_t s, hipEvent_t stop) {
@@ -499,7 +540,9 @@ void lin8_run(const Lin8Args& a, int way, hipStream_t s, hipEvent_t stop) {
     switch (way) {
     case 0: return lin8_rows<1, 1, GATED, kActI8, 8, 2>(a, s, stop);
     case 1: return lin8_rows<1, 2, GATED, kActI8, 4, GATED ? 2 : 3>(a, s, stop);
-    case 2: return lin8_rows<GATED ? 1 : 2, 2, GATED, kActI8, 8, 2>(a, s, stop);
+    case 2:
+        if constexpr (!GATED) return lin8_rows<2, 2, GATED, kActI8, 8, 2>(a, s, stop);
+        break;
     case 3: return lin8_rows<GATED ? 2 : 4, 2, GATED, kActI8, 4, 3>(a, s, stop);
     default: break;
     }
