@@ -58,6 +58,29 @@ __device__ __forceinline__ double wave_sum64(double x) {
     x = add(x, dpp64<0x143, 0xC>(bits(x)));
     return readlane_f64(x, 63);
 }
+// The largest / smallest of the wave. Lanes that a step leaves out get the identity:
+// so each step is one instruction.
+template <bool MAX>
+__device__ __forceinline__ uint32_t wave_top(uint32_t v) {
+    constexpr int id = MAX ? 0 : -1;
+    const auto f = [](uint32_t x, uint32_t y) { return MAX ? max(x, y) : min(x, y); };
+    v = f(v, uint32_t(__builtin_amdgcn_update_dpp(id, int(v), 0xB1, 0xF, 0xF, false)));   // quad_perm 1,0,3,2
+    v = f(v, uint32_t(__builtin_amdgcn_update_dpp(id, int(v), 0x4E, 0xF, 0xF, false)));   // quad_perm 2,3,0,1
+    v = f(v, uint32_t(__builtin_amdgcn_update_dpp(id, int(v), 0x141, 0xF, 0xF, false)));  // row_half_mirror
+    v = f(v, uint32_t(__builtin_amdgcn_update_dpp(id, int(v), 0x140, 0xF, 0xF, false)));  // row_mirror
+    v = f(v, uint32_t(__builtin_amdgcn_update_dpp(id, int(v), 0x142, 0xA, 0xF, false)));  // row_bcast:15
+    v = f(v, uint32_t(__builtin_amdgcn_update_dpp(id, int(v), 0x143, 0xC, 0xF, false)));  // row_bcast:31
+    return uint32_t(__builtin_amdgcn_readlane(int(v), 63));
+}
+// An expert's score, 0 where it is masked (softmax: times the sum of these; `largest`
+// is finite). Without branches, so that the slots' exps run in step.
+__device__ __forceinline__ double sigmoid(float l) { return 1.0 / (1.0 + exp(-double(l))); }
+__device__ __forceinline__ double part(float l, double largest) { return exp(double(l) - largest); }
+// a where m is all ones, b where it is zero.
+__device__ __forceinline__ uint32_t pick(uint32_t m, uint32_t a, uint32_t b) { return (a & m) | (b & ~m); }
+__device__ __forceinline__ uint64_t pick(uint32_t m, uint64_t a, uint64_t b) {
+    return uint64_t(pick(m, uint32_t(a), uint32_t(b))) | uint64_t(pick(m, uint32_t(a >> 32), uint32_t(b >> 32))) << 32;
+}
 __device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 __device__ __forceinline__ uint64_t min64(uint64_t a, uint64_t b) { return a > b ? b : a; }
 
@@ -80,9 +103,10 @@ __device__ __forceinline__ void top_two(uint64_t& m1, uint64_t& m2, int lanes) {
 // value is a few lane steps away and ranks come from lanes' values as scalars. MANY
 // (more groups): experts go round all lanes, and groups' keys and values through LDS.
 //
-// Bound by instructions: about 600 for 256 experts in 8 groups, a third of them the
-// scores' (exp and a quotient in double). A pick is a maximum of the keys' upper words
-// over the wave; only where two lanes have the same do lower words and indexes decide.
+// Bound by instructions: 800 for 256 experts in 8 groups and 8 picks, a third of them the
+// scores' (exp and a quotient in double), which at 8192 tokens is 10.6 of the 14.0 us. A
+// pick is a maximum of the keys' upper words over the wave; only where two lanes have the
+// same do lower words and indexes decide.
 template <class T, int NPL, bool MANY>
 __global__ __launch_bounds__(256) void score_route_kernel(ScoreArgs a) {
     constexpr int WAVES = 4;
@@ -103,31 +127,31 @@ __global__ __launch_bounds__(256) void score_route_kernel(ScoreArgs a) {
     bool bad = false;
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {
-        const int e = first + run * j;
-        l[j] = e < end ? float(lg[e]) : -__int_as_float(0x7f800000);
-        b[j] = a.bias && e < end ? a.bias[e] : 0.0f;
+        const int e = first + run * j, at = min(e, a.n - 1);
+        l[j] = float(lg[at]);
+        b[j] = a.bias ? a.bias[at] : 0.0f;
     }
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {
-        const bool no = !(l[j] <= kMaxFloat) || !(fabsf(b[j]) <= kMaxFloat);
-        bad |= no;
-        l[j] = no ? 0.0f : l[j];   // picks stay indexes of experts
+        const bool in = first + run * j < end, no = !(l[j] <= kMaxFloat) || !(fabsf(b[j]) <= kMaxFloat);
+        bad |= in && no;
+        l[j] = !in ? -__int_as_float(0x7f800000) : no ? 0.0f : l[j];   // picks stay indexes of experts
         b[j] = no ? 0.0f : b[j];
         top = fmaxf(top, l[j]);
     }
     if (__any(bad) && here && lane == 0) atomicOr(a.err, kDevErrNonFinite);
-    double p[NPL], denom = 1.0;
+    double p[NPL], denom = 1.0, largest = 0.0;
     if (a.sigmoid) {
 #pragma unroll
-        for (int j = 0; j < NPL; ++j) p[j] = l[j] >= -kMaxFloat ? 1.0 / (1.0 + exp(-double(l[j]))) : 0.0;
+        for (int j = 0; j < NPL; ++j) p[j] = sigmoid(l[j]);
     } else {
         // the largest logit, by integers that order as floats do
-        const uint32_t ot = wave_ext<true>(ordered(top));
-        top = __uint_as_float((ot & 0x80000000u) ? (ot ^ 0x80000000u) : ~ot);
+        const uint32_t ot = wave_top<true>(ordered(top));
+        largest = double(fmaxf(__uint_as_float((ot & 0x80000000u) ? (ot ^ 0x80000000u) : ~ot), -kMaxFloat));
         double total = 0.0;
 #pragma unroll
         for (int j = 0; j < NPL; ++j) {
-            p[j] = l[j] >= -kMaxFloat ? exp(double(l[j]) - double(top)) : 0.0;
+            p[j] = part(l[j], largest);
             total += p[j];
         }
         denom = wave_sum64(total);
@@ -180,41 +204,70 @@ __global__ __launch_bounds__(256) void score_route_kernel(ScoreArgs a) {
 #pragma unroll
             for (int j = 0; j < NPL; ++j) key[j] = 0;
     }
-    double sum = 0.0, mine = 0.0;
+    // Up to 8 slots: each lane's keys in order first (neighbours change places, so that
+    // equal ones keep theirs), and a pick is the best of the lanes' first ones.
+    constexpr bool SORTED = NPL <= 8;
+    uint32_t slot[NPL];
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) slot[j] = j;
+    if constexpr (SORTED)
+#pragma unroll
+        for (int n = NPL - 1; n > 0; --n)
+#pragma unroll
+            for (int j = 0; j < n; ++j) {
+                const uint32_t swap = key[j] < key[j + 1] ? ~0u : 0u;
+                const uint64_t k0 = key[j], k1 = key[j + 1];
+                const uint32_t s0 = slot[j], s1 = slot[j + 1];
+                key[j] = pick(swap, k1, k0);
+                key[j + 1] = pick(swap, k0, k1);
+                slot[j] = pick(swap, s1, s0);
+                slot[j + 1] = pick(swap, s0, s1);
+            }
     int myid = 0;
     for (int i = 0; i < a.k; ++i) {
-        uint64_t bk = 0;
-        int be = 0;
-        double bs = 0.0;
+        uint64_t bk = key[0];
+        uint32_t be = slot[0];
+        if constexpr (!SORTED)
 #pragma unroll
-        for (int j = 0; j < NPL; ++j) {
-            const bool more = key[j] > bk;
-            bk = more ? key[j] : bk;
-            be = more ? first + run * j : be;
-            bs = more ? p[j] : bs;
-        }
-        const uint32_t hi = uint32_t(bk >> 32), best = wave_ext<true>(hi);
+            for (int j = 1; j < NPL; ++j) {
+                const bool more = key[j] > bk;
+                bk = more ? key[j] : bk;
+                be = more ? uint32_t(j) : be;
+            }
+        const uint32_t hi = uint32_t(bk >> 32), best = wave_top<true>(hi);
         uint64_t who = __ballot(hi == best);
         if (who & (who - 1)) {
-            const uint32_t lo = wave_ext<true>(hi == best ? uint32_t(bk) : 0u);
+            const uint32_t lo = wave_top<true>(hi == best ? uint32_t(bk) : 0u);
             const bool in = hi == best && uint32_t(bk) == lo;
-            const uint32_t e = wave_ext<false>(in ? uint32_t(be) : 0xffffffffu);
-            who = __ballot(in && uint32_t(be) == e);
+            const uint32_t e = uint32_t(first) + uint32_t(run) * be;
+            const uint32_t least = wave_top<false>(in ? e : 0xffffffffu);   // all lanes take part
+            who = __ballot(in && e == least);
         }
         const int from = __builtin_ctzll(who);
-        const int e = __builtin_amdgcn_readlane(be, from);
-        const double s = readlane_f64(bs, from);
+        const uint32_t taken = lane == from ? ~0u : 0u;
+        if constexpr (SORTED) {
 #pragma unroll
-        for (int j = 0; j < NPL; ++j)
-            if (lane == from && first + run * j == e) key[j] = 0;
-        sum += s;
-        if (lane == i) {
-            mine = s;
-            myid = e;
+            for (int j = 0; j + 1 < NPL; ++j) {
+                key[j] = pick(taken, key[j + 1], key[j]);
+                slot[j] = pick(taken, slot[j + 1], slot[j]);
+            }
+            key[NPL - 1] = pick(taken, uint64_t(0), key[NPL - 1]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NPL; ++j) key[j] = taken && uint32_t(j) == be ? 0 : key[j];
         }
+        const int e = __builtin_amdgcn_readlane(first + run * int(be), from);
+        if (lane == i) myid = e;
     }
+    // the picks' scores again, all at once
+    double s = 0.0;
+    if (lane < a.k) {
+        const float x = float(lg[myid]), at = x <= kMaxFloat ? x : 0.0f;
+        s = a.sigmoid ? sigmoid(at) : part(at, largest) / denom;
+    }
+    const double sum = wave_sum64(s);
     if (here && lane < a.k) {
-        const double w = a.renorm ? mine / (sum + 1e-20) : mine;
+        const double w = a.renorm ? s / (sum + 1e-20) : s;
         a.ids[t * a.k + lane] = myid;
         a.w[t * a.k + lane] = float(w * double(a.scale));
     }
