@@ -33,22 +33,6 @@ __device__ __forceinline__ float swiglu1(float g, float u, float lim) {
     return __fdiv_rn(g, 1.0f + expf(-g)) * u;
 }
 
-// 16 bytes of a row at k, those from K on zero.
-__device__ __forceinline__ v4i row16(const int8_t* p, int k, int K, bool in) {
-    v4i v{0, 0, 0, 0};
-    if (in && k < K) {
-        v = *reinterpret_cast<const v4i*>(p + k);
-        if (k + 16 > K) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int left = K - k - 4 * i;   // bytes of this word inside the row
-                v[i] &= left >= 4 ? -1 : left <= 0 ? 0 : (1 << (8 * left)) - 1;
-            }
-        }
-    }
-    return v;
-}
-
 // Eight XCDs take workgroups in turn; tile `b` of `n` so that each XCD works on a
 // run of consecutive tiles, and the tiles in groups of `gm` token tiles deep.
 __device__ __forceinline__ void tile_of(int b, int tm, int tn, int& m, int& n) {

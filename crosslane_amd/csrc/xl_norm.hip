@@ -28,7 +28,7 @@ namespace {
 // as of the row itself. KEEP: registers allow that (rows of up to 8192 values, of 16384
 // in 16 bits); else a row's loads follow the row before.
 template <class T, class RT, int R, bool KEEP>
-__global__ __launch_bounds__(1024) void block_norm_kernel(BlockNormArgs a) {
+__global__ __launch_bounds__(1024, R == 1 ? 6 : 4) void block_norm_kernel(BlockNormArgs a) {
     __shared__ float red[2][3][16];
     const int NT = blockDim.x, D = a.D;
     int at[R];
@@ -184,15 +184,23 @@ int row_threads(int n, int per) { return std::min(1024, ((n + per - 1) / per + 6
 template <class T, class RT>
 hipError_t norm_types(const BlockNormArgs& a, int cus, hipStream_t s, hipEvent_t stop) {
     const int chunks = (a.D + 7) / 8;   // at most 4096
-    const auto go = [&](auto kernel, int per) {
-        const int threads = row_threads(chunks, per);
-        // as many workgroups as the CUs hold at a time (24 waves of up to 81 registers): 8192 x
-        // 5120 bf16 in 77 us, with 16 waves 109, with a workgroup for each row 106
-        const int many = cus * std::max(1, 24 * 64 / threads);
-        hipExtLaunchKernelGGL(kernel, dim3(std::min(a.T, many)), dim3(threads), 0, s, nullptr, stop, 0, a);
+    constexpr bool NARROW = sizeof(T) + sizeof(RT) <= 4;   // two chunks for each thread fit its registers with all that is kept
+    // Workgroups that a CU holds: their waves go round its four SIMDs, each workgroup from
+    // the first one on, six to a SIMD with one chunk (80 registers), four with two (128).
+    const auto held = [&](int per) {
+        const int waves = row_threads(chunks, per) / 64, most = per == 1 ? 6 : 4;
+        return waves < 4 ? most * 4 / waves : most / ((waves + 3) / 4);
     };
-    if (chunks <= 1024) go(block_norm_kernel<T, RT, 1, true>, 1);
-    else if (chunks <= 2048) go(block_norm_kernel<T, RT, 2, sizeof(T) + sizeof(RT) <= 4>, 2);
+    // ... are launched, each with several rows: 8192 x 5120 bf16 in 79 us, with half as many
+    // 109, with half as many again 120, with one for each row 106
+    const auto go = [&](auto kernel, int per) {
+        hipExtLaunchKernelGGL(kernel, dim3(std::min(a.T, cus * std::max(1, held(per)))), dim3(row_threads(chunks, per)), 0, s,
+                              nullptr, stop, 0, a);
+    };
+    // two chunks where the CU then holds more rows: 2048 x 4096 to int8 in 19 us for 22, 1024 x 8192 in 17 for 19
+    const bool two = NARROW && chunks > 256 && chunks <= 2048 && held(2) > held(1);
+    if (chunks <= 1024 && !two) go(block_norm_kernel<T, RT, 1, true>, 1);
+    else if (chunks <= 2048) go(block_norm_kernel<T, RT, 2, NARROW>, 2);
     else go(block_norm_kernel<T, RT, 4, false>, 4);
     return hipGetLastError();
 }

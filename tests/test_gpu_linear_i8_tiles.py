@@ -98,3 +98,52 @@ def test_tiles_again(lane, T):
     lane.sync()
     assert torch.equal(outs[0], sums(x, w) * xs[:, None] * ws)
     assert all(torch.equal(outs[0], o) for o in outs[1:])
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("T,K,N,two", [(1, 16384, 130, True), (1, 16385, 130, False), (1, 8200, 33, False), (1, 4097, 4100, True),
+                                       (2, 16384, 70, False), (1, 7, 50, True)])
+def test_rows_quantized_by_the_call(lane, T, K, N, two, kind):
+    """One float row up to 16384 values is quantized inside the product: as the quantizer does it."""
+    print(f"[gpu-step] linear_i8 float row {T} {K} {N} {two} {kind}", flush=True)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(K + N)
+    x = torch.randn((T, K + 5), device="cuda", generator=g).to(TYPES[kind][0])[:, :K]
+    mats = [rows8(N, K, g) for _ in range(2 if two else 1)]
+    ws = [torch.rand(N, device="cuda", generator=g) * 1e-3 for _ in mats]
+    q, qs = torch.zeros((T, (K + 15) // 16 * 16), dtype=torch.int8, device="cuda")[:, :K], torch.zeros(T, device="cuda")
+    work = torch.empty(xl.linear_i8_work_bytes(T, K, N, two), dtype=torch.uint8, device="cuda")
+    outs = [torch.zeros((T, N), device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    up = (mats[1], ws[1]) if two else (None, None)
+    lane.quantize_rows_async(x, q, qs)
+    lane.linear_i8_async(q, mats[0], ws[0], outs[0], x_scale=qs, up=up[0], up_scale=up[1], work=work)
+    lane.linear_i8_async(x, mats[0], ws[0], outs[1], up=up[0], up_scale=up[1], work=work)
+    lane.sync()
+    assert torch.equal(outs[0], outs[1])
+    xf = x.float().cpu().numpy()   # the quantizer in numpy's float32, whose division is IEEE's
+    s = (np.abs(xf).max(1) / np.float32(127)).astype(np.float32)
+    assert np.array_equal(qs.cpu().numpy(), s)
+    assert np.array_equal(q.cpu().numpy(), np.clip(np.rint(xf / s[:, None]), -127, 127).astype(np.int8))
+    if not two:
+        assert torch.equal(outs[0], sums(q, mats[0]) * qs[:, None] * ws[0])
+
+
+def test_quants_next_to_halves(lane):
+    """Values whose quotient lies next to a half, where one reciprocal a row would round wrong."""
+    print("[gpu-step] quantize_rows next to halves", flush=True)
+    rng = np.random.default_rng(9)
+    top = np.exp(rng.standard_normal(64) * 8).astype(np.float32)
+    x = np.zeros((64, 2048), np.float32)
+    half = (rng.integers(-126, 126, (64, 2047)) + 0.5).astype(np.float64)
+    x[:, 1:] = (half * (top[:, None].astype(np.float64) / 127)).astype(np.float32)
+    x[:, 1:] = np.nextafter(x[:, 1:], (rng.integers(0, 2, (64, 2047)) * 2 - 1) * np.float32(np.inf), dtype=np.float32)
+    x[:, 0] = top
+    s = (np.abs(x).max(1) / np.float32(127)).astype(np.float32)
+    want = np.clip(np.rint(x / s[:, None]), -127, 127).astype(np.int8)
+    q, qs = torch.zeros((64, 2048), dtype=torch.int8, device="cuda"), torch.zeros(64, device="cuda")
+    d = torch.from_numpy(x).cuda()
+    torch.cuda.synchronize()
+    lane.quantize_rows_async(d, q, qs)
+    lane.sync()
+    assert np.array_equal(qs.cpu().numpy(), s) and np.array_equal(q.cpu().numpy(), want)
