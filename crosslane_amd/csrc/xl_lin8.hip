@@ -8,7 +8,12 @@
 //
 // v_mfma_i32_16x16x64_i8: lane l holds 16 consecutive k (16 (l / 16) ...) of row
 // l % 16 of either operand, and of the result column l % 16, rows 4 (l / 16) + i.
-// Tokens are the result's rows, channels its columns.
+// Channels are the result's rows, tokens its columns: a lane has neighbouring
+// channels of one token.
+//
+// Two kernels: lin8_rows_kernel for few tokens, bound by the weights' bytes and
+// latency, and lin8_tile_kernel, bound by the matrix cores, or by the bytes that
+// come from L2 to LDS where tiles are small. What they cost stands in kWays.
 #include <hip/hip_ext.h>
 
 #include <algorithm>
@@ -33,8 +38,9 @@ __device__ __forceinline__ float swiglu1(float g, float u, float lim) {
     return __fdiv_rn(g, 1.0f + expf(-g)) * u;
 }
 
-// Eight XCDs take workgroups in turn; tile `b` of `n` so that each XCD works on a
-// run of consecutive tiles, and the tiles in groups of `gm` token tiles deep.
+// Eight XCDs take workgroups in turn. Tile of workgroup b so that each XCD works on a
+// run of consecutive tiles, ordered in groups eight token tiles deep: the 32 workgroups
+// that an XCD's CUs run at a time are 8 x 4 tiles, and its L2 serves four of five reads.
 __device__ __forceinline__ void tile_of(int b, int tm, int tn, int& m, int& n) {
     const int all = tm * tn, x = b & 7, per = all >> 3, rest = all & 7;
     b = x * per + min(x, rest) + (b >> 3);
@@ -45,10 +51,6 @@ __device__ __forceinline__ void tile_of(int b, int tm, int tn, int& m, int& n) {
     n = r / deep;
 }
 
-// TT tokens x TC channels (of each matrix) per workgroup, WT x WC waves. Weights are
-// the first operand: a lane's results are channels 4 q + i of one token. Row m of a
-// wave's tile i is channel 4 NI (m / 4) + 4 i + m % 4 of the wave's, so that a lane has
-// 4 NI consecutive channels and a token's are stored in runs of 16 NI.
 template <int I>
 using index = std::integral_constant<int, I>;
 template <int N, class F>
@@ -68,7 +70,8 @@ __device__ __forceinline__ v4i rows_of(const int8_t* p, int64_t stride, int64_t 
 // register's value nor, for the compiler, an access to LDS: left to it, every read of
 // LDS behind such a load waits for all of them. wait_loads and the barriers here order
 // loads and reads instead; with the "memory" that each names nothing moves across them.
-// (m0 is nobody else's here, and a register that a statement cannot name.)
+// (m0 is nobody else's here, and a register that a statement cannot name. The scalar
+// operands come from the scalar unit, which a vector instruction's would need waits for.)
 __device__ __forceinline__ void buffer16_lds(v4i r, const int8_t* lds, uint32_t voff, int soff) {
     const uint32_t at = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const int8_t*)lds));
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
@@ -91,6 +94,16 @@ __device__ __forceinline__ v4i bytes_below(int n) {
     return m;
 }
 
+// TT tokens x TC channels (of each matrix) per workgroup, WT x WC waves, S stages of
+// 128 bytes of K in LDS, OCC waves to a SIMD. Row m of a wave's tile i is channel
+// 4 NI (m / 4) + 4 i + m % 4 of the wave's, so that a lane has 4 NI consecutive channels
+// and a token's are stored in runs of 16 NI.
+//
+// Loads go straight to LDS: 55 bytes a clock and CU arrive this way where 32 go through
+// registers and ds_write, and rows are loaded in whole 128-byte lines (64-byte pieces: 27).
+// LDS gives 240 a clock to the waves' reads, no bank conflicts. 8192 x 8192 x 8192 takes
+// 414 us (2.66 POP/s of 5; random values, which pull the clock below 2 GHz; all zeros
+// 333 us), 8192 x 5120 x (2 x 4096) with SwiGLU 294 us, by registers 334.
 template <class OT, bool GATED, int TT, int TC, int WT, int WC, int S, int R, int OCC>
 __global__ __launch_bounds__(64 * WT * WC, OCC) void lin8_tile_kernel(Lin8Args a, int tm, int tn) {
     constexpr int BK = 128, NT = 64 * WT * WC, M = GATED ? 2 : 1;
@@ -301,7 +314,12 @@ __device__ __forceinline__ void store4(const Lin8Args& a, int64_t t, int64_t n, 
 // own in LDS (no barrier; loads of whole 128-byte lines go straight there, as in the
 // tile kernel), and their sums are added in LDS at the end.
 // XT: type of x; other than int8, the one row of x is quantized into LDS by every
-// workgroup, while its first weights are on their way.
+// workgroup, while its first weights are on their way (4096 x 5120: 8.1 us, 9.8 with a
+// launch of its own; two rows gain nothing).
+//
+// Bound by the weights' bytes, latency and launch: 4096 x 5120 in 6.1 us for one to 8.1
+// for 64 tokens (21 MB, 4.4 us at the rate of a copy). With the operands straight from
+// memory to registers, 16 rows of 64 bytes an instruction, it was 6.2 and 12.3.
 template <int NI, int NJ, bool GATED, int XT, int NW, int U>
 __global__ __launch_bounds__(64 * NW) void lin8_rows_kernel(Lin8Args a) {
     constexpr int M = GATED ? 2 : 1, NT = 64 * NW, BK = 128;
