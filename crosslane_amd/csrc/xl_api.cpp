@@ -1993,7 +1993,7 @@ int32_t xl_linear_i8_async(xl_context* ctx, const void* d_x, int32_t x_type, con
         if (x_type != XL_I8 && !xl::lin8_quantizes(T, K)) {
             int8_t* q = static_cast<int8_t*>(d_work);
             float* scale = reinterpret_cast<float*>(q + lw.scale);
-            // both launches carry the event: a launch without one after it costs 2 us more
+            // both launches carry the event: 12.9 us a call of 24 x 5120 x (2 x 2304) for 13.7 with the last one alone
             hip_check(xl::dev::launch_quant_rows(d_x, x_type, x_stride, T, K, q, lw.stride, scale, ctx->err_flag, s, ord.stop()),
                       "row quantization launch");
             a.x = q;
