@@ -30,10 +30,12 @@ namespace {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 
+// The clamps are comparisons that a NaN fails, so it stays one: fminf and fmaxf return the
+// other operand, and a row with a NaN scale would come out as finite numbers.
 __device__ __forceinline__ float swiglu1(float g, float u, float lim) {
     if (lim > 0.0f) {
-        g = fminf(g, lim);
-        u = fminf(fmaxf(u, -lim), lim);
+        g = g > lim ? lim : g;
+        u = u > lim ? lim : u < -lim ? -lim : u;
     }
     return __fdiv_rn(g, 1.0f + expf(-g)) * u;
 }

@@ -459,12 +459,13 @@ int32_t xl_quantize_rows_async(xl_context* ctx, const void* d_x, int32_t type, i
  * quantizes it as xl_quantize_rows_async does. w: N rows of K, 16-byte aligned,
  * w_stride a multiple of 16 (each row readable up to the next multiple of 16; what
  * lies between is not used). With d_up (as w, same stride) and d_up_scale: SwiGLU
- * of the two products, limit > 0 clamping g to <= limit and u to [-limit, limit],
- * out = g / (1 + exp(-g)) * u (the gate and up of a shared expert; its output is
- * the row that the layer and grouped calls take as `shared`). out: XL_F32, XL_F16 or
- * XL_BF16, one rounding. K <= 65536, N and T <= 2^19. d_work: 256-byte aligned,
- * xl_linear_i8_work_bytes(T, K, N, gated) bytes (needed whatever x_type is), used
- * during the call only. out and work overlap nothing else. */
+ * of the two products, limit > 0 clamping g to <= limit and u to [-limit, limit]
+ * (a NaN stays a NaN), out = g / (1 + exp(-g)) * u (the gate and up of a shared
+ * expert; its output is the row that the layer and grouped calls take as
+ * `shared`). out: XL_F32, XL_F16 or XL_BF16, one rounding. K <= 65536, N and T <=
+ * 2^19. d_work: 256-byte aligned, xl_linear_i8_work_bytes(T, K, N, gated) bytes
+ * (needed whatever x_type is), used during the call only. out and work overlap
+ * nothing else. */
 uint64_t xl_linear_i8_work_bytes(int32_t T, int32_t K, int32_t N, int32_t gated);
 int32_t xl_linear_i8_async(xl_context* ctx, const void* d_x, int32_t x_type, const float* d_x_scale_or_null,
                            int64_t x_stride, int32_t T, int32_t K, const int8_t* d_w, const float* d_w_scale,
