@@ -316,8 +316,9 @@ __device__ __forceinline__ void store4(const Lin8Args& a, int64_t t, int64_t n, 
 // own in LDS (no barrier; loads of whole 128-byte lines go straight there, as in the
 // tile kernel), and their sums are added in LDS at the end.
 // XT: type of x; other than int8, the one row of x is quantized into LDS by every
-// workgroup, while its first weights are on their way (4096 x 5120: 8.1 us, 9.8 with a
-// launch of its own; two rows gain nothing).
+// workgroup, while its first weights are on their way (4096 x 5120: 7.2 us, 9.8 with a
+// launch of its own; two rows gain nothing). The quants lie on 16 bytes: behind the odd
+// end of the small arrays, every read of them was split (7.9 us; 1024 x 16384 13.9 for 9.7).
 //
 // Bound by the weights' bytes, latency and launch: 4096 x 5120 in 6.1 us for one to 8.1
 // for 64 tokens (21 MB, 4.4 us at the rate of a copy). With the operands straight from
@@ -332,7 +333,7 @@ __global__ __launch_bounds__(64 * NW) void lin8_rows_kernel(Lin8Args a) {
     constexpr int STAGE = (XR + M * NI * 16) * BK, L = STAGE / 1024;
     __shared__ alignas(16) int8_t lds0[NW][STAGE], lds1[NW][STAGE], lds2[U > 2 ? NW : 1][U > 2 ? STAGE : 16], lds3[U > 3 ? NW : 1][U > 3 ? STAGE : 16];
     static_assert(sizeof(lds0) >= size_t(NW) * M * NI * NJ * 1024, "the sums take the first stage's place");
-    extern __shared__ int8_t xq[];                              // FUSED: K rounded up to 128
+    alignas(16) extern __shared__ int8_t xq[];                  // FUSED: K rounded up to 128; read 16 bytes at a time
     __shared__ float red[16], scale1;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, q = lane >> 4;
