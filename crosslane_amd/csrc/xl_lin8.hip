@@ -73,7 +73,8 @@ __device__ __forceinline__ v4i rows_of(const int8_t* p, int64_t stride, int64_t 
 // LDS behind such a load waits for all of them. wait_loads and the barriers here order
 // loads and reads instead; with the "memory" that each names nothing moves across them.
 // (m0 is nobody else's here, and a register that a statement cannot name. The scalar
-// operands come from the scalar unit, which a vector instruction's would need waits for.)
+// operands come from the scalar unit; a vector instruction's would need five wait states,
+// which the compiler does not put before a statement: tests/test_lin8_code.py looks for them.)
 __device__ __forceinline__ void buffer16_lds(v4i r, const int8_t* lds, uint32_t voff, int soff) {
     const uint32_t at = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const int8_t*)lds));
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
