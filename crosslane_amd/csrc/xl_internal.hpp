@@ -178,7 +178,7 @@ constexpr int kTableBytes = kTableIQ1X + 4096 * 8;
 enum : int { kActF32 = 0, kActF16 = 1, kActBF16 = 2, kActI8 = 3 };
 inline int act_bytes(int type) { return type == kActF32 ? 4 : type == kActI8 ? 1 : 2; }
 constexpr int kNormMaxDim = 32768;     // block norm: 1024 threads of 32 values
-constexpr int kScoreMaxExperts = 1024; // scored router: 16 keys per lane
+constexpr int kScoreMaxExperts = 1024; // scored router: at most 32 keys per lane
 constexpr int kLinMaxK = 65536;        // int8 product: 65536 * 2^14 = 2^30 stays inside an int32
 constexpr int kLinMaxT = 1 << 19;      // ... at most this many tokens and channels
 // Whether the int8 product quantizes a float x itself (one row: each workgroup holds
