@@ -105,8 +105,8 @@ __device__ __forceinline__ v4i bytes_below(int n) {
 // Loads go straight to LDS: 55 bytes a clock and CU arrive this way where 32 go through
 // registers and ds_write, and rows are loaded in whole 128-byte lines (64-byte pieces: 27).
 // LDS gives 240 a clock to the waves' reads, no bank conflicts. 8192 x 8192 x 8192 takes
-// 414 us (2.66 POP/s of 5; random values, which pull the clock below 2 GHz; all zeros
-// 333 us), 8192 x 5120 x (2 x 4096) with SwiGLU 294 us, by registers 334.
+// 406 us (2.71 POP/s of 5; random values, which pull the clock below 2 GHz; all zeros
+// 303 us), 8192 x 5120 x (2 x 4096) with SwiGLU 287 us, by registers 334.
 template <class OT, bool GATED, int TT, int TC, int WT, int WC, int S, int R, int OCC>
 __global__ __launch_bounds__(64 * WT * WC, OCC) void lin8_tile_kernel(Lin8Args a, int tm, int tn) {
     constexpr int BK = 128, NT = 64 * WT * WC, M = GATED ? 2 : 1;
@@ -484,9 +484,12 @@ void lin8_rows(const Lin8Args& a, hipStream_t s, hipEvent_t stop) {
 // The ways to run a call, in order of their tiles: tokens, channels (of each of one or
 // two matrices), workgroups that one CU holds, and the microseconds that they take:
 // fixed, and for each 128-byte step of K with the chip mostly idle and with a workgroup
-// on every CU. Fitted to 285 calls of 1 to 8192 tokens, 64 to 8192 k, 100 to 9216
-// channels, one and two matrices, each run all ways: the way of the least estimate is
-// within 0.3 % of the fastest on average and 16 % at most (7.5 for 6.7 us).
+// on every CU. Fitted to calls of 1 to 8192 tokens, 64 to 8192 k, 100 to 9216 channels,
+// one and two matrices. Over 284 of them, each run all ways (in graphs, 16 calls), the way
+// of the least estimate is 0.9 % slower than the fastest on average. Where it errs most:
+// 8192 x (2 x 100) with 1,024 to 2,048 tokens, 14 to 38 % (25.8 for 18.8 us); 5120 x (2 x
+// 4096) with 48 and 64 tokens, 19 and 20 % (13.6 for 11.4); 5120 x 4096 with 17 to 32, 17 to
+// 19 % (7.4 for 6.3). The next one is 9 %.
 struct Way {
     int tokens, one, two, per_cu;   // two 0: one matrix only
     float fixed, idle, busy;

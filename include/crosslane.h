@@ -430,7 +430,8 @@ int32_t xl_route_scored_async(xl_context* ctx, const void* d_logits, int32_t log
  *   a = y;  post_w: a = a / sqrt(mean(a^2) + eps) * post_w    (norm after the block)
  *   r = alpha * res + gate * a                                (residual scale, gate)
  *   pre_w: x = r / sqrt(mean(r^2) + eps) * pre_w              (norm before the next)
- * float32 throughout, x from the unrounded r. y null: r = alpha * res (gate and
+ * float32 throughout (so values whose squares pass its range, above 1.8e19, leave a
+ * norm as 0), x from the unrounded r. y null: r = alpha * res (gate and
  * post_w null too); res null: r = gate * a. gate: T x D, or one row for all tokens
  * (gate_stride 0), or null (1). y, gate and x have element type `type`, res and
  * res_out `res_type`. Outputs, each optional but one needed: res_out (r), x, and q
@@ -457,8 +458,8 @@ int32_t xl_quantize_rows_async(xl_context* ctx, const void* d_x, int32_t type, i
  * w_scale[r], the sum exact in int32. x: int8 (x_type XL_I8, with d_x_scale; 16-byte
  * aligned, x_stride a multiple of 16) or float (d_x_scale null): then the call
  * quantizes it as xl_quantize_rows_async does. w: N rows of K, 16-byte aligned,
- * w_stride a multiple of 16 (each row readable up to the next multiple of 16; what
- * lies between is not used). With d_up (as w, same stride) and d_up_scale: SwiGLU
+ * w_stride a multiple of 16 (each row of w and of an int8 x readable up to the next
+ * multiple of 16; what lies between is not used). With d_up (as w, same stride) and d_up_scale: SwiGLU
  * of the two products, limit > 0 clamping g to <= limit and u to [-limit, limit]
  * (a NaN stays a NaN), out = g / (1 + exp(-g)) * u (the gate and up of a shared
  * expert; its output is the row that the layer and grouped calls take as

@@ -156,3 +156,16 @@ def test_parts_of_the_norm_over_rows_in_turn(lane, D):
         for n in got:
             assert torch.equal(got[n], few[n]), (c.keys(), n)
         assert not (got[names[0]][:, 0].float() == 9).all()
+
+
+def test_values_whose_squares_pass_float32(lane):
+    """Sums of squares are float32: past its range the norm is 0, with values of the other rows as they are."""
+    print("[gpu-step] block_norm, squares past float32", flush=True)
+    D = 100
+    res = torch.ones((3, D), device="cuda")
+    res[1] = 1e20
+    x, one = torch.full((3, D), 9.0, device="cuda"), torch.ones(D, device="cuda")
+    torch.cuda.synchronize()
+    lane.block_norm_async(res, pre_w=one, eps=EPS, x=x)
+    lane.sync()
+    assert not x[1].any() and ((x[[0, 2]].double() - (1 + EPS) ** -0.5).abs() <= 33 * E).all()
