@@ -309,8 +309,9 @@ void drain(xl_context* ctx, hipStream_t s) {
     int flag = 0;
     hip_check(hipMemcpy(&flag, ctx->err_flag, sizeof flag, hipMemcpyDeviceToHost), "error flag read");
     if (flag) {
-        fail(XL_E_DEVICE, "device error flag 0x%x (%s%s%s%s)", flag, (flag & xl::kDevErrExpertId) ? "expert id out of range " : "",
-             (flag & xl::kDevErrNonFinite) ? "non-finite activation " : "", (flag & xl::kDevErrType) ? "bad block type " : "", (flag & xl::kDevErrTimeout) ? "layer wait timeout" : "");
+        fail(XL_E_DEVICE, "device error flag 0x%x (%s%s%s%s%s)", flag, (flag & xl::kDevErrExpertId) ? "expert id out of range " : "",
+             (flag & xl::kDevErrNonFinite) ? "non-finite activation " : "", (flag & xl::kDevErrType) ? "bad block type " : "", (flag & xl::kDevErrTimeout) ? "layer wait timeout " : "",
+             (flag & xl::kDevErrBatch) ? "cache page, length or start out of range" : "");
     }
 }
 
@@ -2002,6 +2003,208 @@ int32_t xl_linear_i8_async(xl_context* ctx, const void* d_x, int32_t x_type, con
             a.x_type = XL_I8;
         }
         hip_check(xl::dev::launch_lin8(a, ctx->cus, s, ord.stop()), "int8 product launch");
+        ord.carried_by_launch(true);   // the launch records the ordering event itself
+    });
+}
+
+// ---- the attention half of a block ---------------------------------------------------
+namespace {
+
+// A batch's numbers, checked.
+xl::KvBatch kv_numbers(const xl_kv_batch* b) {
+    need(b != nullptr, XL_E_ARG, "null batch");
+    need(b->struct_bytes == sizeof(xl_kv_batch), XL_E_VERSION, "xl_kv_batch size mismatch");
+    need(b->head_dim == 64 || b->head_dim == 128 || b->head_dim == 256, XL_E_ARG, "head_dim must be 64, 128 or 256");
+    need(b->kv_heads >= 1 && b->kv_heads <= 256, XL_E_ARG, "kv_heads outside 1..256");
+    need(b->page_tokens >= 16 && b->page_tokens <= 1024 && b->page_tokens % 16 == 0, XL_E_ARG,
+         "page_tokens must be a multiple of 16 up to 1024");
+    need(b->n_pages >= 1 && b->max_pages >= 1 && int64_t(b->max_pages) * b->page_tokens <= (int64_t(1) << 26), XL_E_ARG,
+         "n_pages below 1, or max_pages * page_tokens outside 1..2^26");
+    need(b->n_seqs >= 1 && b->n_seqs <= 65535 && b->rows >= 1 && b->rows <= xl::kLinMaxT, XL_E_ARG,
+         "n_seqs outside 1..65535 or rows outside 1..2^19");
+    need(b->max_rows >= 1 && b->max_rows <= b->rows, XL_E_ARG, "max_rows outside 1..rows");
+    need(b->reserved == 0, XL_E_ARG, "reserved must be 0");
+    xl::KvBatch k{};
+    k.page_stride = b->page_stride;
+    k.table_stride = b->table_stride;
+    k.dim = b->head_dim;
+    k.kv_heads = b->kv_heads;
+    k.page = b->page_tokens;
+    k.n_pages = b->n_pages;
+    k.max_pages = b->max_pages;
+    k.n_seqs = b->n_seqs;
+    k.rows = b->rows;
+    k.max_rows = b->max_rows;
+    k.page_inv = xl::kv_page_inverse(b->page_tokens);
+    return k;
+}
+// What a batch's calls read besides rows.
+struct KvSpans {
+    Span pages, table, lens, starts;
+};
+// The whole batch, checked.
+xl::KvBatch kv_batch(const xl_kv_batch* b, KvSpans& sp) {
+    xl::KvBatch k = kv_numbers(b);
+    need(b->d_pages && b->d_table && b->d_lens && b->d_starts, XL_E_ARG, "null pointer in the batch");
+    const int64_t bytes = int64_t(k.kv_heads) * int64_t(xl_kv_page_bytes(k.page, k.dim));
+    need(k.page_stride >= bytes && k.page_stride % 16 == 0 && k.page_stride <= (int64_t(1) << 40), XL_E_ARG,
+         "page_stride below a page's bytes, not a multiple of 16 or above 2^40");
+    need(reinterpret_cast<uintptr_t>(b->d_pages) % 16 == 0, XL_E_ARG, "pages not 16-byte aligned");
+    check_rows(b->d_table, k.table_stride, k.max_pages, 4, "table");
+    check_rows(b->d_lens, 1, 1, 4, "lens");
+    check_rows(b->d_starts, 1, 1, 4, "starts");
+    k.pages = static_cast<uint8_t*>(b->d_pages);
+    k.table = b->d_table;
+    k.lens = b->d_lens;
+    k.starts = b->d_starts;
+    sp.pages = Span{b->d_pages, uint64_t(k.n_pages - 1) * uint64_t(k.page_stride) + uint64_t(bytes)};
+    sp.table = Span{b->d_table, extent(k.n_seqs, k.max_pages, k.table_stride, 4)};
+    sp.lens = Span{b->d_lens, uint64_t(k.n_seqs) * 4};
+    sp.starts = Span{b->d_starts, uint64_t(k.n_seqs + 1) * 4};
+    return k;
+}
+void check_heads(int32_t q_heads, int32_t kv_heads) {
+    need(q_heads >= 1 && q_heads <= 1024 && q_heads % kv_heads == 0, XL_E_ARG,
+         "q_heads must be a multiple of kv_heads, at most 1024");
+}
+xl::AttendPlan attend_plan_of(const xl::KvBatch& k, int32_t q_heads) {
+    return xl::attend_plan(k.dim, k.kv_heads, q_heads, k.n_seqs, k.rows, k.max_rows, int64_t(k.max_pages) * k.page);
+}
+
+}  // namespace
+
+uint64_t xl_kv_page_bytes(int32_t page_tokens, int32_t head_dim) {
+    if (page_tokens < 16 || page_tokens > 1024 || page_tokens % 16 || (head_dim != 64 && head_dim != 128 && head_dim != 256)) return 0;
+    return uint64_t(page_tokens) * uint64_t(head_dim) * 5 / 4;
+}
+
+int32_t xl_kv_write_async(xl_context* ctx, const xl_kv_batch* batch, const void* d_k, int64_t k_stride, const void* d_v,
+                          int64_t v_stride, int32_t type, const xl_rotary* rotary_or_null, const void* d_q_or_null,
+                          int64_t q_stride, int32_t q_heads, void* d_q_out_or_null, int64_t q_out_stride, void* stream,
+                          xl_error* err) {
+    return guarded(ctx, err, [&] {
+        KvSpans sp;
+        xl::KvBatch b = kv_batch(batch, sp);
+        need(d_k && d_v, XL_E_ARG, "null device pointer");
+        need(float_type(type), XL_E_ARG, "rows must be f32, f16 or bf16");
+        need((d_q_or_null != nullptr) == (d_q_out_or_null != nullptr), XL_E_ARG, "q and q_out come together");
+        need(rotary_or_null || !d_q_or_null, XL_E_ARG, "q without rotary positions");
+        const int es = xl::act_bytes(type);
+        const int64_t kv = int64_t(b.kv_heads) * b.dim;
+        check_rows(d_k, k_stride, kv, es, "k");
+        check_rows(d_v, v_stride, kv, es, "v");
+        const Span k{d_k, extent(b.rows, kv, k_stride, es)}, v{d_v, extent(b.rows, kv, v_stride, es)};
+        Span q{}, q_out{}, freqs{}, positions{};
+        if (d_q_or_null) {
+            check_heads(q_heads, b.kv_heads);
+            const int64_t width = int64_t(q_heads) * b.dim;
+            check_rows(d_q_or_null, q_stride, width, es, "q");
+            check_rows(d_q_out_or_null, q_out_stride, width, es, "q_out");
+            q = Span{d_q_or_null, extent(b.rows, width, q_stride, es)};
+            q_out = Span{d_q_out_or_null, extent(b.rows, width, q_out_stride, es)};
+        }
+        xl::KvRotary r{};
+        if (const xl_rotary* o = rotary_or_null) {
+            need(o->struct_bytes == sizeof(xl_rotary), XL_E_VERSION, "xl_rotary size mismatch");
+            need(o->n_freqs >= 1 && o->n_freqs <= b.dim / 2, XL_E_ARG, "n_freqs outside 1..head_dim / 2");
+            need(o->n_axes >= 1 && o->n_axes <= 3, XL_E_ARG, "n_axes outside 1..3");
+            int64_t sum = 0;
+            for (int i = 0; i < 3; ++i) {
+                need(o->section[i] >= 0 && (i < o->n_axes || o->section[i] == 0), XL_E_ARG, "a section below 0, or past n_axes");
+                sum += o->section[i];
+            }
+            need(sum == o->n_freqs, XL_E_ARG, "the sections do not add up to n_freqs");
+            need(o->reserved == 0, XL_E_ARG, "reserved must be 0");
+            need(o->d_freqs != nullptr, XL_E_ARG, "null device pointer");
+            need(o->d_positions || o->n_axes == 1, XL_E_ARG, "several axes need positions");
+            check_rows(o->d_freqs, 1, 1, 4, "freqs");
+            freqs = Span{o->d_freqs, uint64_t(o->n_freqs) * 4};
+            if (o->d_positions) {
+                check_rows(o->d_positions, o->positions_stride, b.rows, 4, "positions");
+                positions = Span{o->d_positions, extent(o->n_axes, b.rows, o->positions_stride, 4)};
+            }
+            r = xl::KvRotary{o->d_freqs, o->d_positions, o->positions_stride, o->n_freqs, o->interleaved != 0, o->section[0],
+                             o->section[0] + o->section[1]};
+        }
+        check_apart(sp.pages, {sp.table, sp.lens, sp.starts, k, v, q, freqs, positions}, "the cache");
+        check_apart(q_out, {sp.pages, sp.table, sp.lens, sp.starts, k, v, q, freqs, positions}, "q_out");
+        ready(ctx, false);
+        b.err = ctx->err_flag;
+        hipStream_t s = pick_stream(ctx, stream);
+        Ordered ord(ctx, s);
+        const xl::KvRows x{d_k, d_v, d_q_or_null, nullptr, nullptr, d_q_out_or_null, k_stride, v_stride, q_stride, q_out_stride,
+                           type, q_heads};
+        hip_check(xl::dev::launch_kv_write(b, r, x, s, ord.stop()), "cache write launch");
+        ord.carried_by_launch(true);   // the launch records the ordering event itself
+    });
+}
+
+int32_t xl_kv_read_async(xl_context* ctx, const xl_kv_batch* batch, void* d_k, int64_t k_stride, void* d_v,
+                         int64_t v_stride, int32_t type, void* stream, xl_error* err) {
+    return guarded(ctx, err, [&] {
+        KvSpans sp;
+        xl::KvBatch b = kv_batch(batch, sp);
+        need(d_k && d_v, XL_E_ARG, "null device pointer");
+        need(float_type(type), XL_E_ARG, "rows must be f32, f16 or bf16");
+        const int es = xl::act_bytes(type);
+        const int64_t kv = int64_t(b.kv_heads) * b.dim;
+        check_rows(d_k, k_stride, kv, es, "k");
+        check_rows(d_v, v_stride, kv, es, "v");
+        const Span k{d_k, extent(b.rows, kv, k_stride, es)}, v{d_v, extent(b.rows, kv, v_stride, es)};
+        check_apart(k, {sp.pages, sp.table, sp.lens, sp.starts, v}, "k");
+        check_apart(v, {sp.pages, sp.table, sp.lens, sp.starts}, "v");
+        ready(ctx, false);
+        b.err = ctx->err_flag;
+        hipStream_t s = pick_stream(ctx, stream);
+        Ordered ord(ctx, s);
+        const xl::KvRows x{nullptr, nullptr, nullptr, d_k, d_v, nullptr, k_stride, v_stride, 0, 0, type, 0};
+        hip_check(xl::dev::launch_kv_read(b, x, s, ord.stop()), "cache read launch");
+        ord.carried_by_launch(true);   // the launch records the ordering event itself
+    });
+}
+
+uint64_t xl_attention_work_bytes(const xl_kv_batch* batch, int32_t q_heads) {
+    try {
+        const xl::KvBatch b = kv_numbers(batch);
+        check_heads(q_heads, b.kv_heads);
+        return attend_plan_of(b, q_heads).bytes;
+    } catch (...) {
+        return ~uint64_t(0);
+    }
+}
+
+int32_t xl_attention_async(xl_context* ctx, const xl_kv_batch* batch, const void* d_q, int64_t q_stride, int32_t q_heads,
+                           int32_t type, float scale, int32_t window, float softcap, void* d_out, int64_t out_stride,
+                           void* d_work, uint64_t work_bytes, void* stream, xl_error* err) {
+    return guarded(ctx, err, [&] {
+        KvSpans sp;
+        xl::KvBatch b = kv_batch(batch, sp);
+        need(d_q && d_out, XL_E_ARG, "null device pointer");
+        need(type == XL_F16 || type == XL_BF16, XL_E_ARG, "q and out must be f16 or bf16");
+        check_heads(q_heads, b.kv_heads);
+        need(std::isfinite(scale) && std::isfinite(softcap) && softcap >= 0.0f, XL_E_ARG,
+             "scale must be finite, softcap finite and >= 0");
+        need(window >= 0, XL_E_ARG, "window below 0");
+        const int64_t width = int64_t(q_heads) * b.dim;
+        check_rows(d_q, q_stride, width, 2, "q");
+        check_rows(d_out, out_stride, width, 2, "out");
+        const xl::AttendPlan plan = attend_plan_of(b, q_heads);
+        need(work_bytes >= plan.bytes && (d_work || plan.bytes == 0), XL_E_ARG,
+             "workspace smaller than xl_attention_work_bytes(batch, q_heads)");
+        need(reinterpret_cast<uintptr_t>(d_work) % 256 == 0, XL_E_ARG, "workspace not 256-byte aligned");
+        const Span q{d_q, extent(b.rows, width, q_stride, 2)}, out{d_out, extent(b.rows, width, out_stride, 2)};
+        const Span work{plan.bytes ? d_work : nullptr, plan.bytes};
+        check_apart(out, {sp.pages, sp.table, sp.lens, sp.starts, q, work}, "out");
+        check_apart(work, {sp.pages, sp.table, sp.lens, sp.starts, q}, "workspace");
+        ready(ctx, false);
+        b.err = ctx->err_flag;
+        hipStream_t s = pick_stream(ctx, stream);
+        Ordered ord(ctx, s);
+        uint8_t* w = static_cast<uint8_t*>(d_work);
+        const xl::AttendArgs a{b, d_q, d_out, q_stride, out_stride, type, q_heads, q_heads / b.kv_heads, window, scale, softcap,
+                               plan.bytes ? reinterpret_cast<float*>(w + plan.part) : nullptr,
+                               plan.bytes ? reinterpret_cast<float*>(w + plan.part_ml) : nullptr, plan.splits, plan.tiles};
+        hip_check(xl::dev::launch_attend(a, s, ord.stop()), "attention launch");
         ord.carried_by_launch(true);   // the launch records the ordering event itself
     });
 }

@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <cstdint>
 
+#include "xl_kv_index.hpp"
+
 namespace xl {
 
 // Device-side error bits (OR-ed into the context's flag word by kernels).
@@ -12,6 +14,7 @@ enum : int {
     kDevErrNonFinite = 2,    // non-finite activation seen by a quantizer
     kDevErrType = 4,         // a matrix with an unsupported block type
     kDevErrTimeout = 8,      // a bounded wait of a single-launch layer kernel expired
+    kDevErrBatch = 16,       // a page, length or start of a cache batch out of range
 };
 
 // One planar matrix (see plane_layout in xl_format.hpp).
@@ -201,6 +204,36 @@ struct BlockNormArgs {
     float alpha, eps;
     int* err;
 };
+// Calls over a 4-bit cache (xl_kv.hip, xl_attend.hip).
+struct KvRotary {
+    const float* freqs;
+    const int32_t* positions;   // or null: the position in the sequence
+    int64_t positions_stride;
+    int n, interleaved, end0, end1;   // n frequencies (0: none); axis 0 up to end0, axis 1 up to end1
+};
+struct KvRows {                 // rows of one call: k, v and q (q_out) of a write, k and v of a read
+    const void *k, *v, *q;
+    void *k_out, *v_out, *q_out;
+    int64_t k_stride, v_stride, q_stride, q_out_stride;
+    int type, q_heads;
+};
+struct AttendArgs {
+    KvBatch b;
+    const void* q;
+    void* out;
+    int64_t q_stride, out_stride;
+    int type, q_heads, group, window;
+    float scale, softcap;
+    float* part;                // the splits' sums (AttendPlan)
+    float* part_ml;             // and their maxima and sums of exponentials
+    int splits, tiles;          // parts of the tokens; tiles of rows (set by the launch)
+};
+// How an attention call is cut (numbers of the batch alone): see attend_plan in xl_attend.hip.
+struct AttendPlan {
+    int splits = 1, tiles = 1;
+    uint64_t part = 0, part_ml = 0, bytes = 0;   // offsets in the workspace, and its bytes
+};
+AttendPlan attend_plan(int dim, int kv_heads, int q_heads, int n_seqs, int rows, int max_rows, int64_t max_tokens);
 // Router over softmax or sigmoid scores (xl_score.hip).
 struct ScoreArgs {
     const void* logits;
@@ -355,6 +388,10 @@ hipError_t launch_block_norm(const BlockNormArgs& a, int cus, hipStream_t s, hip
 // to the next multiple of 16 are zeroed.
 hipError_t launch_quant_rows(const void* x, int type, int64_t x_stride, int T, int K, int8_t* q, int64_t q_stride,
                              float* scale, int* err, hipStream_t s, hipEvent_t stop);
+// The cache calls (xl_kv.hip) and the attention over the cache (xl_attend.hip).
+hipError_t launch_kv_write(const KvBatch& b, const KvRotary& r, const KvRows& x, hipStream_t s, hipEvent_t stop);
+hipError_t launch_kv_read(const KvBatch& b, const KvRows& x, hipStream_t s, hipEvent_t stop);
+hipError_t launch_attend(const AttendArgs& a, hipStream_t s, hipEvent_t stop);
 hipError_t launch_score_route(const ScoreArgs& a, hipStream_t s, hipEvent_t stop);
 hipError_t launch_lin8(const Lin8Args& a, int cus, hipStream_t s, hipEvent_t stop);
 // h = SwiGLU(g, u) elementwise over n values, with the limit (lim <= 0: none).

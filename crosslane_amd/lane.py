@@ -58,6 +58,20 @@ _i32p = np.ctypeslib.ndpointer(np.int32, flags="C_CONTIGUOUS")
 _u64p = np.ctypeslib.ndpointer(np.uint64, flags="C_CONTIGUOUS")
 _ErrP = C.POINTER(_Err)
 
+
+class _KVBatch(C.Structure):
+    _fields_ = [("struct_bytes", C.c_uint32), ("head_dim", C.c_int32), ("kv_heads", C.c_int32), ("page_tokens", C.c_int32),
+                ("n_pages", C.c_int32), ("max_pages", C.c_int32), ("n_seqs", C.c_int32), ("rows", C.c_int32),
+                ("max_rows", C.c_int32), ("reserved", C.c_int32), ("page_stride", C.c_int64), ("table_stride", C.c_int64),
+                ("pages", _P), ("table", _P), ("lens", _P), ("starts", _P)]
+
+
+class _Rotary(C.Structure):
+    _fields_ = [("struct_bytes", C.c_uint32), ("n_freqs", C.c_int32), ("n_axes", C.c_int32), ("interleaved", C.c_int32),
+                ("section", C.c_int32 * 3), ("reserved", C.c_int32), ("positions_stride", C.c_int64), ("freqs", _P),
+                ("positions", _P)]
+
+
 class _PackMeta(C.Structure):
     _fields_ = [("struct_bytes", C.c_uint32), ("dim", C.c_int32), ("ff", C.c_int32), ("n_layers", C.c_int32),
                 ("n_experts", C.c_int32), ("top_k", C.c_int32), ("swiglu_limit", C.c_float)]
@@ -118,6 +132,12 @@ _SIGNATURES = {
     "xl_linear_i8_work_bytes": (C.c_uint64, [_I32, _I32, _I32, _I32]),
     "xl_linear_i8_async": (_I32, [_P, _P, _I32, _P, C.c_int64, _I32, _I32, _P, _P, _P, _P, C.c_int64, _I32, C.c_float,
                                   _P, _I32, C.c_int64, _P, C.c_uint64, _P, _ErrP]),
+    "xl_kv_page_bytes": (C.c_uint64, [_I32, _I32]),
+    "xl_kv_write_async": (_I32, [_P, _P, _P, C.c_int64, _P, C.c_int64, _I32, _P, _P, C.c_int64, _I32, _P, C.c_int64, _P, _ErrP]),
+    "xl_kv_read_async": (_I32, [_P, _P, _P, C.c_int64, _P, C.c_int64, _I32, _P, _ErrP]),
+    "xl_attention_work_bytes": (C.c_uint64, [_P, _I32]),
+    "xl_attention_async": (_I32, [_P, _P, _P, C.c_int64, _I32, _I32, C.c_float, _I32, C.c_float, _P, C.c_int64, _P, C.c_uint64,
+                                  _P, _ErrP]),
     "xl_profile_begin": (_I32, [_P, _I32, _ErrP]),
     "xl_profile_end": (_I32, [_P, _f32p, _I32, C.POINTER(_I32), C.POINTER(_I32), C.c_char_p, _I32, _ErrP]),
     "xl_profile_timeline": (_I32, [_P, _u64p, _I32, C.POINTER(_I32), _ErrP]),
@@ -275,6 +295,72 @@ def _vec(t, n: int, what: str, kind: int = 0):
     if not (t.is_cuda and t.is_contiguous() and t.numel() == n and _KINDS[t.dtype] == kind):
         _refuse(f"{what}: {n} contiguous values of the right type on the GPU are wanted")
     return t.data_ptr()
+
+
+def _heads(t, what: str, shape):
+    """[rows, heads, head_dim] on the GPU, a row's heads consecutive: address, row stride, element type."""
+    sh, st = t.shape, t.stride()
+    if sh != shape:
+        _refuse(f"{what}: shape {tuple(sh)} where {tuple(shape)} is wanted")
+    if st[2] != 1 or (st[1] != sh[2] and sh[1] != 1):
+        _refuse(f"{what}: a row's heads must be consecutive")
+    if not t.is_cuda:
+        _refuse(f"{what}: not on the GPU")
+    row = st[0]
+    if sh[0] == 1 and row < sh[1] * sh[2]:
+        row = sh[1] * sh[2]
+    return t.data_ptr(), row, _KINDS[t.dtype]
+
+
+def kv_page_bytes(page_tokens: int, head_dim: int) -> int:
+    """Bytes of one kv head in a page of the 4-bit cache (0: not a size it takes)."""
+    return int(lib().xl_kv_page_bytes(page_tokens, head_dim))
+
+
+class KVBatch:
+    """A batch of sequences over a 4-bit cache of keys and values, for `kv_write_async`,
+    `kv_read_async` and `attention_async`.
+
+    cache    uint8 [n_pages, kv_heads, kv_page_bytes(page_tokens, head_dim)], pages at any stride (a
+             multiple of 16 bytes)
+    table    int32 [n_seqs, max_pages]: the pages of each sequence's tokens, in order
+    lens     int32 [n_seqs]: tokens of each sequence, those of the rows among them
+    starts   int32 [n_seqs + 1]: where each sequence's rows begin among the `rows` rows of a
+             call, and behind the last; a sequence's rows are its last tokens
+    max_rows the most rows that a sequence has (default: `rows`)
+
+    It holds addresses, checked once: their contents may change from call to call, and
+    the tensors are kept alive with it. A layer with a cache of its own has a batch of its own."""
+
+    def __init__(self, cache, table, lens, starts, rows: int, head_dim: int, max_rows: Optional[int] = None):
+        sh, st = cache.shape, cache.stride()
+        if len(sh) != 3 or str(cache.dtype) != "torch.uint8" or st[2] != 1 or (st[1] != sh[2] and sh[1] != 1):
+            _refuse("cache: uint8 [n_pages, kv_heads, bytes] with a page's heads consecutive is wanted")
+        if not cache.is_cuda:
+            _refuse("cache: not on the GPU")
+        page = sh[2] * 4 // (5 * head_dim) if head_dim > 0 else 0
+        if page < 1 or kv_page_bytes(page, head_dim) != sh[2]:
+            _refuse(f"cache: {sh[2]} bytes are no page of head_dim {head_dim}")
+        stride = st[0] if sh[0] > 1 else max(st[0], sh[1] * sh[2])
+        tp, ts, tk = _mat(table, "table")
+        if tk != _INT32:
+            _refuse("table: int32 is wanted")
+        n = int(table.shape[0])
+        self.tensors = (cache, table, lens, starts)
+        self.rows, self.kv_heads, self.head_dim, self.page_tokens = int(rows), int(sh[1]), int(head_dim), int(page)
+        self.struct = _KVBatch(C.sizeof(_KVBatch), head_dim, sh[1], page, sh[0], table.shape[1], n, rows,
+                               rows if max_rows is None else max_rows, 0, stride, ts, cache.data_ptr(), tp,
+                               _vec(lens, n, "lens", _INT32), _vec(starts, n + 1, "starts", _INT32))
+        self.ref = C.addressof(self.struct)
+        self._kv_shape = (self.rows, self.kv_heads, self.head_dim)
+
+
+def attention_work_bytes(batch: KVBatch, q_heads: int) -> int:
+    """Workspace bytes attention_async needs for the batch and q_heads heads of q."""
+    need = int(lib().xl_attention_work_bytes(batch.ref, q_heads))
+    if need == 2 ** 64 - 1:
+        _refuse("a batch or a head count that attention does not take")
+    return need
 
 
 def pack_types(pack_dir: str, first_layer: int, n_layers: int, n_experts: int) -> np.ndarray:
@@ -691,6 +777,81 @@ class Lane:
             self._ctx, xp, kind, _vec(x_scale, T, "x_scale"), xs, T, K, wp, _vec(w_scale, N, "w_scale"), up_,
             _vec(up_scale, N, "up_scale"), ws, N, float(limit), op, _act(out, "out"), os_, work.data_ptr(), work.nbytes,
             None if stream is None else int(stream), self._errp), self._err)
+
+    def kv_write_async(self, batch: KVBatch, k, v, q=None, q_out=None, freqs=None, positions=None, sections=None,
+                       interleaved: bool = False, stream=None) -> None:
+        """Rows of k and v [rows, kv_heads, head_dim] into the batch's cache; with freqs
+        [n] (float32, angles a position), k and q [rows, q_heads, head_dim] are turned first, q
+        into q_out. positions: int32 [axes, rows] or [rows] (None: positions in the sequences);
+        sections: how many of the frequencies go by each axis."""
+        kp, ks, kind = _heads(k, "k", batch._kv_shape)
+        vp, vs, vk = _heads(v, "v", batch._kv_shape)
+        if not 0 <= kind < _INT8 or vk != kind:
+            _refuse("k and v must have one element type, f32, f16 or bf16")
+        qp, qs, heads, op, os_ = None, 0, 0, None, 0
+        if q is not None:
+            if q_out is None:
+                _refuse("q needs q_out")
+            heads = q.shape[1] if q.dim() == 3 else 0
+            shape = (batch.rows, heads, batch.head_dim)
+            qp, qs, qk = _heads(q, "q", shape)
+            op, os_, ok = _heads(q_out, "q_out", shape)
+            if qk != kind or ok != kind:
+                _refuse("q and q_out must have k's element type")
+        elif q_out is not None:
+            _refuse("q_out without q")
+        rotary = None
+        if freqs is not None:
+            n = freqs.numel()
+            pp, pstride, axes = None, 0, 1
+            if positions is not None:
+                if positions.dim() == 1:
+                    pp, pstride = _vec(positions, batch.rows, "positions", _INT32), batch.rows
+                else:
+                    axes = positions.shape[0]
+                    pp, pstride, pk = _mat(positions, "positions", (axes, batch.rows))
+                    if pk != _INT32:
+                        _refuse("positions: int32 is wanted")
+            parts = [n] if sections is None else list(sections)
+            if len(parts) != axes or not 1 <= axes <= 3:
+                _refuse("a section for each of one to three axes is wanted")
+            rotary = _Rotary(C.sizeof(_Rotary), n, axes, bool(interleaved), tuple(parts + [0] * (3 - axes)), 0, pstride,
+                             _vec(freqs, n, "freqs"), pp)
+        elif q is not None or positions is not None or sections is not None:
+            _refuse("q, positions and sections go with freqs")
+        _check(lib().xl_kv_write_async(self._ctx, batch.ref, kp, ks, vp, vs, kind, None if rotary is None else C.addressof(rotary),
+                                       qp, qs, heads, op, os_, None if stream is None else int(stream), self._errp), self._err)
+
+    def kv_read_async(self, batch: KVBatch, k, v, stream=None) -> None:
+        """What the batch's cache holds at its rows' positions, into k and v [rows, kv_heads, head_dim]."""
+        kp, ks, kind = _heads(k, "k", batch._kv_shape)
+        vp, vs, vk = _heads(v, "v", batch._kv_shape)
+        if not 0 <= kind < _INT8 or vk != kind:
+            _refuse("k and v must have one element type, f32, f16 or bf16")
+        _check(lib().xl_kv_read_async(self._ctx, batch.ref, kp, ks, vp, vs, kind, None if stream is None else int(stream),
+                                      self._errp), self._err)
+
+    def attention_async(self, batch: KVBatch, q, out, scale: Optional[float] = None, window: int = 0, softcap: float = 0.0,
+                        work=None, stream=None) -> None:
+        """out [rows, q_heads, head_dim] = attention of the rows of q over the batch's cache (f16 or
+        bf16): tokens up to each row's own, with window > 0 the last `window` of them, softcap > 0: scores
+        through softcap * tanh(score / softcap). scale: 1 / sqrt(head_dim) by default. work:
+        attention_work_bytes(batch, q_heads) bytes (None where that is 0)."""
+        heads = q.shape[1] if q.dim() == 3 else 0
+        shape = (batch.rows, heads, batch.head_dim)
+        qp, qs, kind = _heads(q, "q", shape)
+        op, os_, ok = _heads(out, "out", shape)
+        if kind not in (1, 2) or ok != kind:
+            _refuse("q and out must have one element type, f16 or bf16")
+        wp, wb = None, 0
+        if work is not None:
+            if not (work.is_cuda and work.is_contiguous()):
+                _refuse("work: a contiguous GPU buffer is wanted")
+            wb = work.nbytes
+            wp = work.data_ptr() if wb else None
+        _check(lib().xl_attention_async(self._ctx, batch.ref, qp, qs, heads, kind, batch.head_dim ** -0.5 if scale is None else scale,
+                                        window, softcap, op, os_, wp, wb, None if stream is None else int(stream), self._errp),
+               self._err)
 
     def swiglu_async(self, g, u, h, limit: float = 0.0, stream=None) -> None:
         self._call("xl_swiglu_async", _ptr(g), _ptr(u), int(g.numel()), float(limit), _ptr(h),

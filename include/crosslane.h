@@ -474,6 +474,101 @@ int32_t xl_linear_i8_async(xl_context* ctx, const void* d_x, int32_t x_type, con
                            float limit, void* d_out, int32_t out_type, int64_t out_stride, void* d_work,
                            uint64_t work_bytes, void* stream, xl_error* err);
 
+/* ---- the attention half of a block (device pointers) ----------------------------
+ * A cache of pages that holds keys and values in 4 bits, filled with rotary
+ * positions applied, read back, and attended to. No counterpart in the reference
+ * (its dense stage keeps another attention). The calls use neither the bank nor the
+ * context's workspace; element types and strides as in the section above, a row's
+ * heads consecutive (head_dim values each).
+ *
+ * A page holds page_tokens tokens: for each kv head xl_kv_page_bytes(page_tokens,
+ * head_dim) bytes, the heads' parts consecutive. A group of 32 values of a head is
+ * held as m = float16(min), s = float16((max - m) * float(1/15)) and codes
+ * clamp(rint((x - m) * (1 / s)), 0, 15) (s = 0: codes 0), separate float32 roundings, and
+ * stands for s * code + m; values past +-32768 are held as +-32768. A row (a token's
+ * keys, or values, of one head) with an infinity or a NaN sets the device flag and is held as
+ * NaNs. One head's part, P = page_tokens, D = head_dim, G = D / 32:
+ *   keys' codes     P x [4][G] words; word (c, g): dims 32g + 8c ..+7, dim 2i of them
+ *                   in nibble i, dim 2i + 1 in nibble i + 4
+ *   keys' scales    P x [G][2] float16: s, m
+ *   values' codes   P/4 x [D/8][2][2][2] halfwords: [c][b][h][e] has dims 8c + 4h ..+3
+ *                   of token 2b + e of the four, in order
+ *   values' scales  P/4 x [G][2][4] float16: s of the four tokens, then m
+ * A kernel of the caller's own may fill it too, if scales are >= 0 and a row's
+ * scales are either all finite or all the NaN 0x7e00 with m NaN.
+ *
+ * A batch: sequence b has d_lens[b] tokens, token j in page d_table[b * table_stride
+ * + j / page_tokens] at j % page_tokens. Its rows are d_starts[b] .. d_starts[b + 1] - 1
+ * of the call's q, k, v and outputs (n_seqs + 1 starts, ascending), the last tokens of the
+ * sequence: row i of n is at position d_lens[b] - n + i. A row at a position below 0
+ * has no token: nothing is written to the cache for it, and its outputs are zeros.
+ * Rows outside every sequence are not read, nor their outputs written. Sequences may share pages
+ * (a common prefix) that the call does not write; where two tokens of a
+ * write have one place, it ends up with codes and scales of either. A page or a length out of range, or
+ * starts that descend or pass `rows`, set the device flag; what they name is skipped, never
+ * read or written out of bounds. Only entries of the table that a token needs are read. */
+typedef struct xl_kv_batch {
+    uint32_t struct_bytes;   /* sizeof(xl_kv_batch) */
+    int32_t head_dim;        /* 64, 128 or 256 */
+    int32_t kv_heads;        /* 1..256 */
+    int32_t page_tokens;     /* a multiple of 16 up to 1024 */
+    int32_t n_pages;
+    int32_t max_pages;       /* columns of the table; max_pages * page_tokens <= 2^26 */
+    int32_t n_seqs;          /* 1..65535 */
+    int32_t rows;            /* rows of q, k, v and the outputs, 1..2^19 */
+    int32_t max_rows;        /* no sequence has more rows (1..rows); more: the device flag */
+    int32_t reserved;        /* 0 */
+    int64_t page_stride;     /* bytes from page to page, a multiple of 16 */
+    int64_t table_stride;    /* entries from a sequence's row of the table to the next's */
+    void* d_pages;           /* 16-byte aligned */
+    const int32_t* d_table;
+    const int32_t* d_lens;
+    const int32_t* d_starts;
+} xl_kv_batch;
+
+/* Rotary positions: frequency i turns a pair of dims by the angle position * freq[i],
+ * a' = a * cos - b * sin, b' = b * cos + a * sin: the angle in double, its cosine and sine
+ * rounded to float, then separate float32 roundings. Pairs are dims (i, i + n_freqs), or (2i, 2i + 1) with
+ * `interleaved`; dims from 2 * n_freqs on stay. The first section[0] frequencies go by
+ * axis 0's positions, the next section[1] by axis 1's (time, height, width). d_positions: n_axes
+ * rows of one position for each row of q and k; null (one axis): the position in the sequence. */
+typedef struct xl_rotary {
+    uint32_t struct_bytes;   /* sizeof(xl_rotary) */
+    int32_t n_freqs;         /* 1..head_dim / 2, the sum of the sections */
+    int32_t n_axes;          /* 1..3 */
+    int32_t interleaved;
+    int32_t section[3];      /* of the first n_axes, each >= 0; the others 0 */
+    int32_t reserved;        /* 0 */
+    int64_t positions_stride;/* entries from an axis's positions to the next's, >= rows */
+    const float* d_freqs;
+    const int32_t* d_positions;
+} xl_rotary;
+
+/* Bytes of one kv head in a page (0: not a size the cache takes). */
+uint64_t xl_kv_page_bytes(int32_t page_tokens, int32_t head_dim);
+/* The rows' keys (turned by `rotary`, null: as they are) and values into the cache,
+ * and q (turned too) to q_out; q, q_out null: the cache alone (q_out with q, both only with
+ * rotary). k, v: rows of kv_heads heads, q and q_out rows of q_heads. q_out overlaps nothing else. */
+int32_t xl_kv_write_async(xl_context* ctx, const xl_kv_batch* batch, const void* d_k, int64_t k_stride, const void* d_v,
+                          int64_t v_stride, int32_t type, const xl_rotary* rotary_or_null, const void* d_q_or_null,
+                          int64_t q_stride, int32_t q_heads, void* d_q_out_or_null, int64_t q_out_stride, void* stream,
+                          xl_error* err);
+/* What the cache holds at the rows' positions, as floats (one rounding to `type`). */
+int32_t xl_kv_read_async(xl_context* ctx, const xl_kv_batch* batch, void* d_k, int64_t k_stride, void* d_v,
+                         int64_t v_stride, int32_t type, void* stream, xl_error* err);
+/* Attention of the rows over the cache: for each row at position i and head h,
+ *   score_j = scale * q . key_j, with softcap > 0: softcap * tanh(score_j / softcap)
+ *   out = sum_j softmax(score)_j * value_j over j <= i, with window > 0 also j > i - window
+ * keys and values of kv head h / (q_heads / kv_heads) (q_heads a multiple of kv_heads, at most 1024). q and out:
+ * XL_F16 or XL_BF16. Scores, maxima and sums are float32. A token held as NaN makes
+ * the outputs of the rows that see it NaN, of no others; so does a value of q that is not finite for its row and head. d_work: 256-byte aligned,
+ * xl_attention_work_bytes(batch, q_heads) bytes, used during the call only (0 bytes:
+ * may be null). The size goes by the batch's numbers, not by its pointers. out and work overlap nothing else. */
+uint64_t xl_attention_work_bytes(const xl_kv_batch* batch, int32_t q_heads);
+int32_t xl_attention_async(xl_context* ctx, const xl_kv_batch* batch, const void* d_q, int64_t q_stride, int32_t q_heads,
+                           int32_t type, float scale, int32_t window, float softcap, void* d_out, int64_t out_stride,
+                           void* d_work, uint64_t work_bytes, void* stream, xl_error* err);
+
 /* ---- stage profiling --------------------------------------------------------
  * Between xl_profile_begin and xl_profile_end, the first max_calls layer calls
  * record a HIP event before and after each kernel on the stream it runs on
