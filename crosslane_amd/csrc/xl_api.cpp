@@ -2020,8 +2020,8 @@ xl::KvBatch kv_numbers(const xl_kv_batch* b) {
          "page_tokens must be a multiple of 16 up to 1024");
     need(b->n_pages >= 1 && b->max_pages >= 1 && int64_t(b->max_pages) * b->page_tokens <= (int64_t(1) << 26), XL_E_ARG,
          "n_pages below 1, or max_pages * page_tokens outside 1..2^26");
-    need(b->n_seqs >= 1 && b->n_seqs <= 65535 && b->rows >= 1 && b->rows <= xl::kLinMaxT, XL_E_ARG,
-         "n_seqs outside 1..65535 or rows outside 1..2^19");
+    need(b->n_seqs >= 1 && b->n_seqs <= 65535 && b->rows >= 1 && b->rows <= 1 << 24, XL_E_ARG,
+         "n_seqs outside 1..65535 or rows outside 1..2^24");
     need(b->max_rows >= 1 && b->max_rows <= b->rows, XL_E_ARG, "max_rows outside 1..rows");
     need(b->reserved == 0, XL_E_ARG, "reserved must be 0");
     xl::KvBatch k{};
@@ -2189,6 +2189,7 @@ int32_t xl_attention_async(xl_context* ctx, const xl_kv_batch* batch, const void
         check_rows(d_q, q_stride, width, 2, "q");
         check_rows(d_out, out_stride, width, 2, "out");
         const xl::AttendPlan plan = attend_plan_of(b, q_heads);
+        need(plan.groups <= 0x7fffffff, XL_E_ARG, "more workgroups than a launch takes: n_seqs * max_rows * q_heads too large");
         need(work_bytes >= plan.bytes && (d_work || plan.bytes == 0), XL_E_ARG,
              "workspace smaller than xl_attention_work_bytes(batch, q_heads)");
         need(reinterpret_cast<uintptr_t>(d_work) % 256 == 0, XL_E_ARG, "workspace not 256-byte aligned");

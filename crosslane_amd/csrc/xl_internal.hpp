@@ -231,6 +231,7 @@ struct AttendArgs {
 // How an attention call is cut (numbers of the batch alone): see attend_plan in xl_attend.hip.
 struct AttendPlan {
     int splits = 1, tiles = 1;
+    int64_t groups = 1;                          // workgroups of its largest launch
     uint64_t part = 0, part_ml = 0, bytes = 0;   // offsets in the workspace, and its bytes
 };
 AttendPlan attend_plan(int dim, int kv_heads, int q_heads, int n_seqs, int rows, int max_rows, int64_t max_tokens);
