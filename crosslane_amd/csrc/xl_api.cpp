@@ -2204,7 +2204,8 @@ int32_t xl_attention_async(xl_context* ctx, const xl_kv_batch* batch, const void
         uint8_t* w = static_cast<uint8_t*>(d_work);
         const xl::AttendArgs a{b, d_q, d_out, q_stride, out_stride, type, q_heads, q_heads / b.kv_heads, window, scale, softcap,
                                plan.bytes ? reinterpret_cast<float*>(w + plan.part) : nullptr,
-                               plan.bytes ? reinterpret_cast<float*>(w + plan.part_ml) : nullptr, plan.splits, plan.tiles};
+                               plan.bytes ? reinterpret_cast<float*>(w + plan.part_ml) : nullptr, plan.splits, plan.tiles,
+                               plan.few};
         hip_check(xl::dev::launch_attend(a, s, ord.stop()), "attention launch");
         ord.carried_by_launch(true);   // the launch records the ordering event itself
     });

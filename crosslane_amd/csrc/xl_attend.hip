@@ -18,18 +18,20 @@
 namespace xl {
 namespace {
 
+constexpr int kFewRows = 32;      // rows (of a sequence and a kv head) up to which attend_few_kernel takes them
 constexpr int kSplitTokens = 256; // the least tokens that are worth a workgroup of their own
 
 }  // namespace
 
-// Splits: as many workgroups as fill the card four times (1024), where each has kSplitTokens at least.
+// Splits: as many workgroups as fill the card, where each has tokens enough.
 AttendPlan attend_plan(int dim, int kv_heads, int q_heads, int n_seqs, int rows, int max_rows, int64_t max_tokens) {
     AttendPlan p;
-    const int group = q_heads / kv_heads;
-    const int64_t most = int64_t(max_rows) * group;
-    p.tiles = int((most + 15) / 16);
-    const int64_t wgs = int64_t(n_seqs) * kv_heads * p.tiles;
-    const int64_t want = (1024 + wgs - 1) / wgs, can = (max_tokens + kSplitTokens - 1) / kSplitTokens;
+    const int64_t group = q_heads / kv_heads, most = max_rows * group;
+    p.few = most <= kFewRows;
+    p.tiles = p.few ? int((most + 15) / 16) : int((rows * group >> 7) + n_seqs);
+    const int64_t wgs = (p.few ? int64_t(n_seqs) : int64_t(1)) * kv_heads * p.tiles;
+    const int64_t want = p.few ? (1024 + wgs - 1) / wgs : (512 + wgs - 1) / wgs;
+    const int64_t least = p.few ? kSplitTokens : 1024, can = (max_tokens + least - 1) / least;
     p.splits = int(std::max<int64_t>(1, std::min<int64_t>(128, std::min(want, can))));
     p.groups = std::max(wgs * p.splits, int64_t(rows) * q_heads);
     if (p.splits > 1) {
@@ -365,6 +367,284 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
     }
 }
 
+// Many rows: a workgroup has 128 (of one sequence and kv head), its four waves 32 each, and one of `splits` parts
+// of the tokens, TT at a time.
+//
+// Bound by vector instructions: a tile's 16 + 16 products of v_mfma_f32_32x32x16_f16 take a wave 1024 cycles, the softmax of its
+// 32 scores a lane about as many, and its quarter of the tile's codes made float16. So the workgroup makes them once for all its
+// rows, into LDS (keys as rows of dims, values as rows of tokens, the next tile while this one is used), and scores stay in
+// the lanes that need them as weights, as above: values' tokens lie in LDS in the order in which the scores come out.
+template <int D>
+struct Many {
+    static constexpr int TT = 8192 / D;      // tokens of a tile: 16 KiB each of keys and values
+    static constexpr int G = D / 32, C = D / 8, KS = D / 16, NT = D / 32, MT = TT / 32, U = TT / 8;
+    // Places in LDS, in halves: units of eight are spread over the banks.
+    static __device__ __forceinline__ int key(int tok, int unit) { return tok * D + 8 * (unit ^ (tok & (C < 16 ? C - 1 : 15))); }
+    static __device__ __forceinline__ int value(int dim, int unit) {
+        return dim * TT + 8 * (unit ^ ((U >= 8 ? dim ^ dim >> 3 : dim ^ dim >> 2 ^ dim >> 4) & (U - 1)));
+    }
+};
+typedef float f16x __attribute__((ext_vector_type(16)));
+
+template <class T, int D>
+__global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
+    using M = Many<D>;
+    constexpr int TT = M::TT, G = M::G, C = M::C;
+    __shared__ __attribute__((aligned(16))) f16 ksh[2][TT * D];
+    __shared__ __attribute__((aligned(16))) f16 vsh[2][TT * D];
+    __shared__ __attribute__((aligned(16))) uint8_t odd_sh[2][TT / 4];   // of four tokens: held as NaN (bits 0..3), no page (bit 4)
+    const KvBatch& b = a.b;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane >> 5;
+    // Sequence q's tiles are numbered from starts[q] * group / 128 + q on: at least as many numbers as it has tiles. The last ones,
+    // which see the most tokens, go first.
+    uint32_t at = blockIdx.x;
+    const int head = at % b.kv_heads;
+    at /= b.kv_heads;
+    const int split = at % a.splits;
+    const int number = a.tiles - 1 - int(at / a.splits);
+    const auto first_number = [&](int q) { return int(int64_t(b.starts[q]) * a.group >> 7) + q; };
+    int seq = 0;
+    for (int hi = b.n_seqs; hi - seq > 1;) {
+        const int mid = (seq + hi) >> 1;
+        if (first_number(mid) <= number) seq = mid;
+        else hi = mid;
+    }
+    if (blockIdx.x == 0)
+        for (int i = tid; i < b.n_seqs; i += 256)
+            if (seq_rows(b, i).bad) atomicOr(b.err, kDevErrBatch);
+    const SeqRows s = seq_rows(b, seq);
+    const int row0 = 128 * (number - first_number(seq)), rows = min(128, s.n * a.group - row0);
+    if (row0 < 0 || rows <= 0) return;
+    const int before = s.len - s.n;
+    const auto sees = [&](int row) { return before + row / a.group + 1; };   // tokens up to a row's own
+    const auto from = [&](int upto) { return a.window ? max(0, upto - a.window) : 0; };
+    // this lane's row, and the tokens that it sees: lo ..hi - 1; the same for the wave's first and last row, and the workgroup's
+    const int row = row0 + min(32 * wave + (lane & 31), rows - 1), row_t = row / a.group;
+    const int row_h = head * a.group + row - row_t * a.group;
+    const int hi = sees(row), lo = from(hi);
+    const int hi_least = sees(row0 + min(32 * wave, rows - 1)), hi_most = sees(row0 + min(32 * wave + 31, rows - 1));
+    const int lo_least = from(hi_least), lo_most = from(hi_most);
+    const int hi_all = sees(row0 + rows - 1), lo_all = from(sees(row0));
+    const int tile0 = lo_all / TT, tiles = hi_all > lo_all ? (hi_all + TT - 1) / TT - tile0 : 0;
+    const int per = max(1024 / TT, (tiles + a.splits - 1) / a.splits);
+    const int begin = tile0 + split * per, end = tile0 + min(tiles, (split + 1) * per);
+
+    const Slab<D> slab(b.page);
+    const uint8_t* base = b.pages + int64_t(head) * slab.bytes();
+    // this thread's part of a tile: four words of one token's keys, and eight dims of four tokens' values
+    const int k_tok = tid / (C / 4), k_sub = tid % (C / 4), v_quad = tid / C, v_chunk = tid % C;
+    int64_t k_page = -1, v_page = -1;
+    int k_run = 0, v_run = 0;
+    bool k_ok = false, v_ok = false;
+    u4 k_code, v_code, v_scale;
+    uint32_t k_scale[G < 4 ? G : 4];
+    const auto pages = [&](int tl) {   // of the tile's runs; behind the last token: any page
+        const int last = (hi_all - 1) >> 4;
+        k_page = page_at(b, seq, uint32_t(min(tl * (TT / 16) + (k_tok >> 4), last)), k_run);
+        v_page = page_at(b, seq, uint32_t(min(tl * (TT / 16) + (v_quad >> 2), last)), v_run);
+    };
+    const auto fetch = [&] {
+        k_ok = k_page >= 0;
+        v_ok = v_page >= 0;
+        const uint8_t* k = base + (k_ok ? k_page : 0);
+        const uint8_t* v = base + (v_ok ? v_page : 0);
+        const int tok = 16 * k_run + (k_tok & 15), quad = 4 * v_run + (v_quad & 3);
+        __builtin_memcpy(&k_code, __builtin_assume_aligned(k + 4 * (tok * C + 4 * k_sub), 16), 16);
+        __builtin_memcpy(k_scale, __builtin_assume_aligned(k + slab.k_scale(tok, 4 * k_sub % G), sizeof k_scale), sizeof k_scale);
+        __builtin_memcpy(&v_code, __builtin_assume_aligned(v + slab.v_codes() + 2 * (quad * D + v_chunk * 8), 16), 16);
+        __builtin_memcpy(&v_scale, __builtin_assume_aligned(v + slab.v_scales() + 16 * (quad * G + v_chunk / 4), 16), 16);
+    };
+    const auto stage = [&](int tl, int buf) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int w = 4 * k_sub + i, g = w % G, unit = 4 * g + w / G;
+            const h2 sm = as_h2(k_scale[i % (G < 4 ? G : 4)]);
+            h2 k[4];
+            codes8(k_code[i], k);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) k[j] = __builtin_elementwise_fma(k[j], both(sm[0]), both(sm[1]));
+            *reinterpret_cast<h8*>(&ksh[buf][M::key(k_tok, unit)]) = join(k[0], k[1], k[2], k[3]);
+        }
+        // values that no row sees, or whose token is held as NaN, are 0
+        uint32_t sc[4] = {v_scale[0], v_scale[1], v_scale[2], v_scale[3]}, odd = v_ok ? 0u : 16u;
+        const int tok = TT * tl + 4 * v_quad;
+        if (tok + 4 > hi_all || !v_ok || worst(sc[0], sc[1], 0, 0) >= 0x7c00u) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t keep = j & 1 ? 0x0000ffffu : 0xffff0000u;
+                const bool nan = ((j & 1 ? sc[j >> 1] >> 16 : sc[j >> 1]) & 0x7fffu) >= 0x7c00u, none = tok + j >= hi_all || !v_ok;
+                if (nan && !none) odd |= 1u << j;
+                if (nan || none) {
+                    sc[j >> 1] &= keep;
+                    sc[2 + (j >> 1)] &= keep;
+                }
+            }
+        }
+        if (v_chunk == 0) odd_sh[buf][v_quad] = uint8_t(odd);
+        const int unit = 2 * (v_quad >> 2) + (v_quad & 1), half = 4 * (v_quad >> 1 & 1);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            h2 x[4], y[4];
+            codes8(v_code[h], x);
+            codes8(v_code[2 + h], y);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[j] = __builtin_elementwise_fma(x[j], as_h2(sc[0]), as_h2(sc[2]));
+                y[j] = __builtin_elementwise_fma(y[j], as_h2(sc[1]), as_h2(sc[3]));
+                *reinterpret_cast<u2*>(&vsh[buf][M::value(8 * v_chunk + 4 * h + j, unit) + half]) = u2{as_u32(x[j]), as_u32(y[j])};
+            }
+        }
+        if (!(k_ok && v_ok)) atomicOr(b.err, kDevErrBatch);
+    };
+
+    if (begin < end) {
+        pages(begin);
+        fetch();
+        if (begin + 1 < end) pages(begin + 1);
+    }
+    // q: the second operand, row lane % 32, dims 16k + 8c ..+7
+    h8 q[M::KS];
+    bool bad;
+    float up;
+    {
+        const T* p = static_cast<const T*>(a.q) + int64_t(s.first + row_t) * a.q_stride + int64_t(row_h) * D + 8 * c;
+        Eight<T> v[M::KS];
+        float m = 0.0f;
+#pragma unroll
+        for (int k = 0; k < M::KS; ++k) {
+            v[k] = eight(p + 16 * k, 8);
+            float w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = float(v[k].v[i]);
+            m = amax8(w, m);
+        }
+        m = fmaxf(m, __shfl_xor(m, 32));
+        bad = m > 3.402823466e38f;
+        const int e = row_exponent<T>(m);
+        // a scale below 0 turns q, so that the largest product is the largest score; 0 becomes the least that still hides -inf
+        const float scale = a.softcap > 0.0f ? a.scale : a.scale * kLog2e;
+#pragma unroll
+        for (int k = 0; k < M::KS; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float w = __builtin_amdgcn_ldexpf(float(v[k].v[i]), -e);
+                q[k][i] = bad ? f16(0.0f) : f16(scale < 0.0f ? -w : w);
+            }
+        up = fmaxf(__builtin_amdgcn_ldexpf(fabsf(scale), e), 1.17549435e-38f);
+    }
+    const Cap cap{2.0f * kLog2e / a.softcap, a.softcap * kLog2e};
+
+    float top = kLowest, sum = 0.0f;
+    f16x o[M::NT] = {};
+    if (begin < end) {
+        stage(begin, 0);
+        if (begin + 1 < end) fetch();
+        if (begin + 2 < end) pages(begin + 2);
+    }
+    for (int tl = begin; tl < end; ++tl) {
+        const int buf = (tl - begin) & 1;
+        __syncthreads();
+        if (tl + 1 < end) {
+            stage(tl + 1, buf ^ 1);
+            if (tl + 2 < end) fetch();
+            if (tl + 3 < end) pages(tl + 3);
+        }
+        if (TT * tl >= hi_most || TT * (tl + 1) <= lo_least) continue;   // no row of this wave sees the tile
+        f16x x[M::MT];
+#pragma unroll
+        for (int m = 0; m < M::MT; ++m) {
+            x[m] = f16x{};
+#pragma unroll
+            for (int k = 0; k < M::KS; ++k) {
+                const h8 key = *reinterpret_cast<const h8*>(&ksh[buf][M::key(32 * m + (lane & 31), 2 * k + c)]);
+                x[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, q[k], x[m], 0, 0, 0);
+            }
+        }
+        float upx = up;
+        if (a.softcap > 0.0f) {
+#pragma unroll
+            for (int m = 0; m < M::MT; ++m)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[m][i] = cap(x[m][i] * up);
+            upx = 1.0f;
+        }
+        // tokens that some rows do not see, or that are held as NaN or have no page
+        uint32_t odd = 0;
+#pragma unroll
+        for (int i = 0; i < TT / 16; ++i) odd |= reinterpret_cast<const uint32_t*>(odd_sh[buf])[i];
+        if (TT * tl < lo_most || TT * (tl + 1) > hi_least || __builtin_amdgcn_readfirstlane(odd)) {
+#pragma unroll
+            for (int m = 0; m < M::MT; ++m)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int in = 32 * m + 8 * (i >> 2) + 4 * c + (i & 3), tok = TT * tl + in;
+                    const uint32_t e = odd_sh[buf][in >> 2];
+                    if (tok < lo || tok >= hi || e >= 16) x[m][i] = -INFINITY;
+                    else if (e >> (i & 3) & 1) x[m][i] = NAN;
+                }
+        }
+        float most = kLowest;
+#pragma unroll
+        for (int m = 0; m < M::MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) most = fmaxf(most, x[m][i]);
+        most *= upx;
+        if (__any(most > top + kLazy)) {
+            const float m = fmaxf(fmaxf(most, __shfl_xor(most, 32)), top);
+            const float f = __builtin_amdgcn_exp2f(top - m);
+            top = m;
+            sum *= f;
+#pragma unroll
+            for (int n = 0; n < M::NT; ++n) o[n] *= f;
+        }
+        h8 w[TT / 16];
+#pragma unroll
+        for (int m = 0; m < M::MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(x[m][i], upx, -top));
+                sum += p;
+                w[2 * m + (i >> 3)][i & 7] = f16(p);
+            }
+#pragma unroll
+        for (int n = 0; n < M::NT; ++n)
+#pragma unroll
+            for (int k = 0; k < TT / 16; ++k) {
+                const h8 v = *reinterpret_cast<const h8*>(&vsh[buf][M::value(32 * n + (lane & 31), 2 * k + c)]);
+                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w[k], o[n], 0, 0, 0);
+            }
+    }
+
+    sum += __shfl_xor(sum, 32);
+    if (bad && hi > 0) sum = NAN;
+    if (32 * wave + (lane & 31) >= rows) return;
+    const int64_t out_row = int64_t(s.first + row_t);
+    if (a.splits == 1) {
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        T* p = static_cast<T*>(a.out) + out_row * a.out_stride + int64_t(row_h) * D + 4 * c;
+#pragma unroll
+        for (int n = 0; n < M::NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                T v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = T(o[n][4 * i + j] * inv);
+                __builtin_memcpy(p + 32 * n + 8 * i, v, sizeof v);
+            }
+    } else {
+        const int64_t i = (out_row * a.q_heads + row_h) * a.splits + split;
+        float* p = a.part + i * D + 4 * c;
+#pragma unroll
+        for (int n = 0; n < M::NT; ++n)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) *reinterpret_cast<f4*>(p + 32 * n + 8 * k) = f4{o[n][4 * k], o[n][4 * k + 1], o[n][4 * k + 2], o[n][4 * k + 3]};
+        if (c == 0) {
+            a.part_ml[2 * i] = top;
+            a.part_ml[2 * i + 1] = sum;
+        }
+    }
+}
+
 // The splits' sums together: a workgroup for each row and head, threads of D / 4 and of the splits.
 template <class T, int D>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
@@ -399,8 +679,12 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
 
 template <class T, int D>
 hipError_t attend_go(const AttendArgs& a, hipStream_t s, hipEvent_t stop) {
-    const uint32_t grid = uint32_t(a.b.n_seqs) * uint32_t(a.tiles) * uint32_t(a.splits) * uint32_t(a.b.kv_heads);
-    hipExtLaunchKernelGGL((attend_few_kernel<T, D>), dim3(grid), dim3(256), 0, s, nullptr, a.splits == 1 ? stop : nullptr, 0, a);
+    const uint32_t grid = uint32_t(a.few ? a.b.n_seqs : 1) * uint32_t(a.tiles) * uint32_t(a.splits) * uint32_t(a.b.kv_heads);
+    const auto go = [&](auto kernel) {
+        hipExtLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, s, nullptr, a.splits == 1 ? stop : nullptr, 0, a);
+    };
+    if (a.few) go(attend_few_kernel<T, D>);
+    else go(attend_many_kernel<T, D>);
     if (a.splits > 1)
         hipExtLaunchKernelGGL((attend_join_kernel<T, D>), dim3(uint32_t(a.b.rows) * uint32_t(a.q_heads)), dim3(256), 0, s, nullptr, stop, 0, a);
     return hipGetLastError();

@@ -226,11 +226,12 @@ struct AttendArgs {
     float scale, softcap;
     float* part;                // the splits' sums (AttendPlan)
     float* part_ml;             // and their maxima and sums of exponentials
-    int splits, tiles;          // parts of the tokens; tiles of rows (set by the launch)
+    int splits, tiles, few;     // as in AttendPlan
 };
 // How an attention call is cut (numbers of the batch alone): see attend_plan in xl_attend.hip.
 struct AttendPlan {
-    int splits = 1, tiles = 1;
+    int splits = 1, tiles = 1;                   // parts of the tokens; tiles of rows, of a sequence (few) or of all
+    bool few = true;                             // which kernel
     int64_t groups = 1;                          // workgroups of its largest launch
     uint64_t part = 0, part_ml = 0, bytes = 0;   // offsets in the workspace, and its bytes
 };
