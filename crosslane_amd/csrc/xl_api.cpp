@@ -2067,8 +2067,8 @@ void check_heads(int32_t q_heads, int32_t kv_heads) {
     need(q_heads >= 1 && q_heads <= 1024 && q_heads % kv_heads == 0, XL_E_ARG,
          "q_heads must be a multiple of kv_heads, at most 1024");
 }
-xl::AttendPlan attend_plan_of(const xl::KvBatch& k, int32_t q_heads) {
-    return xl::attend_plan(k.dim, k.kv_heads, q_heads, k.n_seqs, k.rows, k.max_rows, int64_t(k.max_pages) * k.page);
+xl::AttendPlan attend_plan_of(const xl::KvBatch& k, int32_t q_heads, int32_t window) {
+    return xl::attend_plan(k.dim, k.kv_heads, q_heads, k.n_seqs, k.rows, k.max_rows, int64_t(k.max_pages) * k.page, window);
 }
 
 }  // namespace
@@ -2167,7 +2167,7 @@ uint64_t xl_attention_work_bytes(const xl_kv_batch* batch, int32_t q_heads) {
     try {
         const xl::KvBatch b = kv_numbers(batch);
         check_heads(q_heads, b.kv_heads);
-        return attend_plan_of(b, q_heads).bytes;
+        return attend_plan_of(b, q_heads, 0).bytes;
     } catch (...) {
         return ~uint64_t(0);
     }
@@ -2188,13 +2188,14 @@ int32_t xl_attention_async(xl_context* ctx, const xl_kv_batch* batch, const void
         const int64_t width = int64_t(q_heads) * b.dim;
         check_rows(d_q, q_stride, width, 2, "q");
         check_rows(d_out, out_stride, width, 2, "out");
-        const xl::AttendPlan plan = attend_plan_of(b, q_heads);
+        const xl::AttendPlan plan = attend_plan_of(b, q_heads, window);
+        const uint64_t whole = attend_plan_of(b, q_heads, 0).bytes;
         need(plan.groups <= 0x7fffffff, XL_E_ARG, "more workgroups than a launch takes: n_seqs * max_rows * q_heads too large");
-        need(work_bytes >= plan.bytes && (d_work || plan.bytes == 0), XL_E_ARG,
+        need(work_bytes >= whole && (d_work || whole == 0), XL_E_ARG,
              "workspace smaller than xl_attention_work_bytes(batch, q_heads)");
         need(reinterpret_cast<uintptr_t>(d_work) % 256 == 0, XL_E_ARG, "workspace not 256-byte aligned");
         const Span q{d_q, extent(b.rows, width, q_stride, 2)}, out{d_out, extent(b.rows, width, out_stride, 2)};
-        const Span work{plan.bytes ? d_work : nullptr, plan.bytes};
+        const Span work{whole ? d_work : nullptr, whole};
         check_apart(out, {sp.pages, sp.table, sp.lens, sp.starts, q, work}, "out");
         check_apart(work, {sp.pages, sp.table, sp.lens, sp.starts, q}, "workspace");
         ready(ctx, false);

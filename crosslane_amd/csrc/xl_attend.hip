@@ -19,20 +19,21 @@ namespace xl {
 namespace {
 
 constexpr int kFewRows = 32;      // rows (of a sequence and a kv head) up to which attend_few_kernel takes them
-constexpr int kSplitTokens = 256; // the least tokens that are worth a workgroup of their own
 
 }  // namespace
 
-// Splits: as many workgroups as fill the card, where each has tokens enough.
-AttendPlan attend_plan(int dim, int kv_heads, int q_heads, int n_seqs, int rows, int max_rows, int64_t max_tokens) {
+// Splits: as many workgroups as the card holds at once (four a CU, two of those that take many rows or heads of 256
+// values), where each has 256 tokens at least (of many rows: 1024), or four times as many for an even end, where each has 1024.
+AttendPlan attend_plan(int dim, int kv_heads, int q_heads, int n_seqs, int rows, int max_rows, int64_t max_tokens, int window) {
     AttendPlan p;
     const int64_t group = q_heads / kv_heads, most = max_rows * group;
     p.few = most <= kFewRows;
     p.tiles = p.few ? int((most + 15) / 16) : int((rows * group >> 7) + n_seqs);
     const int64_t wgs = (p.few ? int64_t(n_seqs) : int64_t(1)) * kv_heads * p.tiles;
-    const int64_t want = p.few ? (1024 + wgs - 1) / wgs : (512 + wgs - 1) / wgs;
-    const int64_t least = p.few ? kSplitTokens : 1024, can = (max_tokens + least - 1) / least;
-    p.splits = int(std::max<int64_t>(1, std::min<int64_t>(128, std::min(want, can))));
+    const int64_t held = p.few && dim < 256 ? 1024 : 512;
+    const int64_t tokens = window ? std::min(max_tokens, int64_t(window) + max_rows) : max_tokens;
+    const auto splits = [&](int64_t groups, int64_t least) { return std::min((groups + wgs - 1) / wgs, (tokens + least - 1) / least); };
+    p.splits = int(std::min<int64_t>(128, std::max<int64_t>(1, p.few ? std::max(splits(held, 256), splits(4 * held, 1024)) : splits(held, 1024))));
     p.groups = std::max(wgs * p.splits, int64_t(rows) * q_heads);
     if (p.splits > 1) {
         const uint64_t parts = uint64_t(rows) * uint64_t(q_heads) * uint64_t(p.splits);
@@ -73,15 +74,13 @@ __device__ __forceinline__ h8 join(h2 a, h2 b, h2 c, h2 d) {
 }
 __device__ __forceinline__ f4 mfma16(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
-// The largest of four pairs of float16 as bit patterns without sign: 0x7c00 and above are no numbers.
-__device__ __forceinline__ uint32_t worst(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    constexpr uint32_t M = 0x7fff7fffu;
-    typedef uint16_t s2 __attribute__((ext_vector_type(2)));
-    const auto most = [](s2 x, s2 y) { return __builtin_elementwise_max(x, y); };
-    const auto v = [](uint32_t x) { return __builtin_bit_cast(s2, x & M); };
-    const s2 m = most(most(v(a), v(b)), most(v(c), v(d)));
-    return max(uint32_t(m[0]), uint32_t(m[1]));
+// Whether any lane has a NaN among four pairs of float16 (sums keep one).
+__device__ __forceinline__ bool has_nan(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    const h2 v = (as_h2(a) + as_h2(b)) + (as_h2(c) + as_h2(d));
+    return __any(v[0] != v[0] || v[1] != v[1]);
 }
+typedef float f2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ h2 pack(float a, float b) { return __builtin_convertvector(f2{a, b}, h2); }
 // Maximum / sum over the four runs of 16 lanes, in every lane.
 __device__ __forceinline__ float rows_max(float v) {
     v = fmaxf(v, __shfl_xor(v, 16));
@@ -108,29 +107,51 @@ __device__ __forceinline__ int row_exponent(float top) {
     return top > 0.0f && top <= 3.402823466e38f ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
 }
 
+// A value of q; a scale below 0 turns it, so that the largest product is the largest score.
+__device__ __forceinline__ f16 turned_q(float v, int e, bool bad, float scale) {
+    const float w = __builtin_amdgcn_ldexpf(v, e);
+    return bad ? f16(0.0f) : f16(scale < 0.0f ? -w : w);
+}
+// What takes a row's products to scores, times log2(e) unless a cap follows: above 0, so that -inf stays hidden.
+__device__ __forceinline__ float row_factor(const AttendArgs& a, int e) {
+    const float scale = fabsf(a.scale) * (a.softcap > 0.0f ? 1.0f : kLog2e);
+    return fmaxf(__builtin_amdgcn_ldexpf(scale, e), 1.17549435e-38f);
+}
+
 // What a lane loads of a tile of 32 tokens (two runs of 16), for keys as the first operand of the scores
 // (token lane % 16 of each run, the eight dims 32g + 8c with c = lane / 16 of every group g), and for values as
-// the first operand of the outputs (dims D / 16 * (lane % 16) on, the four tokens 4c of each run).
+// the first operand of the outputs (dims D / 16 * (lane % 16) on, the four tokens 4c of each run). An address is a
+// run's place, the same for the wave, and an offset of the lane's that stays.
 template <int D>
 struct TileLoads {
     static constexpr int G = D / 32;
-    uint32_t kc[2][G], ks[2][G], vc[2][D >= 128 ? D / 32 : 4];
-    u4 vs[2];
+    uint32_t kc[2][G], ks[2][G], vc[2][D >= 128 ? D / 32 : 4], vs[2][4];
+    uint32_t kc_at, ks_at, vc_at, vs_at;
     template <int N>
     static __device__ __forceinline__ void load(const uint8_t* p, uint32_t (&w)[N]) {
         __builtin_memcpy(w, __builtin_assume_aligned(p, N >= 4 ? 16 : 4 * N), 4 * N);
     }
-    __device__ __forceinline__ void keys(int i, const uint8_t* slab, const Slab<D>& s, int run, int lane) {
-        const int tok = 16 * run + (lane & 15);
-        load(slab + 4 * (tok * (D / 8) + (lane >> 4) * G), kc[i]);
-        load(slab + s.k_scale(tok, 0), ks[i]);
+    __device__ __forceinline__ explicit TileLoads(int lane) {
+        const int tok = lane & 15, c = lane >> 4, chunk = D >= 128 ? tok * (D / 128) : tok >> 1;
+        kc_at = 4 * (tok * (D / 8) + c * G);
+        ks_at = 4 * tok * G;
+        vc_at = 2 * (c * D + chunk * 8);
+        vs_at = 16 * (c * G + chunk / 4);
     }
-    __device__ __forceinline__ void values(int i, const uint8_t* slab, const Slab<D>& s, int run, int lane) {
-        const int quad = 4 * run + (lane >> 4), chunk = D >= 128 ? (lane & 15) * (D / 128) : (lane & 15) >> 1;
-        load(slab + s.v_codes() + 2 * (quad * D + chunk * 8), vc[i]);
-        __builtin_memcpy(&vs[i], __builtin_assume_aligned(slab + s.v_scales() + 16 * (quad * G + chunk / 4), 16), 16);
+    __device__ __forceinline__ void keys(int i, const uint8_t* slab, const Slab<D>& s, int run) {
+        load(slab + 8 * D * run + kc_at, kc[i]);
+        load(slab + s.k_scales() + 64 * G * run + ks_at, ks[i]);
+    }
+    __device__ __forceinline__ void values(int i, const uint8_t* slab, const Slab<D>& s, int run) {
+        load(slab + s.v_codes() + 8 * D * run + vc_at, vc[i]);
+        load(slab + s.v_scales() + 64 * G * run + vs_at, vs[i]);
     }
 };
+
+// A load at an address that is the same for the wave, of memory that the kernel does not write: by the scalar unit.
+__device__ __forceinline__ int scalar_load(const int32_t* p) {
+    return *(const __attribute__((address_space(4))) int32_t*)(reinterpret_cast<uintptr_t>(p));
+}
 
 // Few rows (of one sequence and kv head: its tokens' rows, each with `group` heads): a workgroup has 16 of them and
 // one of `splits` parts of the tokens, its four waves every fourth tile of 32.
@@ -166,29 +187,46 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
     const int lo_all = a.window ? max(0, before + first_t + 1 - a.window) : 0, hi_all = before + last_t + 1;
     const int lo_most = a.window ? max(0, before + last_t + 1 - a.window) : 0, hi_least = before + first_t + 1;
     const int tile0 = lo_all >> 5, tiles = hi_all > lo_all ? ((hi_all + 31) >> 5) - tile0 : 0;
-    const int per = max(kSplitTokens / 32, ((tiles + a.splits - 1) / a.splits + 3) & ~3);
+    const int per = max(8, ((tiles + a.splits - 1) / a.splits + 3) & ~3);
     const int begin = tile0 + split * per + wave, end = tile0 + min(tiles, (split + 1) * per);
 
     const Slab<D> slab(b.page);
     const uint8_t* base = b.pages + int64_t(head) * slab.bytes();
     const int last_run = (hi_all - 1) >> 4;
-    TileLoads<D> t;
-    // a run's page (of the last one where the tile's second run lies behind it); a bad page's tokens are hidden
-    const auto page = [&](int run, int& in, bool& ok) {
-        const int64_t p = page_at(b, seq, uint32_t(min(run, last_run)), in);
-        ok = p >= 0;
-        return base + (ok ? p : 0);
-    };
-    const uint8_t* pg[2];
-    int in[2];
-    bool ok[2];
-    if (begin < end) {
+    TileLoads<D> t(lane);
+    // A tile's pages, by the table's entries, which are read a tile before they are used. Where a tile's second run lies
+    // behind the last token, it is the last run; where an entry is no page, the first page: such tokens are hidden.
+    const int32_t* row_of_table = b.table + int64_t(seq) * b.table_stride;
+    int id[2], in[2];
+    const auto look = [&](int tl) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            pg[i] = page(2 * begin + i, in[i], ok[i]);
-            t.keys(i, pg[i], slab, in[i], lane);
-            t.values(i, pg[i], slab, in[i], lane);
+            const uint32_t run = uint32_t(min(2 * tl + i, last_run));
+            const uint32_t col = b.page_inv ? __umulhi(run, b.page_inv) : run;
+            in[i] = int(run - col * uint32_t(b.page >> 4));
+            id[i] = scalar_load(row_of_table + col);
         }
+    };
+    const uint8_t* pg[2];
+    int run[2];
+    bool ok[2];
+    const auto turn_to = [&] {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            ok[i] = uint32_t(id[i]) < uint32_t(b.n_pages);
+            pg[i] = base + (ok[i] ? int64_t(id[i]) * b.page_stride : 0);
+            run[i] = in[i];
+        }
+    };
+    if (begin < end) {
+        look(begin);
+        turn_to();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            t.keys(i, pg[i], slab, run[i]);
+            t.values(i, pg[i], slab, run[i]);
+        }
+        if (begin + 4 < end) look(begin + 4);
     }
 
     // q: the second operand, row lane % 16, dims 32g + 8c ..+7
@@ -209,19 +247,18 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q[g][i] = bad ? f16(0.0f) : f16(__builtin_amdgcn_ldexpf(v[g][i], -e));
-        up = __builtin_amdgcn_ldexpf(a.softcap > 0.0f ? a.scale : a.scale * kLog2e, e);
+            for (int i = 0; i < 8; ++i) q[g][i] = turned_q(v[g][i], -e, bad, a.scale);
+        up = row_factor(a, e);
     }
     const Cap cap{2.0f * kLog2e / a.softcap, a.softcap * kLog2e};
 
     float top = kLowest, sum = 0.0f;
     f4 o[N] = {};
     for (int tl = begin; tl < end; tl += 4) {
-        const bool more = tl + 4 < end;
-        const bool ok0 = ok[0], ok1 = ok[1];
+        const bool more = tl + 4 < end, ok0 = ok[0], ok1 = ok[1];
         if (more) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) pg[i] = page(2 * (tl + 4) + i, in[i], ok[i]);
+            turn_to();
+            if (tl + 8 < end) look(tl + 8);
         }
         float x[8];
 #pragma unroll
@@ -237,15 +274,17 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
                 acc = mfma16(join(k[0], k[1], k[2], k[3]), q[g], acc);
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[4 * i + j] = acc[j] * up;
+            for (int j = 0; j < 4; ++j) x[4 * i + j] = acc[j];
         }
         if (more) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) t.keys(i, pg[i], slab, in[i], lane);
+            for (int i = 0; i < 2; ++i) t.keys(i, pg[i], slab, run[i]);
         }
+        float upx = up;
         if (a.softcap > 0.0f) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = cap(x[j]);
+            for (int j = 0; j < 8; ++j) x[j] = cap(x[j] * up);
+            upx = 1.0f;
         }
         // the first and last tiles hide tokens from some rows; what no row sees may be anything
         if (32 * tl < lo_most || 32 * tl + 32 > hi_least || !(ok0 && ok1)) {
@@ -255,15 +294,13 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
                 const bool there = j < 4 ? ok0 : ok1;
                 if (tok < lo || tok >= hi || !there) x[j] = -INFINITY;
                 if (tok >= hi_all || !there) {
-                    uint32_t& w0 = reinterpret_cast<uint32_t*>(&t.vs[j >> 2])[(j & 3) >> 1];
-                    uint32_t& w1 = reinterpret_cast<uint32_t*>(&t.vs[j >> 2])[2 + ((j & 3) >> 1)];
-                    w0 &= j & 1 ? 0x0000ffffu : 0xffff0000u;
-                    w1 &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+                    t.vs[j >> 2][(j & 3) >> 1] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+                    t.vs[j >> 2][2 + ((j & 3) >> 1)] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
                 }
             }
             if (lane == 0 && !(ok0 && ok1)) atomicOr(b.err, kDevErrBatch);
         }
-        float m = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        float m = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * upx;
         if (__any(m > top + kLazy)) {
             m = fmaxf(rows_max(m), top);
             const float f = __builtin_amdgcn_exp2f(top - m);
@@ -275,27 +312,24 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
         float p[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            p[j] = __builtin_amdgcn_exp2f(x[j] - top);
+            p[j] = __builtin_amdgcn_exp2f(fmaf(x[j], upx, -top));
             sum += p[j];
         }
         // a token held as NaN: its values as 0, and the rows that see it NaN by their sum
-        {
-            const uint32_t w = worst(t.vs[0][0], t.vs[0][1], t.vs[1][0], t.vs[1][1]);
-            if (__any(w >= 0x7c00u)) {
+        if (has_nan(t.vs[0][0], t.vs[0][1], t.vs[1][0], t.vs[1][1])) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    uint32_t& w0 = reinterpret_cast<uint32_t*>(&t.vs[j >> 2])[(j & 3) >> 1];
-                    uint32_t& w1 = reinterpret_cast<uint32_t*>(&t.vs[j >> 2])[2 + ((j & 3) >> 1)];
-                    const uint32_t e = (j & 1 ? w0 >> 16 : w0) & 0x7fffu;
-                    if (e >= 0x7c00u) {
-                        w0 &= j & 1 ? 0x0000ffffu : 0xffff0000u;
-                        w1 &= j & 1 ? 0x0000ffffu : 0xffff0000u;
-                        if (x[j] != -INFINITY) sum = NAN;
-                    }
+            for (int j = 0; j < 8; ++j) {
+                uint32_t& w0 = t.vs[j >> 2][(j & 3) >> 1];
+                uint32_t& w1 = t.vs[j >> 2][2 + ((j & 3) >> 1)];
+                const uint32_t e = (j & 1 ? w0 >> 16 : w0) & 0x7fffu;
+                if (e >= 0x7c00u) {
+                    w0 &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+                    w1 &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+                    if (x[j] != -INFINITY) sum = NAN;
                 }
             }
         }
-        const h8 w = {f16(p[0]), f16(p[1]), f16(p[2]), f16(p[3]), f16(p[4]), f16(p[5]), f16(p[6]), f16(p[7])};
+        const h8 w = join(pack(p[0], p[1]), pack(p[2], p[3]), pack(p[4], p[5]), pack(p[6], p[7]));
         // words of two tokens: [run][pair of the four][half of the chunk], four dims each
 #pragma unroll
         for (int n = 0; n < N / 4; ++n) {
@@ -318,7 +352,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
         }
         if (more) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) t.values(i, pg[i], slab, in[i], lane);
+            for (int i = 0; i < 2; ++i) t.values(i, pg[i], slab, run[i]);
         }
     }
 
@@ -468,7 +502,7 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
         // values that no row sees, or whose token is held as NaN, are 0
         uint32_t sc[4] = {v_scale[0], v_scale[1], v_scale[2], v_scale[3]}, odd = v_ok ? 0u : 16u;
         const int tok = TT * tl + 4 * v_quad;
-        if (tok + 4 > hi_all || !v_ok || worst(sc[0], sc[1], 0, 0) >= 0x7c00u) {
+        if (tok + 4 > hi_all || !v_ok || has_nan(sc[0], sc[1], 0, 0)) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const uint32_t keep = j & 1 ? 0x0000ffffu : 0xffff0000u;
@@ -521,16 +555,11 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
         m = fmaxf(m, __shfl_xor(m, 32));
         bad = m > 3.402823466e38f;
         const int e = row_exponent<T>(m);
-        // a scale below 0 turns q, so that the largest product is the largest score; 0 becomes the least that still hides -inf
-        const float scale = a.softcap > 0.0f ? a.scale : a.scale * kLog2e;
 #pragma unroll
         for (int k = 0; k < M::KS; ++k)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float w = __builtin_amdgcn_ldexpf(float(v[k].v[i]), -e);
-                q[k][i] = bad ? f16(0.0f) : f16(scale < 0.0f ? -w : w);
-            }
-        up = fmaxf(__builtin_amdgcn_ldexpf(fabsf(scale), e), 1.17549435e-38f);
+            for (int i = 0; i < 8; ++i) q[k][i] = turned_q(float(v[k].v[i]), -e, bad, a.scale);
+        up = row_factor(a, e);
     }
     const Cap cap{2.0f * kLog2e / a.softcap, a.softcap * kLog2e};
 
@@ -602,10 +631,15 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
         for (int m = 0; m < M::MT; ++m)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(x[m][i], upx, -top));
-                sum += p;
-                w[2 * m + (i >> 3)][i & 7] = f16(p);
+                x[m][i] = __builtin_amdgcn_exp2f(fmaf(x[m][i], upx, -top));
+                sum += x[m][i];
             }
+#pragma unroll
+        for (int k = 0; k < TT / 16; ++k) {
+            const f16x& y = x[k >> 1];
+            const int i = 8 * (k & 1);
+            w[k] = join(pack(y[i], y[i + 1]), pack(y[i + 2], y[i + 3]), pack(y[i + 4], y[i + 5]), pack(y[i + 6], y[i + 7]));
+        }
 #pragma unroll
         for (int n = 0; n < M::NT; ++n)
 #pragma unroll
@@ -645,36 +679,69 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
     }
 }
 
-// The splits' sums together: a workgroup for each row and head, threads of D / 4 and of the splits.
-template <class T, int D>
+// The splits' sums together: W waves for each row and head, 256 / D splits of them at a time in a wave. A wave has
+// the splits' maxima and sums in its lanes (two each: at most 128), and their weights from there.
+template <class T, int D, int W>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
-    constexpr int L = D / 4, W = 256 / L;   // threads of one split's row, splits at a time
-    __shared__ f4 sums[W][L];
-    const int64_t row = blockIdx.x;
+    constexpr int L = D / 4, P = 64 / L;   // lanes of one split's row, splits at a time
+    __shared__ f4 sums[4][L];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % W;
+    const int64_t row = int64_t(blockIdx.x) * (4 / W) + wave / W;
     const int t = int(row / a.q_heads), h = int(row - int64_t(t) * a.q_heads);
     // rows of no sequence have no parts
-    const SeqRows s = seq_rows(a.b, seq_of(a.b, t));
-    if (t < s.first || t >= s.first + s.n) return;
-    const float* ml = a.part_ml + 2 * row * a.splits;
-    float most = kLowest, total = 0.0f;
-    for (int i = 0; i < a.splits; ++i) most = fmaxf(most, ml[2 * i]);
-    for (int i = 0; i < a.splits; ++i) total += ml[2 * i + 1] * __builtin_amdgcn_exp2f(ml[2 * i] - most);
-    const int w = threadIdx.x / L, d = threadIdx.x % L;
-    f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i = w; i < a.splits; i += W) {
-        if (ml[2 * i + 1] == 0.0f) continue;
-        y += *reinterpret_cast<const f4*>(a.part + (row * a.splits + i) * D + 4 * d) * __builtin_amdgcn_exp2f(ml[2 * i] - most);
+    bool there = t < a.b.rows;
+    if (there) {
+        const SeqRows s = seq_rows(a.b, seq_of(a.b, t));
+        there = t >= s.first && t < s.first + s.n;
     }
-    sums[w][d] = y;
-    __syncthreads();
-    if (w) return;
+    f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+    float total = 0.0f;
+    if (there) {
+        const f2* ml = reinterpret_cast<const f2*>(a.part_ml) + row * a.splits;
+        const f2 none = {kLowest, 0.0f};
+        const f2 u = lane < a.splits ? ml[lane] : none, v = lane + 64 < a.splits ? ml[lane + 64] : none;
+        float most = fmaxf(u[0], v[0]);
 #pragma unroll
-    for (int i = 1; i < W; ++i) y += sums[i][d];
+        for (int i = 32; i; i >>= 1) most = fmaxf(most, __shfl_xor(most, i));
+        const float fu = __builtin_amdgcn_exp2f(u[0] - most), fv = __builtin_amdgcn_exp2f(v[0] - most);
+        total = u[1] * fu + v[1] * fv;
+#pragma unroll
+        for (int i = 32; i; i >>= 1) total += __shfl_xor(total, i);
+        const int d = lane % L;
+        const float* p = a.part + row * a.splits * D + 4 * d;
+        for (int k = part * P; k < a.splits; k += 8 * W * P) {   // eight loads on their way
+            f4 x[8];
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int i = k + j * W * P + lane / L, in = min(i, a.splits - 1);
+                x[j] = *reinterpret_cast<const f4*>(p + int64_t(in) * D);
+                const float f0 = __shfl(fu, in & 63), f1 = __shfl(fv, in & 63);
+                f[j] = i >= a.splits ? 0.0f : in < 64 ? f0 : f1;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y += x[j] * f[j];
+        }
+#pragma unroll
+        for (int i = L; i < 64; i <<= 1)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] += __shfl_xor(y[j], i);
+    }
+    if constexpr (W > 1) {
+        if (lane < L) sums[wave][lane] = y;
+        __syncthreads();
+        if (wave) return;
+        if (lane < L) {
+#pragma unroll
+            for (int i = 1; i < W; ++i) y += sums[i][lane];
+        }
+    }
+    if (!there || lane >= L) return;
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     T v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = T(y[i] * inv);
-    __builtin_memcpy(static_cast<T*>(a.out) + int64_t(t) * a.out_stride + int64_t(h) * D + 4 * d, v, sizeof v);
+    __builtin_memcpy(static_cast<T*>(a.out) + int64_t(t) * a.out_stride + int64_t(h) * D + 4 * lane, v, sizeof v);
 }
 
 template <class T, int D>
@@ -685,8 +752,14 @@ hipError_t attend_go(const AttendArgs& a, hipStream_t s, hipEvent_t stop) {
     };
     if (a.few) go(attend_few_kernel<T, D>);
     else go(attend_many_kernel<T, D>);
-    if (a.splits > 1)
-        hipExtLaunchKernelGGL((attend_join_kernel<T, D>), dim3(uint32_t(a.b.rows) * uint32_t(a.q_heads)), dim3(256), 0, s, nullptr, stop, 0, a);
+    if (a.splits > 1) {
+        const int64_t heads = int64_t(a.b.rows) * a.q_heads;
+        const auto join = [&](auto kernel, int w) {
+            hipExtLaunchKernelGGL(kernel, dim3(uint32_t((heads * w + 3) / 4)), dim3(256), 0, s, nullptr, stop, 0, a);
+        };
+        if (a.splits > 16) join(attend_join_kernel<T, D, 4>, 4);
+        else join(attend_join_kernel<T, D, 1>, 1);
+    }
     return hipGetLastError();
 }
 template <class T>

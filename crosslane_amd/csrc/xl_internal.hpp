@@ -235,7 +235,8 @@ struct AttendPlan {
     int64_t groups = 1;                          // workgroups of its largest launch
     uint64_t part = 0, part_ml = 0, bytes = 0;   // offsets in the workspace, and its bytes
 };
-AttendPlan attend_plan(int dim, int kv_heads, int q_heads, int n_seqs, int rows, int max_rows, int64_t max_tokens);
+AttendPlan attend_plan(int dim, int kv_heads, int q_heads, int n_seqs, int rows, int max_rows, int64_t max_tokens, int window);
+// The same with a window never takes more of the workspace.
 // Router over softmax or sigmoid scores (xl_score.hip).
 struct ScoreArgs {
     const void* logits;
