@@ -61,14 +61,19 @@ __device__ __forceinline__ uint32_t as_u32(h2 v) { return __builtin_bit_cast(uin
 __device__ __forceinline__ h2 both(f16 v) { return h2{v, v}; }
 
 // Nibbles 0 and 4, 1 and 5, 2 and 6, 3 and 7 of a word, as pairs of whole numbers in float16: a nibble
-// under the exponent of 1024 is 1024 + code, four bits higher under that of 64 it is 64 + code.
-__device__ __forceinline__ void codes8(uint32_t w, h2 (&c)[4]) {
-    const uint32_t u = w >> 8;
-    c[0] = as_h2((w & 0x000f000fu) | 0x64006400u) - both(f16(1024.0f));
-    c[1] = as_h2((w & 0x00f000f0u) | 0x54005400u) - both(f16(64.0f));
-    c[2] = as_h2((u & 0x000f000fu) | 0x64006400u) - both(f16(1024.0f));
-    c[3] = as_h2((u & 0x00f000f0u) | 0x54005400u) - both(f16(64.0f));
-}
+// under the exponent of 1024 is 1024 + code, four bits higher under that of 64 it is 64 + code. The masks lie in
+// vector registers and the exponents in scalar ones: an instruction takes no two constants, but so it is v_and_or_b32.
+struct Codes {
+    uint32_t low = 0x000f000fu, high = 0x00f000f0u, e1024 = 0x64006400u, e64 = 0x54005400u;
+    __device__ __forceinline__ Codes() { asm("" : "+v"(low), "+v"(high), "+s"(e1024), "+s"(e64)); }
+    __device__ __forceinline__ void operator()(uint32_t w, h2 (&c)[4]) const {
+        const uint32_t u = w >> 8;
+        c[0] = as_h2((w & low) | e1024) - both(f16(1024.0f));
+        c[1] = as_h2((w & high) | e64) - both(f16(64.0f));
+        c[2] = as_h2((u & low) | e1024) - both(f16(1024.0f));
+        c[3] = as_h2((u & high) | e64) - both(f16(64.0f));
+    }
+};
 __device__ __forceinline__ h8 join(h2 a, h2 b, h2 c, h2 d) {
     return __builtin_bit_cast(h8, u4{as_u32(a), as_u32(b), as_u32(c), as_u32(d)});
 }
@@ -98,24 +103,42 @@ struct Cap {
     }
 };
 
-// Rows of q in float16. A bfloat16 row is taken times a power of two that brings its largest value to 1..2, so
-// that float16 holds all its bits, down to 2^-25 of that value; `up` is that power's inverse. A row with a value that is not
-// finite is 0 here and `bad`.
-template <class T>
-__device__ __forceinline__ int row_exponent(float top) {
-    if (sizeof(T) == 2 && __is_same(T, f16)) return 0;
-    return top > 0.0f && top <= 3.402823466e38f ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
-}
-
-// A value of q; a scale below 0 turns it, so that the largest product is the largest score.
-__device__ __forceinline__ f16 turned_q(float v, int e, bool bad, float scale) {
-    const float w = __builtin_amdgcn_ldexpf(v, e);
-    return bad ? f16(0.0f) : f16(scale < 0.0f ? -w : w);
-}
-// What takes a row's products to scores, times log2(e) unless a cap follows: above 0, so that -inf stays hidden.
-__device__ __forceinline__ float row_factor(const AttendArgs& a, int e) {
-    const float scale = fabsf(a.scale) * (a.softcap > 0.0f ? 1.0f : kLog2e);
-    return fmaxf(__builtin_amdgcn_ldexpf(scale, e), 1.17549435e-38f);
+// A lane's part of a row of q in float16 (K chunks of eight values), which `most` joins with the row's other lanes; a scale
+// below 0 turns it, so that the largest product is the largest score. A bfloat16 row is taken times a power of two that
+// brings its largest value to 1..2, so that float16 holds all its bits, down to 2^-25 of that value. A row with a value that is
+// not finite is all NaN. Returns what takes its products to scores, times log2(e) unless a cap follows: above 0, so that
+// -inf stays hidden.
+template <class T, int K, class F>
+__device__ __forceinline__ float take_q(const AttendArgs& a, const T* p, int stride, h8 (&q)[K], F&& most) {
+    typedef uint16_t s2 __attribute__((ext_vector_type(2)));
+    u4 w[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) __builtin_memcpy(&w[k], p + k * stride, 16);
+    s2 m = {0, 0};   // magnitudes order as their bits
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(s2, w[k][i] & 0x7fff7fffu));
+    const uint32_t top = most(max(uint32_t(m[0]), uint32_t(m[1])));
+    constexpr bool BF = __is_same(T, bf16);
+    const bool bad = top >= (BF ? 0x7f80u : 0x7c00u);
+    const int e = BF ? (top < 0x80u ? -126 : int(top >> 7) - 127) : 0;   // (subnormal rows: as the smallest normal ones)
+    const float sign = bad ? NAN : a.scale < 0.0f ? -1.0f : 1.0f;
+    if constexpr (BF) {
+        const float f = __builtin_amdgcn_ldexpf(sign, -e);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            h2 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = pack(__uint_as_float(w[k][i] << 16) * f, __uint_as_float(w[k][i] & 0xffff0000u) * f);
+            q[k] = join(v[0], v[1], v[2], v[3]);
+        }
+    } else {
+        const h2 f = both(f16(sign));
+#pragma unroll
+        for (int k = 0; k < K; ++k) q[k] = join(as_h2(w[k][0]) * f, as_h2(w[k][1]) * f, as_h2(w[k][2]) * f, as_h2(w[k][3]) * f);
+    }
+    return fmaxf(__builtin_amdgcn_ldexpf(fabsf(a.scale) * (a.softcap > 0.0f ? 1.0f : kLog2e), e), 1.17549435e-38f);
 }
 
 // What a lane loads of a tile of 32 tokens (two runs of 16), for keys as the first operand of the scores
@@ -194,6 +217,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
     const uint8_t* base = b.pages + int64_t(head) * slab.bytes();
     const int last_run = (hi_all - 1) >> 4;
     TileLoads<D> t(lane);
+    const Codes codes;
     // A tile's pages, by the table's entries, which are read a tile before they are used. Where a tile's second run lies
     // behind the last token, it is the last run; where an entry is no page, the first page: such tokens are hidden.
     const int32_t* row_of_table = b.table + int64_t(seq) * b.table_stride;
@@ -231,25 +255,11 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
 
     // q: the second operand, row lane % 16, dims 32g + 8c ..+7
     h8 q[G];
-    bool bad;
-    float up;
-    {
-        const T* p = static_cast<const T*>(a.q) + int64_t(s.first + row_t) * a.q_stride + int64_t(row_h) * D + 8 * c;
-        float v[G][8], m = 0.0f;
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            load8(p + 32 * g, 8, v[g]);
-            m = amax8(v[g], m);
-        }
-        m = rows_max(m);
-        bad = m > 3.402823466e38f;
-        const int e = row_exponent<T>(m);
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) q[g][i] = turned_q(v[g][i], -e, bad, a.scale);
-        up = row_factor(a, e);
-    }
+    const float up = take_q(a, static_cast<const T*>(a.q) + int64_t(s.first + row_t) * a.q_stride + int64_t(row_h) * D + 8 * c, 32, q,
+                            [](uint32_t v) {
+                                v = max(v, uint32_t(__shfl_xor(int(v), 16)));
+                                return max(v, uint32_t(__shfl_xor(int(v), 32)));
+                            });
     const Cap cap{2.0f * kLog2e / a.softcap, a.softcap * kLog2e};
 
     float top = kLowest, sum = 0.0f;
@@ -268,7 +278,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
             for (int g = 0; g < G; ++g) {
                 const h2 sm = as_h2(t.ks[i][g]), step = both(sm[0]), small = both(sm[1]);
                 h2 k[4];
-                codes8(t.kc[i][g], k);
+                codes(t.kc[i][g], k);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) k[j] = __builtin_elementwise_fma(k[j], step, small);
                 acc = mfma16(join(k[0], k[1], k[2], k[3]), q[g], acc);
@@ -342,7 +352,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
                     if constexpr (D == 64) word = lane & 1 ? t.vc[i][2 * k + 1] : t.vc[i][2 * k];
                     else word = t.vc[i][(n >> 1) * 4 + 2 * k + (n & 1)];
                     h2 code[4];
-                    codes8(word, code);
+                    codes(word, code);
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         v[2 * i + k][j] = __builtin_elementwise_fma(code[j], as_h2(t.vs[i][k]), as_h2(t.vs[i][2 + k]));
@@ -373,7 +383,6 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
 #pragma unroll
         for (int n = 0; n < N; ++n) at_row[n] = o[n][i] * f;
     }
-    if (bad && hi > 0 && lane < 16) sum_sh[wave][lane] = NAN;
     __syncthreads();
     const int r = threadIdx.x >> 4, d = (threadIdx.x & 15) * N;
     if (r >= rows) return;
@@ -411,22 +420,21 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
 template <int D>
 struct Many {
     static constexpr int TT = 8192 / D;      // tokens of a tile: 16 KiB each of keys and values
-    static constexpr int G = D / 32, C = D / 8, KS = D / 16, NT = D / 32, MT = TT / 32, U = TT / 8;
-    // Places in LDS, in halves: units of eight are spread over the banks.
-    static __device__ __forceinline__ int key(int tok, int unit) { return tok * D + 8 * (unit ^ (tok & (C < 16 ? C - 1 : 15))); }
-    static __device__ __forceinline__ int value(int dim, int unit) {
-        return dim * TT + 8 * (unit ^ ((U >= 8 ? dim ^ dim >> 3 : dim ^ dim >> 2 ^ dim >> 4) & (U - 1)));
-    }
+    static constexpr int G = D / 32, C = D / 8, KS = D / 16, NT = D / 32, MT = TT / 32;
+    // Rows in LDS are 16 bytes longer than their values, so that eight lanes' 16 bytes of eight rows lie in banks of their own. A
+    // value's row is (dim % 8) * C + dim / 8: the lanes that write, of chunks of eight dims, have neighbouring rows then.
+    static constexpr int KP = D + 8, VP = TT + 8;
 };
 typedef float f16x __attribute__((ext_vector_type(16)));
 
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
     using M = Many<D>;
-    constexpr int TT = M::TT, G = M::G, C = M::C;
-    __shared__ __attribute__((aligned(16))) f16 ksh[2][TT * D];
-    __shared__ __attribute__((aligned(16))) f16 vsh[2][TT * D];
-    __shared__ __attribute__((aligned(16))) uint8_t odd_sh[2][TT / 4];   // of four tokens: held as NaN (bits 0..3), no page (bit 4)
+    constexpr int TT = M::TT, G = M::G, C = M::C, KP = M::KP, VP = M::VP, RW = D == 64 ? 2 : 1;
+    __shared__ __attribute__((aligned(16))) f16 ksh[2][TT * KP];
+    __shared__ __attribute__((aligned(16))) f16 vsh[2][D * VP];
+    __shared__ uint8_t odd_sh[2][TT / 4];   // of four tokens: held as NaN (bits 0..3), no page (bit 4)
+    __shared__ int odd_tile[2];             // the last tile that had such tokens
     const KvBatch& b = a.b;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane >> 5;
     // Sequence q's tiles are numbered from starts[q] * group / 128 + q on: at least as many numbers as it has tiles. The last ones,
@@ -436,7 +444,7 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
     at /= b.kv_heads;
     const int split = at % a.splits;
     const int number = a.tiles - 1 - int(at / a.splits);
-    const auto first_number = [&](int q) { return int(int64_t(b.starts[q]) * a.group >> 7) + q; };
+    const auto first_number = [&](int q) { return int(int64_t(scalar_load(b.starts + q)) * a.group >> 7) + q; };
     int seq = 0;
     for (int hi = b.n_seqs; hi - seq > 1;) {
         const int mid = (seq + hi) >> 1;
@@ -455,7 +463,7 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
     // this lane's row, and the tokens that it sees: lo ..hi - 1; the same for the wave's first and last row, and the workgroup's
     const int row = row0 + min(32 * wave + (lane & 31), rows - 1), row_t = row / a.group;
     const int row_h = head * a.group + row - row_t * a.group;
-    const int hi = sees(row), lo = from(hi);
+    const int hi = before + row_t + 1, lo = from(hi);
     const int hi_least = sees(row0 + min(32 * wave, rows - 1)), hi_most = sees(row0 + min(32 * wave + 31, rows - 1));
     const int lo_least = from(hi_least), lo_most = from(hi_most);
     const int hi_all = sees(row0 + rows - 1), lo_all = from(sees(row0));
@@ -463,120 +471,127 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
     const int per = max(1024 / TT, (tiles + a.splits - 1) / a.splits);
     const int begin = tile0 + split * per, end = tile0 + min(tiles, (split + 1) * per);
 
+    // This thread's part of a tile: four words of one token's keys, and eight dims of four tokens' values. A wave has one run
+    // of 16 tokens (or two, or half of one), whose page is looked up a tile before it is used; a run behind the last token is the last
+    // one, an entry that is no page the first page.
     const Slab<D> slab(b.page);
+    const Codes codes;
     const uint8_t* base = b.pages + int64_t(head) * slab.bytes();
-    // this thread's part of a tile: four words of one token's keys, and eight dims of four tokens' values
+    const int32_t* row_of_table = b.table + int64_t(seq) * b.table_stride;
     const int k_tok = tid / (C / 4), k_sub = tid % (C / 4), v_quad = tid / C, v_chunk = tid % C;
-    int64_t k_page = -1, v_page = -1;
-    int k_run = 0, v_run = 0;
-    bool k_ok = false, v_ok = false;
+    const uint32_t kc_at = 4 * ((k_tok & 15) * C + 4 * k_sub), ks_at = 4 * ((k_tok & 15) * G + 4 * k_sub % G);
+    const uint32_t vc_at = 2 * ((v_quad & 3) * D + v_chunk * 8), vs_at = 16 * ((v_quad & 3) * G + v_chunk / 4);
+    const int last_run = (hi_all - 1) >> 4;
+    int id[RW], in[RW];
+    const auto look = [&](int tl) {
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+            const int first = D == 64 ? 8 * tl + 2 * wave + i : D == 128 ? 4 * tl + wave : 2 * tl + (wave >> 1);
+            const uint32_t run = uint32_t(min(first, last_run));
+            const uint32_t col = b.page_inv ? __umulhi(run, b.page_inv) : run;
+            in[i] = int(run - col * uint32_t(b.page >> 4));
+            id[i] = scalar_load(row_of_table + col);
+        }
+    };
+    bool ok = false;
     u4 k_code, v_code, v_scale;
     uint32_t k_scale[G < 4 ? G : 4];
-    const auto pages = [&](int tl) {   // of the tile's runs; behind the last token: any page
-        const int last = (hi_all - 1) >> 4;
-        k_page = page_at(b, seq, uint32_t(min(tl * (TT / 16) + (k_tok >> 4), last)), k_run);
-        v_page = page_at(b, seq, uint32_t(min(tl * (TT / 16) + (v_quad >> 2), last)), v_run);
-    };
     const auto fetch = [&] {
-        k_ok = k_page >= 0;
-        v_ok = v_page >= 0;
-        const uint8_t* k = base + (k_ok ? k_page : 0);
-        const uint8_t* v = base + (v_ok ? v_page : 0);
-        const int tok = 16 * k_run + (k_tok & 15), quad = 4 * v_run + (v_quad & 3);
-        __builtin_memcpy(&k_code, __builtin_assume_aligned(k + 4 * (tok * C + 4 * k_sub), 16), 16);
-        __builtin_memcpy(k_scale, __builtin_assume_aligned(k + slab.k_scale(tok, 4 * k_sub % G), sizeof k_scale), sizeof k_scale);
-        __builtin_memcpy(&v_code, __builtin_assume_aligned(v + slab.v_codes() + 2 * (quad * D + v_chunk * 8), 16), 16);
-        __builtin_memcpy(&v_scale, __builtin_assume_aligned(v + slab.v_scales() + 16 * (quad * G + v_chunk / 4), 16), 16);
+        const uint8_t* pg[RW];
+        bool good[RW];
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+            good[i] = uint32_t(id[i]) < uint32_t(b.n_pages);
+            pg[i] = base + (good[i] ? int64_t(id[i]) * b.page_stride : 0);
+        }
+        const int w = RW == 1 ? 0 : lane >> 5;
+        ok = w ? good[RW - 1] : good[0];
+        const uint8_t* p = w ? pg[RW - 1] : pg[0];
+        const int run = w ? in[RW - 1] : in[0];
+        const uint8_t *kc = p + 8 * D * run + kc_at, *ks = p + slab.k_scales() + 64 * G * run + ks_at;
+        const uint8_t *vc = p + slab.v_codes() + 8 * D * run + vc_at, *vs = p + slab.v_scales() + 64 * G * run + vs_at;
+        __builtin_memcpy(&k_code, __builtin_assume_aligned(kc, 16), 16);
+        __builtin_memcpy(k_scale, __builtin_assume_aligned(ks, sizeof k_scale), sizeof k_scale);
+        __builtin_memcpy(&v_code, __builtin_assume_aligned(vc, 16), 16);
+        __builtin_memcpy(&v_scale, __builtin_assume_aligned(vs, 16), 16);
     };
+    f16* const k_put = &ksh[0][k_tok * KP + 8 * (D == 64 ? 2 * k_sub : D == 128 ? k_sub : 16 * (k_sub & 1) + (k_sub >> 1))];
+    f16* const v_put = &vsh[0][v_chunk * VP + 16 * (v_quad >> 2) + 8 * (v_quad & 1) + 4 * (v_quad >> 1 & 1)];
     const auto stage = [&](int tl, int buf) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int w = 4 * k_sub + i, g = w % G, unit = 4 * g + w / G;
             const h2 sm = as_h2(k_scale[i % (G < 4 ? G : 4)]);
             h2 k[4];
-            codes8(k_code[i], k);
+            codes(k_code[i], k);
 #pragma unroll
             for (int j = 0; j < 4; ++j) k[j] = __builtin_elementwise_fma(k[j], both(sm[0]), both(sm[1]));
-            *reinterpret_cast<h8*>(&ksh[buf][M::key(k_tok, unit)]) = join(k[0], k[1], k[2], k[3]);
+            const int unit = D == 64 ? 4 * (i & 1) + (i >> 1) : 4 * i;   // 4g + c of word 4 * k_sub + i = c * G + g, besides k_put's part
+            *reinterpret_cast<h8*>(k_put + buf * (TT * KP) + 8 * unit) = join(k[0], k[1], k[2], k[3]);
         }
         // values that no row sees, or whose token is held as NaN, are 0
-        uint32_t sc[4] = {v_scale[0], v_scale[1], v_scale[2], v_scale[3]}, odd = v_ok ? 0u : 16u;
+        uint32_t sc[4] = {v_scale[0], v_scale[1], v_scale[2], v_scale[3]};
         const int tok = TT * tl + 4 * v_quad;
-        if (tok + 4 > hi_all || !v_ok || has_nan(sc[0], sc[1], 0, 0)) {
+        if (TT * (tl + 1) > hi_all || __any(!ok) || has_nan(sc[0], sc[1], 0, 0)) {
+            uint32_t odd = ok ? 0u : 16u;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const uint32_t keep = j & 1 ? 0x0000ffffu : 0xffff0000u;
-                const bool nan = ((j & 1 ? sc[j >> 1] >> 16 : sc[j >> 1]) & 0x7fffu) >= 0x7c00u, none = tok + j >= hi_all || !v_ok;
+                const bool nan = ((j & 1 ? sc[j >> 1] >> 16 : sc[j >> 1]) & 0x7fffu) >= 0x7c00u, none = tok + j >= hi_all || !ok;
                 if (nan && !none) odd |= 1u << j;
                 if (nan || none) {
                     sc[j >> 1] &= keep;
                     sc[2 + (j >> 1)] &= keep;
                 }
             }
+            if (v_chunk == 0) odd_sh[buf][v_quad] = uint8_t(odd);
+            if (odd) odd_tile[buf] = tl;
+            if (!ok) atomicOr(b.err, kDevErrBatch);
+        } else if (v_chunk == 0) {
+            odd_sh[buf][v_quad] = 0;
         }
-        if (v_chunk == 0) odd_sh[buf][v_quad] = uint8_t(odd);
-        const int unit = 2 * (v_quad >> 2) + (v_quad & 1), half = 4 * (v_quad >> 1 & 1);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             h2 x[4], y[4];
-            codes8(v_code[h], x);
-            codes8(v_code[2 + h], y);
+            codes(v_code[h], x);
+            codes(v_code[2 + h], y);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 x[j] = __builtin_elementwise_fma(x[j], as_h2(sc[0]), as_h2(sc[2]));
                 y[j] = __builtin_elementwise_fma(y[j], as_h2(sc[1]), as_h2(sc[3]));
-                *reinterpret_cast<u2*>(&vsh[buf][M::value(8 * v_chunk + 4 * h + j, unit) + half]) = u2{as_u32(x[j]), as_u32(y[j])};
+                *reinterpret_cast<u2*>(v_put + buf * (D * VP) + (4 * h + j) * C * VP) = u2{as_u32(x[j]), as_u32(y[j])};
             }
         }
-        if (!(k_ok && v_ok)) atomicOr(b.err, kDevErrBatch);
     };
 
+    if (tid < 2) odd_tile[tid] = -1;
     if (begin < end) {
-        pages(begin);
+        look(begin);
         fetch();
-        if (begin + 1 < end) pages(begin + 1);
+        if (begin + 1 < end) look(begin + 1);
     }
     // q: the second operand, row lane % 32, dims 16k + 8c ..+7
     h8 q[M::KS];
-    bool bad;
-    float up;
-    {
-        const T* p = static_cast<const T*>(a.q) + int64_t(s.first + row_t) * a.q_stride + int64_t(row_h) * D + 8 * c;
-        Eight<T> v[M::KS];
-        float m = 0.0f;
-#pragma unroll
-        for (int k = 0; k < M::KS; ++k) {
-            v[k] = eight(p + 16 * k, 8);
-            float w[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = float(v[k].v[i]);
-            m = amax8(w, m);
-        }
-        m = fmaxf(m, __shfl_xor(m, 32));
-        bad = m > 3.402823466e38f;
-        const int e = row_exponent<T>(m);
-#pragma unroll
-        for (int k = 0; k < M::KS; ++k)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) q[k][i] = turned_q(float(v[k].v[i]), -e, bad, a.scale);
-        up = row_factor(a, e);
-    }
+    const float up = take_q(a, static_cast<const T*>(a.q) + int64_t(s.first + row_t) * a.q_stride + int64_t(row_h) * D + 8 * c, 16, q,
+                            [](uint32_t v) { return max(v, uint32_t(__shfl_xor(int(v), 32))); });
     const Cap cap{2.0f * kLog2e / a.softcap, a.softcap * kLog2e};
 
     float top = kLowest, sum = 0.0f;
     f16x o[M::NT] = {};
+    __syncthreads();   // odd_tile
     if (begin < end) {
         stage(begin, 0);
         if (begin + 1 < end) fetch();
-        if (begin + 2 < end) pages(begin + 2);
+        if (begin + 2 < end) look(begin + 2);
     }
+    const f16* const k_get = &ksh[0][(lane & 31) * KP + 8 * c];
+    const f16* const v_get = &vsh[0][(lane & 31) * VP + 8 * c];
     for (int tl = begin; tl < end; ++tl) {
         const int buf = (tl - begin) & 1;
         __syncthreads();
         if (tl + 1 < end) {
             stage(tl + 1, buf ^ 1);
             if (tl + 2 < end) fetch();
-            if (tl + 3 < end) pages(tl + 3);
+            if (tl + 3 < end) look(tl + 3);
         }
         if (TT * tl >= hi_most || TT * (tl + 1) <= lo_least) continue;   // no row of this wave sees the tile
         f16x x[M::MT];
@@ -585,7 +600,7 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
             x[m] = f16x{};
 #pragma unroll
             for (int k = 0; k < M::KS; ++k) {
-                const h8 key = *reinterpret_cast<const h8*>(&ksh[buf][M::key(32 * m + (lane & 31), 2 * k + c)]);
+                const h8 key = *reinterpret_cast<const h8*>(k_get + buf * (TT * KP) + 32 * m * KP + 16 * k);
                 x[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, q[k], x[m], 0, 0, 0);
             }
         }
@@ -598,16 +613,13 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
             upx = 1.0f;
         }
         // tokens that some rows do not see, or that are held as NaN or have no page
-        uint32_t odd = 0;
-#pragma unroll
-        for (int i = 0; i < TT / 16; ++i) odd |= reinterpret_cast<const uint32_t*>(odd_sh[buf])[i];
-        if (TT * tl < lo_most || TT * (tl + 1) > hi_least || __builtin_amdgcn_readfirstlane(odd)) {
+        if (TT * tl < lo_most || TT * (tl + 1) > hi_least || __builtin_amdgcn_readfirstlane(odd_tile[buf]) == tl) {
 #pragma unroll
             for (int m = 0; m < M::MT; ++m)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int in = 32 * m + 8 * (i >> 2) + 4 * c + (i & 3), tok = TT * tl + in;
-                    const uint32_t e = odd_sh[buf][in >> 2];
+                    const int nth = 32 * m + 8 * (i >> 2) + 4 * c + (i & 3), tok = TT * tl + nth;
+                    const uint32_t e = odd_sh[buf][nth >> 2];
                     if (tok < lo || tok >= hi || e >= 16) x[m][i] = -INFINITY;
                     else if (e >> (i & 3) & 1) x[m][i] = NAN;
                 }
@@ -644,38 +656,33 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
         for (int n = 0; n < M::NT; ++n)
 #pragma unroll
             for (int k = 0; k < TT / 16; ++k) {
-                const h8 v = *reinterpret_cast<const h8*>(&vsh[buf][M::value(32 * n + (lane & 31), 2 * k + c)]);
+                const h8 v = *reinterpret_cast<const h8*>(v_get + buf * (D * VP) + 32 * n * VP + 16 * k);
                 o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w[k], o[n], 0, 0, 0);
             }
     }
 
     sum += __shfl_xor(sum, 32);
-    if (bad && hi > 0) sum = NAN;
     if (32 * wave + (lane & 31) >= rows) return;
-    const int64_t out_row = int64_t(s.first + row_t);
-    if (a.splits == 1) {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        T* p = static_cast<T*>(a.out) + out_row * a.out_stride + int64_t(row_h) * D + 4 * c;
+    // the lane has chunks 8u + 4c + i of its row, whose eight dims lie in as many registers (of row j * C + chunk of the products)
+    const int64_t out_row = int64_t(s.first + row_t), part = (out_row * a.q_heads + row_h) * a.splits + split;
+    const float inv = a.splits > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-        for (int n = 0; n < M::NT; ++n)
+    for (int u = 0; u < C / 8; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                T v[4];
+        for (int i = 0; i < 4; ++i) {
+            float y[8];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = T(o[n][4 * i + j] * inv);
-                __builtin_memcpy(p + 32 * n + 8 * i, v, sizeof v);
+            for (int j = 0; j < 8; ++j) {
+                const int r = j * C + 8 * u;
+                y[j] = o[r >> 5][4 * ((r & 31) >> 3) + i] * inv;
             }
-    } else {
-        const int64_t i = (out_row * a.q_heads + row_h) * a.splits + split;
-        float* p = a.part + i * D + 4 * c;
-#pragma unroll
-        for (int n = 0; n < M::NT; ++n)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) *reinterpret_cast<f4*>(p + 32 * n + 8 * k) = f4{o[n][4 * k], o[n][4 * k + 1], o[n][4 * k + 2], o[n][4 * k + 3]};
-        if (c == 0) {
-            a.part_ml[2 * i] = top;
-            a.part_ml[2 * i + 1] = sum;
+            const int d = 8 * (8 * u + 4 * c + i);
+            if (a.splits == 1) store8(static_cast<T*>(a.out) + out_row * a.out_stride + int64_t(row_h) * D + d, 8, y);
+            else store8(a.part + part * D + d, 8, y);
         }
+    if (a.splits > 1 && c == 0) {
+        a.part_ml[2 * part] = top;
+        a.part_ml[2 * part + 1] = sum;
     }
 }
 
