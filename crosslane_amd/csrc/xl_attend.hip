@@ -144,15 +144,21 @@ __device__ __forceinline__ float take_q(const AttendArgs& a, const T* p, int str
 // What a lane loads of a tile of 32 tokens (two runs of 16), for keys as the first operand of the scores
 // (token lane % 16 of each run, the eight dims 32g + 8c with c = lane / 16 of every group g), and for values as
 // the first operand of the outputs (dims D / 16 * (lane % 16) on, the four tokens 4c of each run). An address is a
-// run's place, the same for the wave, and an offset of the lane's that stays.
-template <int D>
+// run's place, the same for the wave, and an offset of the lane's that stays. ONCE: nobody else reads these bytes.
+template <int D, bool ONCE>
 struct TileLoads {
     static constexpr int G = D / 32;
     uint32_t kc[2][G], ks[2][G], vc[2][D >= 128 ? D / 32 : 4], vs[2][4];
     uint32_t kc_at, ks_at, vc_at, vs_at;
     template <int N>
     static __device__ __forceinline__ void load(const uint8_t* p, uint32_t (&w)[N]) {
-        __builtin_memcpy(w, __builtin_assume_aligned(p, N >= 4 ? 16 : 4 * N), 4 * N);
+        if constexpr (ONCE) {
+            typedef uint32_t V __attribute__((ext_vector_type(N)));
+            const V v = __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+            __builtin_memcpy(w, &v, sizeof v);
+        } else {
+            __builtin_memcpy(w, __builtin_assume_aligned(p, N >= 4 ? 16 : 4 * N), 4 * N);
+        }
     }
     __device__ __forceinline__ explicit TileLoads(int lane) {
         const int tok = lane & 15, c = lane >> 4, chunk = D >= 128 ? tok * (D / 128) : tok >> 1;
@@ -184,7 +190,7 @@ __device__ __forceinline__ int scalar_load(const int32_t* p) {
 // first operand, with no LDS and no exchange between lanes; the scores come out in the lanes (row lane % 16, tokens
 // 4 (lane / 16) ..+3 of each run) where the second product wants its weights, since the order of tokens
 // within its sum is free. Loads of the next tile follow the last use of this one's registers.
-template <class T, int D>
+template <class T, int D, bool ONCE>
 __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(AttendArgs a) {
     constexpr int G = D / 32, N = D / 16;
     __shared__ float part[4][16][D + 4];
@@ -216,7 +222,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
     const Slab<D> slab(b.page);
     const uint8_t* base = b.pages + int64_t(head) * slab.bytes();
     const int last_run = (hi_all - 1) >> 4;
-    TileLoads<D> t(lane);
+    TileLoads<D, ONCE> t(lane);
     const Codes codes;
     // A tile's pages, by the table's entries, which are read a tile before they are used. Where a tile's second run lies
     // behind the last token, it is the last run; where an entry is no page, the first page: such tokens are hidden.
@@ -757,8 +763,11 @@ hipError_t attend_go(const AttendArgs& a, hipStream_t s, hipEvent_t stop) {
     const auto go = [&](auto kernel) {
         hipExtLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, s, nullptr, a.splits == 1 ? stop : nullptr, 0, a);
     };
-    if (a.few) go(attend_few_kernel<T, D>);
-    else go(attend_many_kernel<T, D>);
+    // bytes that one workgroup reads past the caches: decode_long 41.1 us -> 38.9, decode_batch 145.8 -> 136.4; not for heads of
+    // 256, whose lanes take 32 bytes in two loads (56.5 us of drafted rows -> 57.9)
+    if (!a.few) go(attend_many_kernel<T, D>);
+    else if (D < 256 && a.tiles == 1) go(attend_few_kernel<T, D, (D < 256)>);
+    else go(attend_few_kernel<T, D, false>);
     if (a.splits > 1) {
         const int64_t heads = int64_t(a.b.rows) * a.q_heads;
         const auto join = [&](auto kernel, int w) {
