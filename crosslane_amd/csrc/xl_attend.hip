@@ -22,18 +22,35 @@ constexpr int kFewRows = 32;      // rows (of a sequence and a kv head) up to wh
 
 }  // namespace
 
-// Splits: as many workgroups as the card holds at once (four a CU, two of those that take many rows or heads of 256
-// values), where each has 256 tokens at least (of many rows: 1024), or four times as many for an even end, where each has 1024.
+// Few rows: as many workgroups as the card holds at once (four a CU, two of heads of 256 values) where each has 256 tokens at
+// least, or four times as many for an even end where each has 1024. Many rows: the least of the rounds that 512 workgroups at a
+// time make, at 0.03 us a token and 5 us a workgroup, and the join's bytes at 4 TB/s.
 AttendPlan attend_plan(int dim, int kv_heads, int q_heads, int n_seqs, int rows, int max_rows, int64_t max_tokens, int window) {
     AttendPlan p;
     const int64_t group = q_heads / kv_heads, most = max_rows * group;
-    p.few = most <= kFewRows;
-    p.tiles = p.few ? int((most + 15) / 16) : int((rows * group >> 7) + n_seqs);
-    const int64_t wgs = (p.few ? int64_t(n_seqs) : int64_t(1)) * kv_heads * p.tiles;
-    const int64_t held = p.few && dim < 256 ? 1024 : 512;
     const int64_t tokens = window ? std::min(max_tokens, int64_t(window) + max_rows) : max_tokens;
-    const auto splits = [&](int64_t groups, int64_t least) { return std::min((groups + wgs - 1) / wgs, (tokens + least - 1) / least); };
-    p.splits = int(std::min<int64_t>(128, std::max<int64_t>(1, p.few ? std::max(splits(held, 256), splits(4 * held, 1024)) : splits(held, 1024))));
+    p.few = most <= kFewRows;
+    int64_t wgs;
+    if (p.few) {
+        p.tiles = int((most + 15) / 16);
+        wgs = int64_t(n_seqs) * kv_heads * p.tiles;
+        const int64_t held = dim < 256 ? 1024 : 512;
+        const auto splits = [&](int64_t groups, int64_t least) { return std::min((groups + wgs - 1) / wgs, (tokens + least - 1) / least); };
+        p.splits = int(std::min<int64_t>(128, std::max(splits(held, 256), splits(4 * held, 1024))));
+    } else {
+        p.tiles = int((rows * group >> 7) + n_seqs);   // numbers for them; about half a tile of each sequence has rows
+        wgs = int64_t(kv_heads) * p.tiles;
+        const int64_t real = kv_heads * (((rows * group + 127) >> 7) + (n_seqs - 1) / 2);
+        double best = 1e30;
+        for (int64_t k = 1; k <= 128 && (k == 1 || (real * k <= 2048 && tokens >= 512 * k)); ++k) {
+            const double rounds = double((real * k + 511) / 512), join = k == 1 ? 0.0 : 4.0 + double(rows) * q_heads * dim * double(k) * 1e-6;
+            const double us = rounds * (0.03 * double(tokens) / double(k) + 5.0) + join;
+            if (us < best) {
+                best = us;
+                p.splits = int(k);
+            }
+        }
+    }
     p.groups = std::max(wgs * p.splits, int64_t(rows) * q_heads);
     if (p.splits > 1) {
         const uint64_t parts = uint64_t(rows) * uint64_t(q_heads) * uint64_t(p.splits);
@@ -425,22 +442,24 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
 // the lanes that need them as weights, as above: values' tokens lie in LDS in the order in which the scores come out.
 template <int D>
 struct Many {
-    static constexpr int TT = 8192 / D;      // tokens of a tile: 16 KiB each of keys and values
+    static constexpr int TT = D == 256 ? 32 : 64;   // tokens of a tile
     static constexpr int G = D / 32, C = D / 8, KS = D / 16, NT = D / 32, MT = TT / 32;
+    // What a thread makes of a tile: KW words of one token's keys; of values the words of VP of the two pairs of four tokens, eight dims.
+    static constexpr int KW = TT * C / 256, VP = TT * C / 512;
     // Rows in LDS are 16 bytes longer than their values, so that eight lanes' 16 bytes of eight rows lie in banks of their own. A
     // value's row is (dim % 8) * C + dim / 8: the lanes that write, of chunks of eight dims, have neighbouring rows then.
-    static constexpr int KP = D + 8, VP = TT + 8;
+    static constexpr int KROW = D + 8, VROW = TT + 8;
 };
 typedef float f16x __attribute__((ext_vector_type(16)));
 
-template <class T, int D>
-__global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
+template <class T, int D, bool CAP>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(AttendArgs a) {
     using M = Many<D>;
-    constexpr int TT = M::TT, G = M::G, C = M::C, KP = M::KP, VP = M::VP, RW = D == 64 ? 2 : 1;
-    __shared__ __attribute__((aligned(16))) f16 ksh[2][TT * KP];
-    __shared__ __attribute__((aligned(16))) f16 vsh[2][D * VP];
-    __shared__ uint8_t odd_sh[2][TT / 4];   // of four tokens: held as NaN (bits 0..3), no page (bit 4)
-    __shared__ int odd_tile[2];             // the last tile that had such tokens
+    constexpr int TT = M::TT, G = M::G, C = M::C, KW = M::KW, VP = M::VP, KROW = M::KROW, VROW = M::VROW;
+    __shared__ __attribute__((aligned(16))) f16 ksh[2][TT * KROW];
+    __shared__ __attribute__((aligned(16))) f16 vsh[2][D * VROW];
+    __shared__ __attribute__((aligned(2))) uint8_t odd_sh[2][TT / 2];   // of two tokens: held as NaN (bits 0 and 1), no page (bit 2)
+    __shared__ int odd_tile[2];                                        // the last tile that had such tokens
     const KvBatch& b = a.b;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane >> 5;
     // Sequence q's tiles are numbered from starts[q] * group / 128 + q on: at least as many numbers as it has tiles. The last ones,
@@ -470,171 +489,183 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
     const int row = row0 + min(32 * wave + (lane & 31), rows - 1), row_t = row / a.group;
     const int row_h = head * a.group + row - row_t * a.group;
     const int hi = before + row_t + 1, lo = from(hi);
-    const int hi_least = sees(row0 + min(32 * wave, rows - 1)), hi_most = sees(row0 + min(32 * wave + 31, rows - 1));
-    const int lo_least = from(hi_least), lo_most = from(hi_most);
+    const int hi_least = sees(row0 + min(32 * wave, rows - 1)), lo_most = from(sees(row0 + min(32 * wave + 31, rows - 1)));
     const int hi_all = sees(row0 + rows - 1), lo_all = from(sees(row0));
     const int tile0 = lo_all / TT, tiles = hi_all > lo_all ? (hi_all + TT - 1) / TT - tile0 : 0;
     const int per = max(1024 / TT, (tiles + a.splits - 1) / a.splits);
     const int begin = tile0 + split * per, end = tile0 + min(tiles, (split + 1) * per);
 
-    // This thread's part of a tile: four words of one token's keys, and eight dims of four tokens' values. A wave has one run
-    // of 16 tokens (or two, or half of one), whose page is looked up a tile before it is used; a run behind the last token is the last
-    // one, an entry that is no page the first page.
+    // This thread's part of a tile: words of one token's keys, and eight dims of four (or two) tokens' values. A wave's lie in one run
+    // of 16 tokens, whose page is looked up a tile before it is used; a run behind the last token is the last one, an entry
+    // that is no page the first page. Keys are loaded a tile before the values of the same tokens.
     const Slab<D> slab(b.page);
     const Codes codes;
     const uint8_t* base = b.pages + int64_t(head) * slab.bytes();
     const int32_t* row_of_table = b.table + int64_t(seq) * b.table_stride;
-    const int k_tok = tid / (C / 4), k_sub = tid % (C / 4), v_quad = tid / C, v_chunk = tid % C;
-    const uint32_t kc_at = 4 * ((k_tok & 15) * C + 4 * k_sub), ks_at = 4 * ((k_tok & 15) * G + 4 * k_sub % G);
-    const uint32_t vc_at = 2 * ((v_quad & 3) * D + v_chunk * 8), vs_at = 16 * ((v_quad & 3) * G + v_chunk / 4);
+    const int k_tok = tid / (C / KW), k_sub = tid % (C / KW);
+    const int v_quad = tid / (2 / VP * C), v_chunk = tid / (2 / VP) % C, v_pair = VP == 1 ? tid & 1 : 0;
+    const uint32_t kc_at = 4 * ((k_tok & 15) * C + KW * k_sub), ks_at = 4 * ((k_tok & 15) * G + KW * k_sub % G);
+    const uint32_t vc_at = 2 * ((v_quad & 3) * D + v_chunk * 8) + 8 * v_pair, vs_at = 16 * ((v_quad & 3) * G + v_chunk / 4) + 4 * v_pair;
     const int last_run = (hi_all - 1) >> 4;
-    int id[RW], in[RW];
+    struct Page {
+        int id, in;
+    };
     const auto look = [&](int tl) {
-#pragma unroll
-        for (int i = 0; i < RW; ++i) {
-            const int first = D == 64 ? 8 * tl + 2 * wave + i : D == 128 ? 4 * tl + wave : 2 * tl + (wave >> 1);
-            const uint32_t run = uint32_t(min(first, last_run));
-            const uint32_t col = b.page_inv ? __umulhi(run, b.page_inv) : run;
-            in[i] = int(run - col * uint32_t(b.page >> 4));
-            id[i] = scalar_load(row_of_table + col);
-        }
+        const uint32_t run = uint32_t(min(TT == 64 ? 4 * tl + wave : 2 * tl + (wave >> 1), last_run));
+        const uint32_t col = b.page_inv ? __umulhi(run, b.page_inv) : run;
+        return Page{scalar_load(row_of_table + col), int(run - col * uint32_t(b.page >> 4))};
     };
-    bool ok = false;
-    u4 k_code, v_code, v_scale;
-    uint32_t k_scale[G < 4 ? G : 4];
-    const auto fetch = [&] {
-        const uint8_t* pg[RW];
-        bool good[RW];
-#pragma unroll
-        for (int i = 0; i < RW; ++i) {
-            good[i] = uint32_t(id[i]) < uint32_t(b.n_pages);
-            pg[i] = base + (good[i] ? int64_t(id[i]) * b.page_stride : 0);
-        }
-        const int w = RW == 1 ? 0 : lane >> 5;
-        ok = w ? good[RW - 1] : good[0];
-        const uint8_t* p = w ? pg[RW - 1] : pg[0];
-        const int run = w ? in[RW - 1] : in[0];
-        const uint8_t *kc = p + 8 * D * run + kc_at, *ks = p + slab.k_scales() + 64 * G * run + ks_at;
-        const uint8_t *vc = p + slab.v_codes() + 8 * D * run + vc_at, *vs = p + slab.v_scales() + 64 * G * run + vs_at;
-        __builtin_memcpy(&k_code, __builtin_assume_aligned(kc, 16), 16);
-        __builtin_memcpy(k_scale, __builtin_assume_aligned(ks, sizeof k_scale), sizeof k_scale);
-        __builtin_memcpy(&v_code, __builtin_assume_aligned(vc, 16), 16);
-        __builtin_memcpy(&v_scale, __builtin_assume_aligned(vs, 16), 16);
+    const auto good = [&](const Page& p) { return uint32_t(p.id) < uint32_t(b.n_pages); };
+    const auto run_at = [&](const Page& p) { return base + (good(p) ? int64_t(p.id) * b.page_stride : 0); };
+    struct RawKeys {
+        uint32_t code[KW], scale[KW < G ? KW : G];
     };
-    f16* const k_put = &ksh[0][k_tok * KP + 8 * (D == 64 ? 2 * k_sub : D == 128 ? k_sub : 16 * (k_sub & 1) + (k_sub >> 1))];
-    f16* const v_put = &vsh[0][v_chunk * VP + 16 * (v_quad >> 2) + 8 * (v_quad & 1) + 4 * (v_quad >> 1 & 1)];
-    const auto stage = [&](int tl, int buf) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const h2 sm = as_h2(k_scale[i % (G < 4 ? G : 4)]);
+    struct RawValues {
+        uint32_t code[2 * VP], step[VP], small[VP];   // [pair][half]; [pair]
+        bool ok;
+    };
+    const auto fetch_keys = [&](const Page& p, RawKeys& r) {
+        const uint8_t* at = run_at(p);
+        __builtin_memcpy(r.code, __builtin_assume_aligned(at + 8 * D * p.in + kc_at, sizeof r.code), sizeof r.code);
+        __builtin_memcpy(r.scale, __builtin_assume_aligned(at + slab.k_scales() + 64 * G * p.in + ks_at, sizeof r.scale), sizeof r.scale);
+    };
+    const auto fetch_values = [&](const Page& p, RawValues& r) {
+        const uint8_t* at = run_at(p);
+        __builtin_memcpy(r.code, __builtin_assume_aligned(at + slab.v_codes() + 8 * D * p.in + vc_at, sizeof r.code), sizeof r.code);
+        uint32_t w[4];
+        const uint8_t* sc = at + slab.v_scales() + 64 * G * p.in + vs_at;
+        if constexpr (VP == 2) {
+            __builtin_memcpy(w, __builtin_assume_aligned(sc, 16), 16);
+            r.step[0] = w[0], r.step[VP - 1] = w[1], r.small[0] = w[2], r.small[VP - 1] = w[3];
+        } else {
+            r.step[0] = *reinterpret_cast<const uint32_t*>(sc);
+            r.small[0] = *reinterpret_cast<const uint32_t*>(sc + 8);
+        }
+        r.ok = good(p);
+    };
+    // word i of the thread's keys is c * G + g of its token: unit 4g + c of eight dims
+    f16* const k_put = &ksh[0][k_tok * KROW + 8 * (D == 256 ? 16 * (k_sub & 1) + (k_sub >> 1) : k_sub)];
+    f16* const v_put = &vsh[0][v_chunk * VROW + 16 * (v_quad >> 2) + 8 * (v_quad & 1) + 4 * (v_quad >> 1 & 1) + 2 * v_pair];
+    // The codes to float16, in slices that go between products: of keys two for each word; of values, for each half of the eight dims,
+    // the codes of each pair of tokens, then as many slices of their dims.
+    constexpr int KSLICES = 2 * KW, VSLICES = 4 * VP;
+    h2 codes_of[VP][4];
+    const auto stage_keys = [&](const RawKeys& r, int buf, int slice) {
+        const int i = slice / 2;
+        if (slice % 2 == 0) {
+            codes(r.code[i], codes_of[0]);
+        } else {
+            const h2 sm = as_h2(r.scale[i % (KW < G ? KW : G)]);
             h2 k[4];
-            codes(k_code[i], k);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) k[j] = __builtin_elementwise_fma(k[j], both(sm[0]), both(sm[1]));
-            const int unit = D == 64 ? 4 * (i & 1) + (i >> 1) : 4 * i;   // 4g + c of word 4 * k_sub + i = c * G + g, besides k_put's part
-            *reinterpret_cast<h8*>(k_put + buf * (TT * KP) + 8 * unit) = join(k[0], k[1], k[2], k[3]);
+            for (int j = 0; j < 4; ++j) k[j] = __builtin_elementwise_fma(codes_of[0][j], both(sm[0]), both(sm[1]));
+            *reinterpret_cast<h8*>(k_put + buf * (TT * KROW) + 32 * i) = join(k[0], k[1], k[2], k[3]);
         }
-        // values that no row sees, or whose token is held as NaN, are 0
-        uint32_t sc[4] = {v_scale[0], v_scale[1], v_scale[2], v_scale[3]};
-        const int tok = TT * tl + 4 * v_quad;
-        if (TT * (tl + 1) > hi_all || __any(!ok) || has_nan(sc[0], sc[1], 0, 0)) {
-            uint32_t odd = ok ? 0u : 16u;
+    };
+    const auto stage_values = [&](const RawValues& r, int buf, int slice) {
+        const int h = slice / (2 * VP), k = slice % (2 * VP);
+        if (k < VP) {
+            codes(r.code[2 * k + h], codes_of[k]);
+        } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t keep = j & 1 ? 0x0000ffffu : 0xffff0000u;
-                const bool nan = ((j & 1 ? sc[j >> 1] >> 16 : sc[j >> 1]) & 0x7fffu) >= 0x7c00u, none = tok + j >= hi_all || !ok;
-                if (nan && !none) odd |= 1u << j;
-                if (nan || none) {
-                    sc[j >> 1] &= keep;
-                    sc[2 + (j >> 1)] &= keep;
+            for (int j = (k - VP) * (4 / VP); j < (k - VP + 1) * (4 / VP); ++j) {
+                f16* at = v_put + buf * (D * VROW) + (4 * h + j) * C * VROW;
+                uint32_t v[VP];
+#pragma unroll
+                for (int i = 0; i < VP; ++i) v[i] = as_u32(__builtin_elementwise_fma(codes_of[i][j], as_h2(r.step[i]), as_h2(r.small[i])));
+                __builtin_memcpy(__builtin_assume_aligned(at, sizeof v), v, sizeof v);
+            }
+        }
+    };
+    // Values that no row sees, or whose token is held as NaN, are 0: by their scales, before they are staged.
+    const auto check_values = [&](RawValues& r, int tl, int buf) {
+        uint32_t odd[VP] = {};
+        if (TT * (tl + 1) > hi_all || !r.ok || has_nan(r.step[0], r.step[VP - 1], 0, 0)) {
+#pragma unroll
+            for (int i = 0; i < VP; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const bool nan = ((j ? r.step[i] >> 16 : r.step[i]) & 0x7fffu) >= 0x7c00u;
+                    const bool none = TT * tl + 4 * v_quad + 2 * (v_pair + i) + j >= hi_all || !r.ok;
+                    if (nan && !none) odd[i] |= 1u << j;
+                    if (nan || none) {
+                        r.step[i] &= j ? 0x0000ffffu : 0xffff0000u;
+                        r.small[i] &= j ? 0x0000ffffu : 0xffff0000u;
+                    }
                 }
+            if (!r.ok) {
+                odd[0] |= 4u;
+                odd[VP - 1] |= 4u;
+                if (TT * tl + 4 * v_quad < hi_all) atomicOr(b.err, kDevErrBatch);
             }
-            if (v_chunk == 0) odd_sh[buf][v_quad] = uint8_t(odd);
-            if (odd) odd_tile[buf] = tl;
-            if (!ok) atomicOr(b.err, kDevErrBatch);
-        } else if (v_chunk == 0) {
-            odd_sh[buf][v_quad] = 0;
+            if (odd[0] | odd[VP - 1]) odd_tile[buf] = tl;
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            h2 x[4], y[4];
-            codes(v_code[h], x);
-            codes(v_code[2 + h], y);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[j] = __builtin_elementwise_fma(x[j], as_h2(sc[0]), as_h2(sc[2]));
-                y[j] = __builtin_elementwise_fma(y[j], as_h2(sc[1]), as_h2(sc[3]));
-                *reinterpret_cast<u2*>(v_put + buf * (D * VP) + (4 * h + j) * C * VP) = u2{as_u32(x[j]), as_u32(y[j])};
-            }
-        }
+        for (int i = 0; i < VP; ++i) odd_sh[buf][2 * v_quad + v_pair + i] = uint8_t(odd[i]);   // (by every lane of these tokens)
     };
 
-    if (tid < 2) odd_tile[tid] = -1;
-    if (begin < end) {
-        look(begin);
-        fetch();
-        if (begin + 1 < end) look(begin + 1);
-    }
     // q: the second operand, row lane % 32, dims 16k + 8c ..+7
     h8 q[M::KS];
     const float up = take_q(a, static_cast<const T*>(a.q) + int64_t(s.first + row_t) * a.q_stride + int64_t(row_h) * D + 8 * c, 16, q,
                             [](uint32_t v) { return max(v, uint32_t(__shfl_xor(int(v), 32))); });
     const Cap cap{2.0f * kLog2e / a.softcap, a.softcap * kLog2e};
+    const float upx = CAP ? 1.0f : up;
 
     float top = kLowest, sum = 0.0f;
     f16x o[M::NT] = {};
-    __syncthreads();   // odd_tile
-    if (begin < end) {
-        stage(begin, 0);
-        if (begin + 1 < end) fetch();
-        if (begin + 2 < end) look(begin + 2);
-    }
-    const f16* const k_get = &ksh[0][(lane & 31) * KP + 8 * c];
-    const f16* const v_get = &vsh[0][(lane & 31) * VP + 8 * c];
-    for (int tl = begin; tl < end; ++tl) {
+    const f16* const k_get = &ksh[0][(lane & 31) * KROW + 8 * c];
+    const f16* const v_get = &vsh[0][(lane & 31) * VROW + 8 * c];
+    constexpr int P1 = M::MT * M::KS, P2 = M::NT * TT / 16;   // products of the scores, and of the values
+    const auto key = [&](int buf, int i) {
+        return *reinterpret_cast<const h8*>(k_get + buf * (TT * KROW) + 32 * (i % M::MT) * KROW + 16 * (i / M::MT));
+    };
+    const auto value = [&](int buf, int i) {
+        return *reinterpret_cast<const h8*>(v_get + buf * (D * VROW) + 32 * (i % M::NT) * VROW + 16 * (i / M::NT));
+    };
+    // Products of the scores x with tile `buf`'s keys, and beside(i) between them; nothing moves from one to the next.
+    const auto score = [&](f16x (&x)[M::MT], int buf, auto&& beside) {
+        h8 k[3] = {key(buf, 0), key(buf, 1)};
+#pragma unroll
+        for (int i = 0; i < P1; ++i) {
+            if (i + 2 < P1) k[(i + 2) % 3] = key(buf, i + 2);
+            const f16x before = i < M::MT ? f16x{} : x[i % M::MT];
+            x[i % M::MT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i % 3], q[i / M::MT], before, 0, 0, 0);
+            beside(i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // A part of new scores: capped where there is a cap, and the largest so far.
+    float most;
+    const auto look_over = [&](f16x (&x)[M::MT], bool fresh, int begin_at, int end_at) {
+#pragma unroll
+        for (int i = begin_at; i < end_at; ++i) {
+            if (CAP && fresh) x[i / 16][i % 16] = cap(x[i / 16][i % 16] * up);
+            most = fmaxf(most, x[i / 16][i % 16]);
+        }
+    };
+    constexpr int S = 16 * M::MT;   // scores of a lane
+    f16x x0[M::MT], x1[M::MT];
+    RawKeys k_raw;
+    RawValues v_raw;
+    Page k_page{}, v_page{};
+    // One tile, whose scores are in x and their largest in `most`: their exponentials beside the next tile's products (to y); then the
+    // values' products beside the codes of the next tile's values and of the keys of the one after it, loaded a tile before.
+    // Behind the last tile that is work on tokens that are there, not used.
+    const auto tile = [&](f16x (&x)[M::MT], f16x (&y)[M::MT], int tl) {
         const int buf = (tl - begin) & 1;
         __syncthreads();
-        if (tl + 1 < end) {
-            stage(tl + 1, buf ^ 1);
-            if (tl + 2 < end) fetch();
-            if (tl + 3 < end) look(tl + 3);
-        }
-        if (TT * tl >= hi_most || TT * (tl + 1) <= lo_least) continue;   // no row of this wave sees the tile
-        f16x x[M::MT];
-#pragma unroll
-        for (int m = 0; m < M::MT; ++m) {
-            x[m] = f16x{};
-#pragma unroll
-            for (int k = 0; k < M::KS; ++k) {
-                const h8 key = *reinterpret_cast<const h8*>(k_get + buf * (TT * KP) + 32 * m * KP + 16 * k);
-                x[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, q[k], x[m], 0, 0, 0);
-            }
-        }
-        float upx = up;
-        if (a.softcap > 0.0f) {
-#pragma unroll
-            for (int m = 0; m < M::MT; ++m)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[m][i] = cap(x[m][i] * up);
-            upx = 1.0f;
-        }
         // tokens that some rows do not see, or that are held as NaN or have no page
         if (TT * tl < lo_most || TT * (tl + 1) > hi_least || __builtin_amdgcn_readfirstlane(odd_tile[buf]) == tl) {
 #pragma unroll
-            for (int m = 0; m < M::MT; ++m)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int nth = 32 * m + 8 * (i >> 2) + 4 * c + (i & 3), tok = TT * tl + nth;
-                    const uint32_t e = odd_sh[buf][nth >> 2];
-                    if (tok < lo || tok >= hi || e >= 16) x[m][i] = -INFINITY;
-                    else if (e >> (i & 3) & 1) x[m][i] = NAN;
-                }
+            for (int i = 0; i < S; ++i) {
+                const int nth = 32 * (i / 16) + 8 * (i % 16 >> 2) + 4 * c + (i & 3), tok = TT * tl + nth;
+                const uint32_t e = odd_sh[buf][nth >> 1];
+                if (tok < lo || tok >= hi || e >= 4) x[i / 16][i % 16] = -INFINITY;
+                else if (e >> (i & 1) & 1) x[i / 16][i % 16] = NAN;
+            }
+            most = kLowest;
+            look_over(x, false, 0, S);
         }
-        float most = kLowest;
-#pragma unroll
-        for (int m = 0; m < M::MT; ++m)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) most = fmaxf(most, x[m][i]);
         most *= upx;
         if (__any(most > top + kLazy)) {
             const float m = fmaxf(fmaxf(most, __shfl_xor(most, 32)), top);
@@ -644,27 +675,65 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
 #pragma unroll
             for (int n = 0; n < M::NT; ++n) o[n] *= f;
         }
-        h8 w[TT / 16];
+        h2 w[S / 2];
+        score(y, buf ^ 1, [&](int i) {
 #pragma unroll
-        for (int m = 0; m < M::MT; ++m)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                x[m][i] = __builtin_amdgcn_exp2f(fmaf(x[m][i], upx, -top));
-                sum += x[m][i];
+            for (int j = i * S / P1; j < (i + 1) * S / P1; ++j) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(x[j / 16][j % 16], upx, -top));
+                sum += p;
+                if (j & 1) w[j / 2] = pack(x[j / 16][j % 16 - 1], p);
+                else x[j / 16][j % 16] = p;
+                if (j & 1) asm volatile("" : "+v"(w[j / 2]), "+v"(sum));   // (keeps the exponentials in their place)
             }
+        });
+        check_values(v_raw, tl + 1, buf ^ 1);
+        most = kLowest;
+        h8 v[3] = {value(buf, 0), value(buf, 1)};
 #pragma unroll
-        for (int k = 0; k < TT / 16; ++k) {
-            const f16x& y = x[k >> 1];
-            const int i = 8 * (k & 1);
-            w[k] = join(pack(y[i], y[i + 1]), pack(y[i + 2], y[i + 3]), pack(y[i + 4], y[i + 5]), pack(y[i + 6], y[i + 7]));
+        for (int i = 0; i < P2; ++i) {
+            if (i + 2 < P2) v[(i + 2) % 3] = value(buf, i + 2);
+            const int k = 4 * (i / M::NT);
+            o[i % M::NT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i % 3], join(w[k], w[k + 1], w[k + 2], w[k + 3]), o[i % M::NT], 0, 0, 0);
+            if (i < VSLICES) stage_values(v_raw, buf ^ 1, i);
+            else stage_keys(k_raw, buf, i - VSLICES);
+            if (i == VSLICES) {
+                fetch_values(v_page, v_raw);
+                v_page = k_page;
+            }
+            look_over(y, true, i * S / P2, (i + 1) * S / P2);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        static_assert(VSLICES + KSLICES == P2);
+        fetch_keys(k_page, k_raw);
+        k_page = look(tl + 4);
+    };
+    if (tid < 2) odd_tile[tid] = -1;
+    if (begin < end) {
+        RawKeys next;
+        const Page p0 = look(begin), p1 = look(begin + 1);
+        fetch_keys(p0, k_raw);
+        fetch_values(p0, v_raw);
+        fetch_keys(p1, next);
+        v_page = look(begin + 2);
+        k_page = look(begin + 3);
+        __syncthreads();   // odd_tile
+        check_values(v_raw, begin, 0);
 #pragma unroll
-        for (int n = 0; n < M::NT; ++n)
+        for (int i = 0; i < KSLICES; ++i) stage_keys(k_raw, 0, i);
 #pragma unroll
-            for (int k = 0; k < TT / 16; ++k) {
-                const h8 v = *reinterpret_cast<const h8*>(v_get + buf * (D * VP) + 32 * n * VP + 16 * k);
-                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w[k], o[n], 0, 0, 0);
-            }
+        for (int i = 0; i < VSLICES; ++i) stage_values(v_raw, 0, i);
+        fetch_values(p1, v_raw);
+        fetch_keys(v_page, k_raw);
+#pragma unroll
+        for (int i = 0; i < KSLICES; ++i) stage_keys(next, 1, i);
+        __syncthreads();
+        score(x0, 0, [](int) {});
+        most = kLowest;
+        look_over(x0, true, 0, S);
+    }
+    for (int tl = begin; tl < end; tl += 2) {
+        tile(x0, x1, tl);
+        if (tl + 1 < end) tile(x1, x0, tl + 1);
     }
 
     sum += __shfl_xor(sum, 32);
@@ -765,7 +834,8 @@ hipError_t attend_go(const AttendArgs& a, hipStream_t s, hipEvent_t stop) {
     };
     // bytes that one workgroup reads past the caches: decode_long 41.1 us -> 38.9, decode_batch 145.8 -> 136.4; not for heads of
     // 256, whose lanes take 32 bytes in two loads (56.5 us of drafted rows -> 57.9)
-    if (!a.few) go(attend_many_kernel<T, D>);
+    if (!a.few && a.softcap > 0.0f) go(attend_many_kernel<T, D, true>);
+    else if (!a.few) go(attend_many_kernel<T, D, false>);
     else if (D < 256 && a.tiles == 1) go(attend_few_kernel<T, D, (D < 256)>);
     else go(attend_few_kernel<T, D, false>);
     if (a.splits > 1) {
