@@ -458,8 +458,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
     constexpr int TT = M::TT, G = M::G, C = M::C, KW = M::KW, VP = M::VP, KROW = M::KROW, VROW = M::VROW;
     __shared__ __attribute__((aligned(16))) f16 ksh[2][TT * KROW];
     __shared__ __attribute__((aligned(16))) f16 vsh[2][D * VROW];
-    __shared__ __attribute__((aligned(2))) uint8_t odd_sh[2][TT / 2];   // of two tokens: held as NaN (bits 0 and 1), no page (bit 2)
-    __shared__ int odd_tile[2];                                        // the last tile that had such tokens
     const KvBatch& b = a.b;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane >> 5;
     // Sequence q's tiles are numbered from starts[q] * group / 128 + q on: at least as many numbers as it has tiles. The last ones,
@@ -504,50 +502,63 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
     const int32_t* row_of_table = b.table + int64_t(seq) * b.table_stride;
     const int k_tok = tid / (C / KW), k_sub = tid % (C / KW);
     const int v_quad = tid / (2 / VP * C), v_chunk = tid / (2 / VP) % C, v_pair = VP == 1 ? tid & 1 : 0;
-    const uint32_t kc_at = 4 * ((k_tok & 15) * C + KW * k_sub), ks_at = 4 * ((k_tok & 15) * G + KW * k_sub % G);
-    const uint32_t vc_at = 2 * ((v_quad & 3) * D + v_chunk * 8) + 8 * v_pair, vs_at = 16 * ((v_quad & 3) * G + v_chunk / 4) + 4 * v_pair;
+    const uint32_t kc_at = 4 * ((k_tok & 15) * C + KW * k_sub);
+    const uint32_t ks_at = slab.k_scales() + 4 * ((k_tok & 15) * G + KW * k_sub % G);
+    const uint32_t kv_at = slab.v_scales() + 2 * ((k_tok >> 2 & 3) * 8 * G + (k_tok & 3));   // the scale of the same token's values
+    const uint32_t vc_at = slab.v_codes() + 2 * ((v_quad & 3) * D + v_chunk * 8) + 8 * v_pair;
+    const uint32_t vs_at = slab.v_scales() + 16 * ((v_quad & 3) * G + v_chunk / 4) + 4 * v_pair;
     const int last_run = (hi_all - 1) >> 4;
     struct Page {
         int id, in;
+    };
+    struct Run {   // where a run's codes begin, and its scales, both without their parts' offsets
+        const uint8_t *code, *scale;
+        bool ok;
     };
     const auto look = [&](int tl) {
         const uint32_t run = uint32_t(min(TT == 64 ? 4 * tl + wave : 2 * tl + (wave >> 1), last_run));
         const uint32_t col = b.page_inv ? __umulhi(run, b.page_inv) : run;
         return Page{scalar_load(row_of_table + col), int(run - col * uint32_t(b.page >> 4))};
     };
-    const auto good = [&](const Page& p) { return uint32_t(p.id) < uint32_t(b.n_pages); };
-    const auto run_at = [&](const Page& p) { return base + (good(p) ? int64_t(p.id) * b.page_stride : 0); };
+    const auto run_of = [&](const Page& p) {
+        const bool ok = uint32_t(p.id) < uint32_t(b.n_pages);
+        const uint8_t* at = base + (ok ? int64_t(p.id) * b.page_stride : 0);
+        return Run{at + 8 * D * p.in, at + 64 * G * p.in, ok};
+    };
     struct RawKeys {
         uint32_t code[KW], scale[KW < G ? KW : G];
+        f16 of_value;
+        bool ok;
     };
     struct RawValues {
         uint32_t code[2 * VP], step[VP], small[VP];   // [pair][half]; [pair]
         bool ok;
     };
-    const auto fetch_keys = [&](const Page& p, RawKeys& r) {
-        const uint8_t* at = run_at(p);
-        __builtin_memcpy(r.code, __builtin_assume_aligned(at + 8 * D * p.in + kc_at, sizeof r.code), sizeof r.code);
-        __builtin_memcpy(r.scale, __builtin_assume_aligned(at + slab.k_scales() + 64 * G * p.in + ks_at, sizeof r.scale), sizeof r.scale);
+    const auto fetch_keys = [&](const Run& at, RawKeys& r) {
+        __builtin_memcpy(r.code, __builtin_assume_aligned(at.code + kc_at, sizeof r.code), sizeof r.code);
+        __builtin_memcpy(r.scale, __builtin_assume_aligned(at.scale + ks_at, sizeof r.scale), sizeof r.scale);
+        r.of_value = *reinterpret_cast<const f16*>(at.scale + kv_at);
+        r.ok = at.ok;
     };
-    const auto fetch_values = [&](const Page& p, RawValues& r) {
-        const uint8_t* at = run_at(p);
-        __builtin_memcpy(r.code, __builtin_assume_aligned(at + slab.v_codes() + 8 * D * p.in + vc_at, sizeof r.code), sizeof r.code);
-        uint32_t w[4];
-        const uint8_t* sc = at + slab.v_scales() + 64 * G * p.in + vs_at;
+    const auto fetch_values = [&](const Run& at, RawValues& r) {
+        __builtin_memcpy(r.code, __builtin_assume_aligned(at.code + vc_at, sizeof r.code), sizeof r.code);
         if constexpr (VP == 2) {
-            __builtin_memcpy(w, __builtin_assume_aligned(sc, 16), 16);
+            uint32_t w[4];
+            __builtin_memcpy(w, __builtin_assume_aligned(at.scale + vs_at, 16), 16);
             r.step[0] = w[0], r.step[VP - 1] = w[1], r.small[0] = w[2], r.small[VP - 1] = w[3];
         } else {
-            r.step[0] = *reinterpret_cast<const uint32_t*>(sc);
-            r.small[0] = *reinterpret_cast<const uint32_t*>(sc + 8);
+            r.step[0] = *reinterpret_cast<const uint32_t*>(at.scale + vs_at);
+            r.small[0] = *reinterpret_cast<const uint32_t*>(at.scale + vs_at + 8);
         }
-        r.ok = good(p);
+        r.ok = at.ok;
     };
     // word i of the thread's keys is c * G + g of its token: unit 4g + c of eight dims
     f16* const k_put = &ksh[0][k_tok * KROW + 8 * (D == 256 ? 16 * (k_sub & 1) + (k_sub >> 1) : k_sub)];
     f16* const v_put = &vsh[0][v_chunk * VROW + 16 * (v_quad >> 2) + 8 * (v_quad & 1) + 4 * (v_quad >> 1 & 1) + 2 * v_pair];
     // The codes to float16, in slices that go between products: of keys two for each word; of values, for each half of the eight dims,
-    // the codes of each pair of tokens, then as many slices of their dims.
+    // the codes of each pair of tokens, then as many slices of their dims. Where a token's values are held as NaN, so are its
+    // keys here, which the scores carry to the rows that see it; the values become numbers (maxima leave a NaN), since a
+    // weight of 0 makes no 0 of a NaN.
     constexpr int KSLICES = 2 * KW, VSLICES = 4 * VP;
     h2 codes_of[VP][4];
     const auto stage_keys = [&](const RawKeys& r, int buf, int slice) {
@@ -555,7 +566,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
         if (slice % 2 == 0) {
             codes(r.code[i], codes_of[0]);
         } else {
-            const h2 sm = as_h2(r.scale[i % (KW < G ? KW : G)]);
+            h2 sm = as_h2(r.scale[i % (KW < G ? KW : G)]);
+            if (i == 0) sm[1] = __builtin_elementwise_fma(r.of_value, f16(0.0f), sm[1]);
             h2 k[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) k[j] = __builtin_elementwise_fma(codes_of[0][j], both(sm[0]), both(sm[1]));
@@ -577,31 +589,31 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
             }
         }
     };
-    // Values that no row sees, or whose token is held as NaN, are 0: by their scales, before they are staged.
-    const auto check_values = [&](RawValues& r, int tl, int buf) {
-        uint32_t odd[VP] = {};
-        if (TT * (tl + 1) > hi_all || !r.ok || has_nan(r.step[0], r.step[VP - 1], 0, 0)) {
+    // Values that no row sees are 0, and those of a page that is none (whose keys are 0 too); none is NaN.
+    const auto check_values = [&](RawValues& r, int tl) {
+#pragma unroll
+        for (int i = 0; i < VP; ++i) {
+            r.step[i] = as_u32(__builtin_elementwise_max(as_h2(r.step[i]), both(f16(0.0f))));
+            r.small[i] = as_u32(__builtin_elementwise_max(as_h2(r.small[i]), both(f16(-65504.0f))));
+        }
+        if (TT * (tl + 1) > hi_all || !r.ok) {
 #pragma unroll
             for (int i = 0; i < VP; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const bool nan = ((j ? r.step[i] >> 16 : r.step[i]) & 0x7fffu) >= 0x7c00u;
-                    const bool none = TT * tl + 4 * v_quad + 2 * (v_pair + i) + j >= hi_all || !r.ok;
-                    if (nan && !none) odd[i] |= 1u << j;
-                    if (nan || none) {
+                for (int j = 0; j < 2; ++j)
+                    if (TT * tl + 4 * v_quad + 2 * (v_pair + i) + j >= hi_all || !r.ok) {
                         r.step[i] &= j ? 0x0000ffffu : 0xffff0000u;
                         r.small[i] &= j ? 0x0000ffffu : 0xffff0000u;
                     }
-                }
-            if (!r.ok) {
-                odd[0] |= 4u;
-                odd[VP - 1] |= 4u;
-                if (TT * tl + 4 * v_quad < hi_all) atomicOr(b.err, kDevErrBatch);
-            }
-            if (odd[0] | odd[VP - 1]) odd_tile[buf] = tl;
+            if (!r.ok && TT * tl + 4 * v_quad < hi_all) atomicOr(b.err, kDevErrBatch);
         }
+    };
+    const auto check_keys = [&](RawKeys& r) {
+        if (!r.ok) {
 #pragma unroll
-        for (int i = 0; i < VP; ++i) odd_sh[buf][2 * v_quad + v_pair + i] = uint8_t(odd[i]);   // (by every lane of these tokens)
+            for (int i = 0; i < (KW < G ? KW : G); ++i) r.scale[i] = 0;
+            r.of_value = f16(0.0f);
+        }
     };
 
     // q: the second operand, row lane % 32, dims 16k + 8c ..+7
@@ -615,6 +627,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
     f16x o[M::NT] = {};
     const f16* const k_get = &ksh[0][(lane & 31) * KROW + 8 * c];
     const f16* const v_get = &vsh[0][(lane & 31) * VROW + 8 * c];
+    constexpr int AHEAD = 2;                                  // operands read from LDS before their products
     constexpr int P1 = M::MT * M::KS, P2 = M::NT * TT / 16;   // products of the scores, and of the values
     const auto key = [&](int buf, int i) {
         return *reinterpret_cast<const h8*>(k_get + buf * (TT * KROW) + 32 * (i % M::MT) * KROW + 16 * (i / M::MT));
@@ -624,12 +637,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
     };
     // Products of the scores x with tile `buf`'s keys, and beside(i) between them; nothing moves from one to the next.
     const auto score = [&](f16x (&x)[M::MT], int buf, auto&& beside) {
-        h8 k[3] = {key(buf, 0), key(buf, 1)};
+        h8 k[AHEAD + 1];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) k[i] = key(buf, i);
 #pragma unroll
         for (int i = 0; i < P1; ++i) {
-            if (i + 2 < P1) k[(i + 2) % 3] = key(buf, i + 2);
+            if (i + AHEAD < P1) k[(i + AHEAD) % (AHEAD + 1)] = key(buf, i + AHEAD);
             const f16x before = i < M::MT ? f16x{} : x[i % M::MT];
-            x[i % M::MT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i % 3], q[i / M::MT], before, 0, 0, 0);
+            x[i % M::MT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i % (AHEAD + 1)], q[i / M::MT], before, 0, 0, 0);
             beside(i);
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -647,21 +662,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
     f16x x0[M::MT], x1[M::MT];
     RawKeys k_raw;
     RawValues v_raw;
-    Page k_page{}, v_page{};
+    Page page{};    // of the keys to load the next but one time
+    Run k_run{}, v_run{};   // of the keys and values to load next
     // One tile, whose scores are in x and their largest in `most`: their exponentials beside the next tile's products (to y); then the
-    // values' products beside the codes of the next tile's values and of the keys of the one after it, loaded a tile before.
+    // values' products beside the codes of the keys of the tile after the next and of the next one's values, loaded a tile before.
     // Behind the last tile that is work on tokens that are there, not used.
     const auto tile = [&](f16x (&x)[M::MT], f16x (&y)[M::MT], int tl) {
         const int buf = (tl - begin) & 1;
         __syncthreads();
-        // tokens that some rows do not see, or that are held as NaN or have no page
-        if (TT * tl < lo_most || TT * (tl + 1) > hi_least || __builtin_amdgcn_readfirstlane(odd_tile[buf]) == tl) {
+        if (TT * tl < lo_most || TT * (tl + 1) > hi_least) {   // tokens that some rows do not see
 #pragma unroll
             for (int i = 0; i < S; ++i) {
-                const int nth = 32 * (i / 16) + 8 * (i % 16 >> 2) + 4 * c + (i & 3), tok = TT * tl + nth;
-                const uint32_t e = odd_sh[buf][nth >> 1];
-                if (tok < lo || tok >= hi || e >= 4) x[i / 16][i % 16] = -INFINITY;
-                else if (e >> (i & 1) & 1) x[i / 16][i % 16] = NAN;
+                const int tok = TT * tl + 32 * (i / 16) + 8 * (i % 16 >> 2) + 4 * c + (i & 3);
+                if (tok < lo || tok >= hi) x[i / 16][i % 16] = -INFINITY;
             }
             most = kLowest;
             look_over(x, false, 0, S);
@@ -686,44 +699,47 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
                 if (j & 1) asm volatile("" : "+v"(w[j / 2]), "+v"(sum));   // (keeps the exponentials in their place)
             }
         });
-        check_values(v_raw, tl + 1, buf ^ 1);
+        check_keys(k_raw);
+        check_values(v_raw, tl + 1);
         most = kLowest;
-        h8 v[3] = {value(buf, 0), value(buf, 1)};
+        h8 v[AHEAD + 1];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) v[i] = value(buf, i);
 #pragma unroll
         for (int i = 0; i < P2; ++i) {
-            if (i + 2 < P2) v[(i + 2) % 3] = value(buf, i + 2);
+            if (i + AHEAD < P2) v[(i + AHEAD) % (AHEAD + 1)] = value(buf, i + AHEAD);
             const int k = 4 * (i / M::NT);
-            o[i % M::NT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i % 3], join(w[k], w[k + 1], w[k + 2], w[k + 3]), o[i % M::NT], 0, 0, 0);
-            if (i < VSLICES) stage_values(v_raw, buf ^ 1, i);
-            else stage_keys(k_raw, buf, i - VSLICES);
-            if (i == VSLICES) {
-                fetch_values(v_page, v_raw);
-                v_page = k_page;
-            }
+            o[i % M::NT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i % (AHEAD + 1)], join(w[k], w[k + 1], w[k + 2], w[k + 3]), o[i % M::NT], 0, 0, 0);
+            if (i < KSLICES) stage_keys(k_raw, buf, i);
+            else stage_values(v_raw, buf ^ 1, i - KSLICES);
+            if (i == KSLICES) fetch_keys(k_run, k_raw);
             look_over(y, true, i * S / P2, (i + 1) * S / P2);
             __builtin_amdgcn_sched_barrier(0);
         }
         static_assert(VSLICES + KSLICES == P2);
-        fetch_keys(k_page, k_raw);
-        k_page = look(tl + 4);
+        fetch_values(v_run, v_raw);
+        v_run = k_run;
+        k_run = run_of(page);
+        page = look(tl + 5);
     };
-    if (tid < 2) odd_tile[tid] = -1;
     if (begin < end) {
         RawKeys next;
-        const Page p0 = look(begin), p1 = look(begin + 1);
-        fetch_keys(p0, k_raw);
-        fetch_values(p0, v_raw);
-        fetch_keys(p1, next);
-        v_page = look(begin + 2);
-        k_page = look(begin + 3);
-        __syncthreads();   // odd_tile
-        check_values(v_raw, begin, 0);
+        const Run r0 = run_of(look(begin)), r1 = run_of(look(begin + 1));
+        fetch_keys(r0, k_raw);
+        fetch_values(r0, v_raw);
+        fetch_keys(r1, next);
+        v_run = run_of(look(begin + 2));
+        k_run = run_of(look(begin + 3));
+        page = look(begin + 4);
+        check_keys(k_raw);
+        check_values(v_raw, begin);
 #pragma unroll
         for (int i = 0; i < KSLICES; ++i) stage_keys(k_raw, 0, i);
 #pragma unroll
         for (int i = 0; i < VSLICES; ++i) stage_values(v_raw, 0, i);
-        fetch_values(p1, v_raw);
-        fetch_keys(v_page, k_raw);
+        fetch_keys(v_run, k_raw);
+        fetch_values(r1, v_raw);
+        check_keys(next);
 #pragma unroll
         for (int i = 0; i < KSLICES; ++i) stage_keys(next, 1, i);
         __syncthreads();
