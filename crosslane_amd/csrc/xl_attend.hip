@@ -777,69 +777,83 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
     }
 }
 
-// The splits' sums together: W waves for each row and head, 256 / D splits of them at a time in a wave. A wave has
-// the splits' maxima and sums in its lanes (two each: at most 128), and their weights from there.
-template <class T, int D, int W>
-__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
-    constexpr int L = D / 4, P = 64 / L;   // lanes of one split's row, splits at a time
-    __shared__ f4 sums[4][L];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % W;
-    const int64_t row = int64_t(blockIdx.x) * (4 / W) + wave / W;
-    const int t = int(row / a.q_heads), h = int(row - int64_t(t) * a.q_heads);
-    // rows of no sequence have no parts
-    bool there = t < a.b.rows;
-    if (there) {
-        const SeqRows s = seq_rows(a.b, seq_of(a.b, t));
-        there = t >= s.first && t < s.first + s.n;
-    }
+// The splits' sums together, few splits: a thread has four dims of a row and head, and all of its splits.
+template <class T, int D>
+__global__ __launch_bounds__(256) void attend_join_few_kernel(AttendArgs a) {
+    constexpr int L = D / 4;
+    const int64_t row = (int64_t(blockIdx.x) * 256 + threadIdx.x) / L;
+    const int d = 4 * (threadIdx.x % L), t = int(row / a.q_heads), h = int(row - int64_t(t) * a.q_heads);
+    if (t >= a.b.rows) return;
+    const SeqRows s = seq_rows(a.b, seq_of(a.b, t));
+    if (t < s.first || t >= s.first + s.n) return;   // rows of no sequence have no parts
+    const f2* ml = reinterpret_cast<const f2*>(a.part_ml) + row * a.splits;
+    const float* p = a.part + row * a.splits * D + d;
+    float most = kLowest, total = 0.0f;
+    for (int i = 0; i < a.splits; ++i) most = fmaxf(most, ml[i][0]);
     f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-    float total = 0.0f;
-    if (there) {
-        const f2* ml = reinterpret_cast<const f2*>(a.part_ml) + row * a.splits;
-        const f2 none = {kLowest, 0.0f};
-        const f2 u = lane < a.splits ? ml[lane] : none, v = lane + 64 < a.splits ? ml[lane + 64] : none;
-        float most = fmaxf(u[0], v[0]);
-#pragma unroll
-        for (int i = 32; i; i >>= 1) most = fmaxf(most, __shfl_xor(most, i));
-        const float fu = __builtin_amdgcn_exp2f(u[0] - most), fv = __builtin_amdgcn_exp2f(v[0] - most);
-        total = u[1] * fu + v[1] * fv;
-#pragma unroll
-        for (int i = 32; i; i >>= 1) total += __shfl_xor(total, i);
-        const int d = lane % L;
-        const float* p = a.part + row * a.splits * D + 4 * d;
-        for (int k = part * P; k < a.splits; k += 8 * W * P) {   // eight loads on their way
-            f4 x[8];
-            float f[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int i = k + j * W * P + lane / L, in = min(i, a.splits - 1);
-                x[j] = *reinterpret_cast<const f4*>(p + int64_t(in) * D);
-                const float f0 = __shfl(fu, in & 63), f1 = __shfl(fv, in & 63);
-                f[j] = i >= a.splits ? 0.0f : in < 64 ? f0 : f1;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y += x[j] * f[j];
-        }
-#pragma unroll
-        for (int i = L; i < 64; i <<= 1)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] += __shfl_xor(y[j], i);
+#pragma unroll 4
+    for (int i = 0; i < a.splits; ++i) {
+        const float f = __builtin_amdgcn_exp2f(ml[i][0] - most);
+        total += ml[i][1] * f;
+        y += *reinterpret_cast<const f4*>(p + i * D) * f;
     }
-    if constexpr (W > 1) {
-        if (lane < L) sums[wave][lane] = y;
-        __syncthreads();
-        if (wave) return;
-        if (lane < L) {
-#pragma unroll
-            for (int i = 1; i < W; ++i) y += sums[i][lane];
-        }
-    }
-    if (!there || lane >= L) return;
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     T v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = T(y[i] * inv);
-    __builtin_memcpy(static_cast<T*>(a.out) + int64_t(t) * a.out_stride + int64_t(h) * D + 4 * lane, v, sizeof v);
+    __builtin_memcpy(static_cast<T*>(a.out) + int64_t(t) * a.out_stride + int64_t(h) * D + d, v, sizeof v);
+}
+
+// ... many splits: a workgroup for each row and head, 1024 / D splits at a time. Its waves have the splits' maxima and sums in
+// their lanes (two each: at most 128), and the weights from there.
+template <class T, int D>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
+    constexpr int L = D / 4, P = 64 / L;   // lanes of one split's row, splits at a time in a wave
+    __shared__ f4 sums[4][L];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = blockIdx.x;
+    const int t = int(row / a.q_heads), h = int(row - int64_t(t) * a.q_heads);
+    const SeqRows s = seq_rows(a.b, seq_of(a.b, t));
+    if (t < s.first || t >= s.first + s.n) return;   // rows of no sequence have no parts
+    const f2* ml = reinterpret_cast<const f2*>(a.part_ml) + row * a.splits;
+    const f2 none = {kLowest, 0.0f};
+    const f2 u = lane < a.splits ? ml[lane] : none, v = lane + 64 < a.splits ? ml[lane + 64] : none;
+    float most = fmaxf(u[0], v[0]);
+#pragma unroll
+    for (int i = 32; i; i >>= 1) most = fmaxf(most, __shfl_xor(most, i));
+    const float fu = __builtin_amdgcn_exp2f(u[0] - most), fv = __builtin_amdgcn_exp2f(v[0] - most);
+    float total = u[1] * fu + v[1] * fv;
+#pragma unroll
+    for (int i = 32; i; i >>= 1) total += __shfl_xor(total, i);
+    const float* p = a.part + row * a.splits * D + 4 * (lane % L);
+    f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = wave * P; k < a.splits; k += 32 * P) {   // eight loads on their way
+        f4 x[8];
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = k + j * 4 * P + lane / L, in = min(i, a.splits - 1);
+            x[j] = *reinterpret_cast<const f4*>(p + int64_t(in) * D);
+            const float f0 = __shfl(fu, in & 63), f1 = __shfl(fv, in & 63);
+            f[j] = i >= a.splits ? 0.0f : in < 64 ? f0 : f1;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y += x[j] * f[j];
+    }
+#pragma unroll
+    for (int i = L; i < 64; i <<= 1)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] += __shfl_xor(y[j], i);
+    if (lane < L) sums[wave][lane] = y;
+    __syncthreads();
+    if (threadIdx.x >= L) return;
+#pragma unroll
+    for (int i = 1; i < 4; ++i) y += sums[i][lane];
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    T o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = T(y[i] * inv);
+    __builtin_memcpy(static_cast<T*>(a.out) + int64_t(t) * a.out_stride + int64_t(h) * D + 4 * lane, o, sizeof o);
 }
 
 template <class T, int D>
@@ -856,11 +870,11 @@ hipError_t attend_go(const AttendArgs& a, hipStream_t s, hipEvent_t stop) {
     else go(attend_few_kernel<T, D, false>);
     if (a.splits > 1) {
         const int64_t heads = int64_t(a.b.rows) * a.q_heads;
-        const auto join = [&](auto kernel, int w) {
-            hipExtLaunchKernelGGL(kernel, dim3(uint32_t((heads * w + 3) / 4)), dim3(256), 0, s, nullptr, stop, 0, a);
+        const auto join = [&](auto kernel, int64_t groups) {
+            hipExtLaunchKernelGGL(kernel, dim3(uint32_t(groups)), dim3(256), 0, s, nullptr, stop, 0, a);
         };
-        if (a.splits > 16) join(attend_join_kernel<T, D, 4>, 4);
-        else join(attend_join_kernel<T, D, 1>, 1);
+        if (a.splits > 16) join(attend_join_kernel<T, D>, heads);
+        else join(attend_join_few_kernel<T, D>, (heads * (D / 4) + 255) / 256);
     }
     return hipGetLastError();
 }
