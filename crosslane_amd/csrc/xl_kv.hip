@@ -148,7 +148,75 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(KvBatch b, KvRotary 
     }
 }
 
-// A block: one row, blockIdx.y of gridDim.y parts of its heads' chunks (keys, then values).
+// Many rows of a sequence: a wave takes a run of 16 tokens of one head, with the widest loads that the cache's layout has (16 bytes
+// of a token's key codes, of four tokens' value codes, and their scales). A sequence's runs that hold rows, from the run of its first row
+// (below 0 where rows come before the first token), are numbered from starts[q] / 16 + 2q on: n rows lie in at most n / 16 + 2 runs.
+template <class T, int D>
+__global__ __launch_bounds__(kThreads) void kv_read_runs_kernel(KvBatch b, KvRows x) {
+    constexpr int G = D / 32, C = D / 8, VP = D == 64 ? 1 : 2, VC = D == 256 ? 2 : 1;   // pairs of four tokens, and chunks, of a lane's values
+    const int lane = threadIdx.x & 63, groups = (b.kv_heads + 3) >> 2;
+    const int number = blockIdx.x / groups, head = 4 * (blockIdx.x % groups) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    check_batch(b);
+    const auto first_number = [&](int q) { return (b.starts[q] >> 4) + 2 * q; };
+    int seq = 0;
+    for (int hi = b.n_seqs; hi - seq > 1;) {
+        const int mid = (seq + hi) >> 1;
+        if (first_number(mid) <= number) seq = mid;
+        else hi = mid;
+    }
+    const SeqRows s = seq_rows(b, seq);
+    const int first = s.len - s.n, run = (first >> 4) + number - first_number(seq);
+    if (head >= b.kv_heads || s.n == 0 || run < first >> 4 || run > (s.len - 1) >> 4) return;
+    const Slab<D> slab(b.page);
+    int in = 0;
+    const int64_t page = run >= 0 ? page_at(b, seq, uint32_t(run), in) : -1;
+    if (run >= 0 && page < 0 && lane == 0) atomicOr(b.err, kDevErrBatch);
+    const uint8_t* at = b.pages + (page < 0 ? 0 : page) + int64_t(head) * slab.bytes();
+    // the row of a token of the run (below 0 or from s.n on: none)
+    const auto row_of = [&](int tok) { return 16 * run + tok - first; };
+    const auto put = [&](void* out, int64_t stride, int tok, int d, const float (&v)[8]) {
+        const int r = row_of(tok);
+        if (r >= 0 && r < s.n) store8(static_cast<T*>(out) + int64_t(s.first + r) * stride + head * D + d, 8, v);
+    };
+    if (page < 0) {   // no tokens, or no page
+        const float v[8] = {};
+        for (int i = lane; i < 16 * C; i += 64) {
+            put(x.k_out, x.k_stride, i / C, i % C * 8, v);
+            put(x.v_out, x.v_stride, i / C, i % C * 8, v);
+        }
+        return;
+    }
+    const int k_tok = lane & 15, c = lane >> 4;
+    uint32_t kc[G], ks[G], vc[VC][2 * VP], vs[4];
+    const int v_quad = lane >> 4, v_chunk = D == 64 ? lane >> 1 & 7 : (lane & 15) * VC, v_pair = VP == 1 ? lane & 1 : 0;
+    __builtin_memcpy(kc, __builtin_assume_aligned(at + 8 * D * in + 4 * (k_tok * C + c * G), G >= 4 ? 16 : 4 * G), sizeof kc);
+    __builtin_memcpy(ks, __builtin_assume_aligned(at + slab.k_scale(16 * in + k_tok, 0), G >= 4 ? 16 : 4 * G), sizeof ks);
+    __builtin_memcpy(vc, __builtin_assume_aligned(at + slab.v_codes() + 8 * D * in + 2 * (v_quad * D + v_chunk * 8) + 8 * v_pair, 8 * VP), sizeof vc);
+    __builtin_memcpy(vs, __builtin_assume_aligned(at + slab.v_scale(16 * in + 4 * v_quad, v_chunk / 4), 16), sizeof vs);
+    const auto half = [](uint32_t w, int i) { return float(__builtin_bit_cast(f16, uint16_t(i ? w >> 16 : w))); };
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = fmaf(float(kc[g] >> (k / 2 * 4 + k % 2 * 16) & 15u), half(ks[g], 0), half(ks[g], 1));
+        put(x.k_out, x.k_stride, k_tok, 32 * g + 8 * c, v);
+    }
+#pragma unroll
+    for (int u = 0; u < VC; ++u)
+#pragma unroll
+        for (int p = 0; p < VP; ++p)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int pair = VP == 1 ? v_pair : p;
+                const uint32_t step = VP == 1 ? (v_pair ? vs[1] : vs[0]) : vs[p], small = VP == 1 ? (v_pair ? vs[3] : vs[2]) : vs[2 + p];
+                float v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = fmaf(float(vc[u][2 * p + k / 4] >> (16 * e + k % 4 * 4) & 15u), half(step, e), half(small, e));
+                put(x.v_out, x.v_stride, 4 * v_quad + 2 * pair + e, 8 * (v_chunk + u), v);
+            }
+}
+
+// Few rows of each: a block has one row, blockIdx.y of gridDim.y parts of its heads' chunks (keys, then values).
 template <class T, int D>
 __global__ __launch_bounds__(kThreads) void kv_read_kernel(KvBatch b, KvRows x) {
     constexpr int C = D / 8;
@@ -200,6 +268,11 @@ hipError_t write_go(const KvBatch& b, const KvRotary& r, const KvRows& x, hipStr
 }
 template <class T, int D>
 hipError_t read_go(const KvBatch& b, const KvRows& x, hipStream_t s, hipEvent_t stop) {
+    if (b.max_rows >= 16) {
+        const int64_t runs = (int64_t(b.rows) >> 4) + 2 * int64_t(b.n_seqs), groups = (b.kv_heads + 3) / 4;
+        hipExtLaunchKernelGGL((kv_read_runs_kernel<T, D>), dim3(uint32_t(runs * groups)), dim3(kThreads), 0, s, nullptr, stop, 0, b, x);
+        return hipGetLastError();
+    }
     const int items = 2 * b.kv_heads * (D / 8);
     hipExtLaunchKernelGGL((kv_read_kernel<T, D>), dim3(b.rows, parts(b.rows, items)), dim3(kThreads), 0, s, nullptr, stop, 0, b, x);
     return hipGetLastError();
