@@ -72,6 +72,9 @@ class _Rotary(C.Structure):
                 ("positions", _P)]
 
 
+_ROTARY_BYTES = C.sizeof(_Rotary)
+
+
 class _PackMeta(C.Structure):
     _fields_ = [("struct_bytes", C.c_uint32), ("dim", C.c_int32), ("ff", C.c_int32), ("n_layers", C.c_int32),
                 ("n_experts", C.c_int32), ("top_k", C.c_int32), ("swiglu_limit", C.c_float)]
@@ -299,16 +302,16 @@ def _vec(t, n: int, what: str, kind: int = 0):
 
 def _heads(t, what: str, shape):
     """[rows, heads, head_dim] on the GPU, a row's heads consecutive: address, row stride, element type."""
-    sh, st = t.shape, t.stride()
-    if sh != shape:
-        _refuse(f"{what}: shape {tuple(sh)} where {tuple(shape)} is wanted")
-    if st[2] != 1 or (st[1] != sh[2] and sh[1] != 1):
-        _refuse(f"{what}: a row's heads must be consecutive")
-    if not t.is_cuda:
+    rows, heads, dim = shape
+    row, st1, st2 = t.stride() if t.shape == shape else (0, 0, 0)
+    if st2 != 1 or (st1 != dim and heads != 1) or not t.is_cuda:
+        if t.shape != shape:
+            _refuse(f"{what}: shape {tuple(t.shape)} where {tuple(shape)} is wanted")
+        if st2 != 1 or (st1 != dim and heads != 1):
+            _refuse(f"{what}: a row's heads must be consecutive")
         _refuse(f"{what}: not on the GPU")
-    row = st[0]
-    if sh[0] == 1 and row < sh[1] * sh[2]:
-        row = sh[1] * sh[2]
+    if rows == 1 and row < heads * dim:
+        row = heads * dim
     return t.data_ptr(), row, _KINDS[t.dtype]
 
 
@@ -353,6 +356,7 @@ class KVBatch:
                                _vec(lens, n, "lens", _INT32), _vec(starts, n + 1, "starts", _INT32))
         self.ref = C.addressof(self.struct)
         self._kv_shape = (self.rows, self.kv_heads, self.head_dim)
+        self.scale = self.head_dim ** -0.5
 
 
 def attention_work_bytes(batch: KVBatch, q_heads: int) -> int:
@@ -792,8 +796,10 @@ class Lane:
         if q is not None:
             if q_out is None:
                 _refuse("q needs q_out")
-            heads = q.shape[1] if q.dim() == 3 else 0
-            shape = (batch.rows, heads, batch.head_dim)
+            shape = q.shape
+            if len(shape) != 3 or shape[0] != batch.rows or shape[2] != batch.head_dim:
+                _refuse(f"q: shape {tuple(shape)} where [{batch.rows}, q_heads, {batch.head_dim}] is wanted")
+            heads = shape[1]
             qp, qs, qk = _heads(q, "q", shape)
             op, os_, ok = _heads(q_out, "q_out", shape)
             if qk != kind or ok != kind:
@@ -812,15 +818,16 @@ class Lane:
                     pp, pstride, pk = _mat(positions, "positions", (axes, batch.rows))
                     if pk != _INT32:
                         _refuse("positions: int32 is wanted")
-            parts = [n] if sections is None else list(sections)
+            parts = (n,) if sections is None else sections
             if len(parts) != axes or not 1 <= axes <= 3:
                 _refuse("a section for each of one to three axes is wanted")
-            rotary = _Rotary(C.sizeof(_Rotary), n, axes, bool(interleaved), tuple(parts + [0] * (3 - axes)), 0, pstride,
-                             _vec(freqs, n, "freqs"), pp)
+            rotary = _Rotary(_ROTARY_BYTES, n, axes, bool(interleaved), (*parts, 0, 0)[:3], 0, pstride, _vec(freqs, n, "freqs"), pp)
         elif q is not None or positions is not None or sections is not None:
             _refuse("q, positions and sections go with freqs")
-        _check(lib().xl_kv_write_async(self._ctx, batch.ref, kp, ks, vp, vs, kind, None if rotary is None else C.addressof(rotary),
-                                       qp, qs, heads, op, os_, None if stream is None else int(stream), self._errp), self._err)
+        rc = lib().xl_kv_write_async(self._ctx, batch.ref, kp, ks, vp, vs, kind, None if rotary is None else C.addressof(rotary),
+                                     qp, qs, heads, op, os_, None if stream is None else int(stream), self._errp)
+        if rc:
+            _check(rc, self._err)
 
     def kv_read_async(self, batch: KVBatch, k, v, stream=None) -> None:
         """What the batch's cache holds at its rows' positions, into k and v [rows, kv_heads, head_dim]."""
@@ -828,8 +835,9 @@ class Lane:
         vp, vs, vk = _heads(v, "v", batch._kv_shape)
         if not 0 <= kind < _INT8 or vk != kind:
             _refuse("k and v must have one element type, f32, f16 or bf16")
-        _check(lib().xl_kv_read_async(self._ctx, batch.ref, kp, ks, vp, vs, kind, None if stream is None else int(stream),
-                                      self._errp), self._err)
+        rc = lib().xl_kv_read_async(self._ctx, batch.ref, kp, ks, vp, vs, kind, None if stream is None else int(stream), self._errp)
+        if rc:
+            _check(rc, self._err)
 
     def attention_async(self, batch: KVBatch, q, out, scale: Optional[float] = None, window: int = 0, softcap: float = 0.0,
                         work=None, stream=None) -> None:
@@ -837,8 +845,10 @@ class Lane:
         bf16): tokens up to each row's own, with window > 0 the last `window` of them, softcap > 0: scores
         through softcap * tanh(score / softcap). scale: 1 / sqrt(head_dim) by default. work:
         attention_work_bytes(batch, q_heads) bytes (None where that is 0)."""
-        heads = q.shape[1] if q.dim() == 3 else 0
-        shape = (batch.rows, heads, batch.head_dim)
+        shape = q.shape
+        if len(shape) != 3 or shape[0] != batch.rows or shape[2] != batch.head_dim:
+            _refuse(f"q: shape {tuple(shape)} where [{batch.rows}, q_heads, {batch.head_dim}] is wanted")
+        heads = shape[1]
         qp, qs, kind = _heads(q, "q", shape)
         op, os_, ok = _heads(out, "out", shape)
         if kind not in (1, 2) or ok != kind:
@@ -849,9 +859,10 @@ class Lane:
                 _refuse("work: a contiguous GPU buffer is wanted")
             wb = work.nbytes
             wp = work.data_ptr() if wb else None
-        _check(lib().xl_attention_async(self._ctx, batch.ref, qp, qs, heads, kind, batch.head_dim ** -0.5 if scale is None else scale,
-                                        window, softcap, op, os_, wp, wb, None if stream is None else int(stream), self._errp),
-               self._err)
+        rc = lib().xl_attention_async(self._ctx, batch.ref, qp, qs, heads, kind, batch.scale if scale is None else scale, window,
+                                      softcap, op, os_, wp, wb, None if stream is None else int(stream), self._errp)
+        if rc:
+            _check(rc, self._err)
 
     def swiglu_async(self, g, u, h, limit: float = 0.0, stream=None) -> None:
         self._call("xl_swiglu_async", _ptr(g), _ptr(u), int(g.numel()), float(limit), _ptr(h),
