@@ -18,7 +18,10 @@
 namespace xl {
 namespace {
 
-constexpr int kFewRows = 32;      // rows (of a sequence and a kv head) up to which attend_few_kernel takes them
+// Rows (of a sequence and a kv head) up to which attend_few_kernel takes them, 16 at a time: of 24 sequences with up to 12 rows and
+// 9000 tokens, group 4 (48 rows), 59 us for 109 of attend_many_kernel; one sequence of 131072 tokens, 48 rows: 96 for 90,
+// 96 rows: 172 for 95; heads of 256, 72 rows: 121 for 229, 192 rows: 231 for 315.
+constexpr int few_rows(int dim) { return dim == 256 ? 192 : 64; }
 
 }  // namespace
 
@@ -29,14 +32,15 @@ AttendPlan attend_plan(int dim, int kv_heads, int q_heads, int n_seqs, int rows,
     AttendPlan p;
     const int64_t group = q_heads / kv_heads, most = max_rows * group;
     const int64_t tokens = window ? std::min(max_tokens, int64_t(window) + max_rows) : max_tokens;
-    p.few = most <= kFewRows;
+    p.few = most <= few_rows(dim);
     int64_t wgs;
     if (p.few) {
         p.tiles = int((most + 15) / 16);
         wgs = int64_t(n_seqs) * kv_heads * p.tiles;
         const int64_t held = dim < 256 ? 1024 : 512;
         const auto splits = [&](int64_t groups, int64_t least) { return std::min((groups + wgs - 1) / wgs, (tokens + least - 1) / least); };
-        p.splits = int(std::min<int64_t>(128, std::max(splits(held, 256), splits(4 * held, 1024))));
+        // (512 tokens: 11.4 us in one piece, 15.3 in two; 1024: 14.7 and 14.7)
+        if (tokens > 768) p.splits = int(std::min<int64_t>(128, std::max(splits(held, 256), splits(4 * held, 1024))));
     } else {
         p.tiles = int((rows * group >> 7) + n_seqs);   // numbers for them; about half a tile of each sequence has rows
         wgs = int64_t(kv_heads) * p.tiles;
