@@ -46,7 +46,7 @@ AttendPlan attend_plan(int dim, int kv_heads, int q_heads, int n_seqs, int rows,
         wgs = int64_t(kv_heads) * p.tiles;
         const int64_t real = kv_heads * (((rows * group + 127) >> 7) + (n_seqs - 1) / 2);
         double best = 1e30;
-        for (int64_t k = 1; k <= 128 && (k == 1 || (real * k <= 2048 && tokens >= 512 * k)); ++k) {
+        for (int64_t k = 1; k <= 128 && (k == 1 || (real * k <= 2048 && tokens >= 256 * k)); ++k) {
             const double rounds = double((real * k + 511) / 512), join = k == 1 ? 0.0 : 4.0 + double(rows) * q_heads * dim * double(k) * 1e-6;
             const double us = rounds * (0.03 * double(tokens) / double(k) + 5.0) + join;
             if (us < best) {
@@ -494,7 +494,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
     const int hi_least = sees(row0 + min(32 * wave, rows - 1)), lo_most = from(sees(row0 + min(32 * wave + 31, rows - 1)));
     const int hi_all = sees(row0 + rows - 1), lo_all = from(sees(row0));
     const int tile0 = lo_all / TT, tiles = hi_all > lo_all ? (hi_all + TT - 1) / TT - tile0 : 0;
-    const int per = max(1024 / TT, (tiles + a.splits - 1) / a.splits);
+    const int per = max(256 / TT, (tiles + a.splits - 1) / a.splits);
     const int begin = tile0 + split * per, end = tile0 + min(tiles, (split + 1) * per);
 
     // This thread's part of a tile: words of one token's keys, and eight dims of four (or two) tokens' values. A wave's lie in one run
