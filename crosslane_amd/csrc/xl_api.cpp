@@ -2020,8 +2020,8 @@ xl::KvBatch kv_numbers(const xl_kv_batch* b) {
          "page_tokens must be a multiple of 16 up to 1024");
     need(b->n_pages >= 1 && b->max_pages >= 1 && int64_t(b->max_pages) * b->page_tokens <= (int64_t(1) << 26), XL_E_ARG,
          "n_pages below 1, or max_pages * page_tokens outside 1..2^26");
-    need(b->n_seqs >= 1 && b->n_seqs <= 65535 && b->rows >= 1 && b->rows <= 1 << 24, XL_E_ARG,
-         "n_seqs outside 1..65535 or rows outside 1..2^24");
+    need(b->n_seqs >= 1 && b->n_seqs <= 65535 && b->rows >= 1 && b->rows <= 1 << 23, XL_E_ARG,
+         "n_seqs outside 1..65535 or rows outside 1..2^23");
     need(b->max_rows >= 1 && b->max_rows <= b->rows, XL_E_ARG, "max_rows outside 1..rows");
     need(b->reserved == 0, XL_E_ARG, "reserved must be 0");
     xl::KvBatch k{};
@@ -2062,6 +2062,12 @@ xl::KvBatch kv_batch(const xl_kv_batch* b, KvSpans& sp) {
     sp.lens = Span{b->d_lens, uint64_t(k.n_seqs) * 4};
     sp.starts = Span{b->d_starts, uint64_t(k.n_seqs + 1) * 4};
     return k;
+}
+// Whether two matrices of n columns are different columns of the same rows.
+bool columns_apart(const void* p, const void* q, int64_t p_stride, int64_t q_stride, int64_t n, int64_t rows, int size) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+    const uint64_t gap = a < b ? b - a : a - b;
+    return p_stride == q_stride && rows > 1 && gap >= uint64_t(n * size) && gap + uint64_t(n * size) <= uint64_t(p_stride * size);
 }
 void check_heads(int32_t q_heads, int32_t kv_heads) {
     need(q_heads >= 1 && q_heads <= 1024 && q_heads % kv_heads == 0, XL_E_ARG,
@@ -2151,8 +2157,9 @@ int32_t xl_kv_read_async(xl_context* ctx, const xl_kv_batch* batch, void* d_k, i
         check_rows(d_k, k_stride, kv, es, "k");
         check_rows(d_v, v_stride, kv, es, "v");
         const Span k{d_k, extent(b.rows, kv, k_stride, es)}, v{d_v, extent(b.rows, kv, v_stride, es)};
-        check_apart(k, {sp.pages, sp.table, sp.lens, sp.starts, v}, "k");
+        check_apart(k, {sp.pages, sp.table, sp.lens, sp.starts}, "k");
         check_apart(v, {sp.pages, sp.table, sp.lens, sp.starts}, "v");
+        if (!columns_apart(d_k, d_v, k_stride, v_stride, kv, b.rows, es)) check_apart(k, {v}, "k");
         ready(ctx, false);
         b.err = ctx->err_flag;
         hipStream_t s = pick_stream(ctx, stream);
@@ -2182,15 +2189,17 @@ int32_t xl_attention_async(xl_context* ctx, const xl_kv_batch* batch, const void
         need(d_q && d_out, XL_E_ARG, "null device pointer");
         need(type == XL_F16 || type == XL_BF16, XL_E_ARG, "q and out must be f16 or bf16");
         check_heads(q_heads, b.kv_heads);
-        need(std::isfinite(scale) && std::isfinite(softcap) && softcap >= 0.0f, XL_E_ARG,
-             "scale must be finite, softcap finite and >= 0");
+        need(std::isfinite(scale) && std::isfinite(softcap) && (softcap == 0.0f || softcap >= 1e-20f), XL_E_ARG,
+             "scale must be finite, softcap 0 or finite and at least 1e-20");
         need(window >= 0, XL_E_ARG, "window below 0");
+        if (window > 1 << 26) window = 0;   // no sequence is longer
         const int64_t width = int64_t(q_heads) * b.dim;
         check_rows(d_q, q_stride, width, 2, "q");
         check_rows(d_out, out_stride, width, 2, "out");
         const xl::AttendPlan plan = attend_plan_of(b, q_heads, window);
         const uint64_t whole = attend_plan_of(b, q_heads, 0).bytes;
-        need(plan.groups <= 0x7fffffff, XL_E_ARG, "more workgroups than a launch takes: n_seqs * max_rows * q_heads too large");
+        // (a launch counts threads in 32 bits)
+        need(plan.groups < 1 << 24, XL_E_ARG, "more workgroups than a launch takes: n_seqs * max_rows * q_heads too large");
         need(work_bytes >= whole && (d_work || whole == 0), XL_E_ARG,
              "workspace smaller than xl_attention_work_bytes(batch, q_heads)");
         need(reinterpret_cast<uintptr_t>(d_work) % 256 == 0, XL_E_ARG, "workspace not 256-byte aligned");

@@ -26,7 +26,7 @@ constexpr int few_rows(int dim) { return dim == 256 ? 192 : 64; }
 }  // namespace
 
 // Few rows: as many workgroups as the card holds at once (four a CU, two of heads of 256 values) where each has 256 tokens at
-// least, or four times as many for an even end where each has 1024. Many rows: the least of the rounds that 512 workgroups at a
+// least, or four times as many for an even end where each has 1536. Many rows: the least of the rounds that 512 workgroups at a
 // time make, at 0.03 us a token and 5 us a workgroup, and the join's bytes at 4 TB/s.
 AttendPlan attend_plan(int dim, int kv_heads, int q_heads, int n_seqs, int rows, int max_rows, int64_t max_tokens, int window) {
     AttendPlan p;
@@ -40,7 +40,7 @@ AttendPlan attend_plan(int dim, int kv_heads, int q_heads, int n_seqs, int rows,
         const int64_t held = dim < 256 ? 1024 : 512;
         const auto splits = [&](int64_t groups, int64_t least) { return std::min((groups + wgs - 1) / wgs, (tokens + least - 1) / least); };
         // (512 tokens: 11.4 us in one piece, 15.3 in two; 1024: 14.7 and 14.7)
-        if (tokens > 768) p.splits = int(std::min<int64_t>(128, std::max(splits(held, 256), splits(4 * held, 1024))));
+        if (tokens > 768) p.splits = int(std::min<int64_t>(128, std::max(splits(held, 256), splits(4 * held, 1536))));
     } else {
         p.tiles = int((rows * group >> 7) + n_seqs);   // numbers for them; about half a tile of each sequence has rows
         wgs = int64_t(kv_heads) * p.tiles;
@@ -55,7 +55,9 @@ AttendPlan attend_plan(int dim, int kv_heads, int q_heads, int n_seqs, int rows,
             }
         }
     }
-    p.groups = std::max(wgs * p.splits, int64_t(rows) * q_heads);
+    const int64_t heads = int64_t(rows) * q_heads;
+    p.groups = wgs * p.splits;
+    if (p.splits > 1) p.groups = std::max(p.groups, p.splits > 16 ? heads : (heads * (dim / 4) + 255) / 256);
     if (p.splits > 1) {
         const uint64_t parts = uint64_t(rows) * uint64_t(q_heads) * uint64_t(p.splits);
         p.part_ml = align256(parts * uint64_t(dim) * 4);

@@ -515,7 +515,7 @@ typedef struct xl_kv_batch {
     int32_t n_pages;
     int32_t max_pages;       /* columns of the table; max_pages * page_tokens <= 2^26 */
     int32_t n_seqs;          /* 1..65535 */
-    int32_t rows;            /* rows of q, k, v and the outputs, 1..2^24 */
+    int32_t rows;            /* rows of q, k, v and the outputs, 1..2^23 */
     int32_t max_rows;        /* no sequence has more rows (1..rows); more: the device flag */
     int32_t reserved;        /* 0 */
     int64_t page_stride;     /* bytes from page to page, a multiple of 16 */

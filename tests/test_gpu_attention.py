@@ -112,7 +112,7 @@ CASES = [
 
 
 @pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(map(str, c)).replace(" ", ""))
-@pytest.mark.parametrize("tail", [None, 0x7e], ids=["", "nan-tail"])
+@pytest.mark.parametrize("tail", [None, 0x7e, 0x7b, 0xfc], ids=["", "nan-tail", "large-tail", "minus-nan-tail"])
 def test_attention(lane, case, tail):  # noqa: F811
     seqs, P, KV, H, D, kind, window, softcap, behind, before, pad = case
     step(f"attention {case} {tail}")
@@ -143,7 +143,7 @@ def test_peaked_and_large(lane, rows, length, H):  # noqa: F811
     out = torch.full((rows, H, 128), 7.0, dtype=torch.bfloat16, device="cuda")
     work = work_of(b, H)
     torch.cuda.synchronize()
-    for scale in (1.0 / big, 0.05 / big, -1.0 / big):
+    for scale in (1.0 / big, 0.05 / big, -1.0 / big, 0.0):
         lane.attention_async(b.kv, q, out, scale=scale, work=work)
         lane.sync()
         check(b, c, q32 * np.float32(big), out.double().cpu().numpy(), H, "bf16", scale, 0, 0.0)
@@ -214,3 +214,19 @@ def test_shared_pages(lane):  # noqa: F811
     lane.attention_async(b.kv, q, out, work=work)
     lane.sync()
     check(b, c, q32, out.double().cpu().numpy(), 4, "f16", 0.125, 0, 0.0)
+
+
+@pytest.mark.parametrize("rows", [3, 90])
+def test_wide_windows(lane, rows):  # noqa: F811
+    """Windows as long as a number can be, with rows before the first token."""
+    step(f"attention, wide windows {rows}")
+    b = Batch([(rows, rows - 2), (rows, 200)], 16, 1, 64)
+    c = filled(b, 2)
+    q, q32 = rand_rows(b.rows, 2, 64, "f16", 5, 0, 0.5)
+    work = work_of(b, 2)
+    for window in (0, 2 ** 31 - 1, 2 ** 26, 200):
+        out = torch.full((b.rows, 2, 64), 7.0, dtype=torch.float16, device="cuda")
+        torch.cuda.synchronize()
+        lane.attention_async(b.kv, q, out, window=window, work=work)
+        lane.sync()
+        check(b, c, q32, out.double().cpu().numpy(), 2, "f16", 0.125, window, 0.0)

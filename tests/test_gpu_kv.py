@@ -251,3 +251,27 @@ def test_batches_out_of_range():
             assert np.array_equal(b.cache.cpu().numpy(), ref.raw), what
         assert (out[-2:] == 7).all() and (got[0][-2:] == 7).all()
         assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+def test_read_into_columns(lane, rows):
+    """Keys and values as columns of the same rows."""
+    step(f"kv read into columns {rows}")
+    b = Batch([(rows, 50), (2, 2)], 16, 2, 64)
+    k, k32 = rand_rows(b.rows, 2, 64, "f16", 1)
+    v, v32 = rand_rows(b.rows, 2, 64, "f16", 2)
+    both = torch.full((b.rows, 5, 64), 7.0, device="cuda")
+    torch.cuda.synchronize()
+    lane.kv_write_async(b.kv, k, v)
+    lane.kv_read_async(b.kv, both[:, 3:], both[:, :2])
+    lane.sync()
+    ref = b.ref()
+    for t, i, p in b.places():
+        for h in range(2):
+            ref.put(b.table[i, p // 16], h, p % 16, k32[t, h], v32[t, h])
+    got = both.cpu().numpy()
+    assert (got[:, 2] == 7).all()
+    for t, i, p in b.places():
+        for h in range(2):
+            x, y = (z[p % 16] for z in ref.values(b.table[i, p // 16], h))
+            assert np.abs(got[t, 3 + h] - x).max() <= 2.0 ** -23 * np.abs(x).max() and np.abs(got[t, h] - y).max() <= 2.0 ** -23 * np.abs(y).max()

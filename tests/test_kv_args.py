@@ -54,7 +54,9 @@ def call(name, change):
     ("xl_kv_write_async", {"r_section": (0, 64, 0)}), ("xl_kv_write_async", {"r_n_freqs": 1, "r_section": (0, 0, 1)}),
     # parts of the same rows
     ("xl_kv_write_async", {"q": 7 * A, "k": 7 * A + 2 * 768, "v": 7 * A + 2 * 1024, "q_stride": 1280, "k_stride": 1280, "v_stride": 1280}),
-    ("xl_kv_read_async", {}), ("xl_attention_async", {}), ("xl_attention_async", {"window": 1, "softcap": 30.0}),
+    ("xl_kv_read_async", {}), ("xl_attention_async", {}), ("xl_attention_async", {"window": 2 ** 31 - 1}),
+    # keys and values as columns of the same rows
+    ("xl_kv_read_async", {"v": 7 * A + 4 * 256, "k_stride": 512, "v_stride": 512}), ("xl_kv_read_async", {"k": 8 * A + 4 * 300, "k_stride": 556, "v_stride": 556}), ("xl_attention_async", {"window": 1, "softcap": 30.0}),
     ("xl_attention_async", {"scale": -1.0}), ("xl_attention_async", {"b_page_tokens": 1024, "b_page_stride": 2 * 1024 * 160}),
     ("xl_attention_async", {"b_page_stride": 1 << 40, "b_n_pages": 1}),
 ], ids=str)
@@ -66,7 +68,7 @@ def test_good_arguments_reach_the_context(name, change):
 BATCH_BAD = [({"b_head_dim": 96}, "head_dim"), ({"b_kv_heads": 0}, "kv_heads"), ({"b_kv_heads": 257}, "kv_heads"),
              ({"b_page_tokens": 24}, "page_tokens"), ({"b_page_tokens": 0}, "page_tokens"), ({"b_page_tokens": 1040}, "page_tokens"),
              ({"b_n_pages": 0}, "n_pages"), ({"b_max_pages": 0}, "max_pages"), ({"b_max_pages": (1 << 21) + 1}, "max_pages"),
-             ({"b_n_seqs": 0}, "n_seqs"), ({"b_n_seqs": 65536}, "n_seqs"), ({"b_rows": 0}, "rows"), ({"b_rows": (1 << 24) + 1}, "rows"),
+             ({"b_n_seqs": 0}, "n_seqs"), ({"b_n_seqs": 65536}, "n_seqs"), ({"b_rows": 0}, "rows"), ({"b_rows": (1 << 23) + 1}, "rows"),
              ({"b_max_rows": 0}, "max_rows"), ({"b_max_rows": 8}, "max_rows"), ({"b_reserved": 1}, "reserved"),
              ({"b_page_stride": 2 * 32 * 160 - 16}, "page_stride"), ({"b_page_stride": 2 * 32 * 160 + 8}, "page_stride"),
              ({"b_page_stride": (1 << 40) + 16}, "page_stride"), ({"b_pages": A + 8}, "16-byte"), ({"b_pages": None}, "null"),
@@ -93,8 +95,10 @@ BAD = [(n, c, m) for n in CALLS for c, m in BATCH_BAD] + [
     ("xl_attention_async", {"q": None}, "null"), ("xl_attention_async", {"out": None}, "null"), ("xl_attention_async", {"type": 0}, "f16"),
     ("xl_attention_async", {"q_heads": 7}, "q_heads"), ("xl_attention_async", {"q_heads": 1026}, "q_heads"),
     ("xl_attention_async", {"scale": float("nan")}, "scale"), ("xl_attention_async", {"softcap": -1.0}, "softcap"),
-    ("xl_attention_async", {"softcap": float("inf")}, "softcap"), ("xl_attention_async", {"window": -1}, "window"),
-    ("xl_attention_async", {"b_n_seqs": 65535, "b_rows": 1 << 24, "b_max_rows": 1 << 24, "b_kv_heads": 256, "q_heads": 1024,
+    ("xl_attention_async", {"softcap": float("inf")}, "softcap"), ("xl_attention_async", {"softcap": 1e-21}, "softcap"),
+    ("xl_kv_read_async", {"v": 7 * A + 4 * 256, "k_stride": 511, "v_stride": 511}, "overlaps"),
+    ("xl_kv_read_async", {"v": 7 * A + 4 * 256, "k_stride": 512, "v_stride": 768}, "overlaps"), ("xl_attention_async", {"window": -1}, "window"),
+    ("xl_attention_async", {"b_n_seqs": 65535, "b_rows": 1 << 23, "b_max_rows": 1 << 23, "b_kv_heads": 256, "q_heads": 1024,
                             "b_page_stride": 256 * 32 * 160, "q_stride": 1 << 17, "out_stride": 1 << 17}, "workgroups"),
     ("xl_attention_async", {"q_stride": 700}, "stride"), ("xl_attention_async", {"out": 8 * A + 1}, "aligned"),
     ("xl_attention_async", {"work": 9 * A + 128}, "256-byte"), ("xl_attention_async", {"out": 7 * A}, "overlaps"),
