@@ -154,8 +154,9 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(KvBatch b, KvRotary 
 template <class T, int D>
 __global__ __launch_bounds__(kThreads) void kv_read_runs_kernel(KvBatch b, KvRows x) {
     constexpr int G = D / 32, C = D / 8, VP = D == 64 ? 1 : 2, VC = D == 256 ? 2 : 1;   // pairs of four tokens, and chunks, of a lane's values
-    const int lane = threadIdx.x & 63, groups = (b.kv_heads + 3) >> 2;
-    const int number = blockIdx.x / groups, head = 4 * (blockIdx.x % groups) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const uint32_t pair = 4 * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // a run's number and a head
+    const int number = pair / uint32_t(b.kv_heads), head = pair - uint32_t(number) * uint32_t(b.kv_heads);
     check_batch(b);
     const auto first_number = [&](int q) { return (b.starts[q] >> 4) + 2 * q; };
     int seq = 0;
@@ -166,7 +167,7 @@ __global__ __launch_bounds__(kThreads) void kv_read_runs_kernel(KvBatch b, KvRow
     }
     const SeqRows s = seq_rows(b, seq);
     const int first = s.len - s.n, run = (first >> 4) + number - first_number(seq);
-    if (head >= b.kv_heads || s.n == 0 || run < first >> 4 || run > (s.len - 1) >> 4) return;
+    if (s.n == 0 || run < first >> 4 || run > (s.len - 1) >> 4) return;
     const Slab<D> slab(b.page);
     int in = 0;
     const int64_t page = run >= 0 ? page_at(b, seq, uint32_t(run), in) : -1;
@@ -269,9 +270,11 @@ hipError_t write_go(const KvBatch& b, const KvRotary& r, const KvRows& x, hipStr
 template <class T, int D>
 hipError_t read_go(const KvBatch& b, const KvRows& x, hipStream_t s, hipEvent_t stop) {
     if (b.max_rows >= 16) {
-        const int64_t runs = (int64_t(b.rows) >> 4) + 2 * int64_t(b.n_seqs), groups = (b.kv_heads + 3) / 4;
-        hipExtLaunchKernelGGL((kv_read_runs_kernel<T, D>), dim3(uint32_t(runs * groups)), dim3(kThreads), 0, s, nullptr, stop, 0, b, x);
-        return hipGetLastError();
+        const int64_t pairs = ((int64_t(b.rows) >> 4) + 2 * int64_t(b.n_seqs)) * b.kv_heads;
+        if (pairs < int64_t(1) << 26) {   // (a launch counts threads in 32 bits)
+            hipExtLaunchKernelGGL((kv_read_runs_kernel<T, D>), dim3(uint32_t((pairs + 3) / 4)), dim3(kThreads), 0, s, nullptr, stop, 0, b, x);
+            return hipGetLastError();
+        }
     }
     const int items = 2 * b.kv_heads * (D / 8);
     hipExtLaunchKernelGGL((kv_read_kernel<T, D>), dim3(b.rows, parts(b.rows, items)), dim3(kThreads), 0, s, nullptr, stop, 0, b, x);
