@@ -2189,8 +2189,8 @@ int32_t xl_attention_async(xl_context* ctx, const xl_kv_batch* batch, const void
         need(d_q && d_out, XL_E_ARG, "null device pointer");
         need(type == XL_F16 || type == XL_BF16, XL_E_ARG, "q and out must be f16 or bf16");
         check_heads(q_heads, b.kv_heads);
-        need(std::isfinite(scale) && std::isfinite(softcap) && (softcap == 0.0f || softcap >= 1e-20f), XL_E_ARG,
-             "scale must be finite, softcap 0 or finite and at least 1e-20");
+        need(std::isfinite(scale) && std::isfinite(softcap) && (softcap == 0.0f || (softcap >= 1e-20f && softcap <= 16384.0f)), XL_E_ARG,
+             "scale must be finite, softcap 0 or 1e-20 to 16384");
         need(window >= 0, XL_E_ARG, "window below 0");
         if (window > 1 << 26) window = 0;   // no sequence is longer
         const int64_t width = int64_t(q_heads) * b.dim;

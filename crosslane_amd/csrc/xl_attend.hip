@@ -5,8 +5,14 @@
 // One pass over the tokens: m is a maximum so far, and where a later one passes it by more
 // than 2^8 in weight, what was summed is scaled down. Codes of 4 bits become float16 by two
 // instructions a pair (bits under an exponent, and that exponent's value off again) and their
-// scale and smallest value by one fused multiply-add, rounded to float16 once: half a step
-// of 2^-11, an eighth of what bfloat16 outputs round away and as much as float16 ones do.
+// scale and smallest value by one fused multiply-add. Scores, maxima, sums and outputs are
+// float32; what is rounded to float16, once each, by at most 2^-11 of itself:
+//   - keys and values, since the matrix cores take float16 operands. Exact ones would be two
+//     operands each (s * code has 15 bits, and m another exponent), so twice the products and
+//     the LDS. An eighth of what bfloat16 outputs round away; as much as float16 ones do, so that
+//     those are within two and a half of their own roundings (rms 5.3e-4 of the outputs' rms, 2.1e-4
+//     with exact operands), most of it by the keys.
+//   - weights, for the second product. Their sum is of the weights before.
 #include <hip/hip_ext.h>
 
 #include <algorithm>
@@ -72,7 +78,6 @@ namespace {
 typedef f16 h2 __attribute__((ext_vector_type(2)));
 typedef f16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLowest = -3.402823466e38f;   // a maximum before any token (below every score but -inf)
@@ -118,12 +123,14 @@ __device__ __forceinline__ float rows_sum(float v) {
     v += __shfl_xor(v, 16);
     return v + __shfl_xor(v, 32);
 }
-// softcap * tanh(x / softcap), times log2(e): tanh y = 1 - 2 / (exp(2 y) + 1), within 2^-22 of 1.
+// Scores through softcap * tanh(score / softcap), of a row's products x: tanh y = 2 / (1 + exp(-2 y)) - 1. A row's scores may all be off
+// by the same, so the -1 is left out: 1 / (1 + exp(-2 y)) of each, and twice softcap (times log2(e)) as the row's factor. What this
+// rounds is 2^-23 of softcap, so the host takes softcap up to 2^14 only (0.003 of a score). (Written with the -1: the largest prefill
+// with a softcap 837 instead of 760 us.)
 struct Cap {
-    float in, out;   // 2 log2(e) / softcap, softcap * log2(e)
-    __device__ __forceinline__ float operator()(float x) const {
-        return out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * in) + 1.0f));
-    }
+    float in, out;   // (a factor that would be infinite makes 0 of no product NaN)
+    __device__ __forceinline__ Cap(float softcap, float up) : in(fmaxf(-2.0f * kLog2e / softcap * up, -3.4e38f)), out(2.0f * softcap * kLog2e) {}
+    __device__ __forceinline__ float operator()(float x) const { return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * in) + 1.0f); }
 };
 
 // A lane's part of a row of q in float16 (K chunks of eight values), which `most` joins with the row's other lanes; a scale
@@ -208,7 +215,8 @@ __device__ __forceinline__ int scalar_load(const int32_t* p) {
 // Few rows (of one sequence and kv head: its tokens' rows, each with `group` heads): a workgroup has 16 of them and
 // one of `splits` parts of the tokens, its four waves every fourth tile of 32.
 //
-// Bound by the cache's bytes. A wave makes score^T = K q^T and out^T = V^T p^T with
+// Bound by the cache's bytes where each is read once (4.7 TB/s of 8 x 4096 tokens and of one
+// sequence of 131072, as a copy), else by the conversion, which each 16 rows do anew. A wave makes score^T = K q^T and out^T = V^T p^T with
 // v_mfma_f32_16x16x32_f16: keys and values go from memory to registers and from there into the matrix cores as the
 // first operand, with no LDS and no exchange between lanes; the scores come out in the lanes (row lane % 16, tokens
 // 4 (lane / 16) ..+3 of each run) where the second product wants its weights, since the order of tokens
@@ -289,7 +297,8 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
                                 v = max(v, uint32_t(__shfl_xor(int(v), 16)));
                                 return max(v, uint32_t(__shfl_xor(int(v), 32)));
                             });
-    const Cap cap{2.0f * kLog2e / a.softcap, a.softcap * kLog2e};
+    const Cap cap(a.softcap, up);
+    const float upx = a.softcap > 0.0f ? cap.out : up;
 
     float top = kLowest, sum = 0.0f;
     f4 o[N] = {};
@@ -319,11 +328,9 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
 #pragma unroll
             for (int i = 0; i < 2; ++i) t.keys(i, pg[i], slab, run[i]);
         }
-        float upx = up;
         if (a.softcap > 0.0f) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = cap(x[j] * up);
-            upx = 1.0f;
+            for (int j = 0; j < 8; ++j) x[j] = cap(x[j]);
         }
         // the first and last tiles hide tokens from some rows; what no row sees may be anything
         if (32 * tl < lo_most || 32 * tl + 32 > hi_least || !(ok0 && ok1)) {
@@ -442,10 +449,14 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
 // Many rows: a workgroup has 128 (of one sequence and kv head), its four waves 32 each, and one of `splits` parts
 // of the tokens, TT at a time.
 //
-// Bound by vector instructions: a tile's 16 + 16 products of v_mfma_f32_32x32x16_f16 take a wave 1024 cycles, the softmax of its
-// 32 scores a lane about as many, and its quarter of the tile's codes made float16. So the workgroup makes them once for all its
-// rows, into LDS (keys as rows of dims, values as rows of tokens, the next tile while this one is used), and scores stay in
-// the lanes that need them as weights, as above: values' tokens lie in LDS in the order in which the scores come out.
+// Bound by matrix and vector instructions alike: a tile's 16 + 16 products of v_mfma_f32_32x32x16_f16 take a wave 1024 cycles, and
+// the softmax of its 32 scores a lane with a quarter of the tile's codes made float16 about as many. So the workgroup makes them
+// once for all its rows, into LDS (keys as rows of dims, values as rows of tokens), scores stay in the lanes that need them as weights,
+// as above (values' tokens lie in LDS in the order in which the scores come out), and both kinds of instructions go side by side:
+// a tile's exponentials between the next tile's scores, and the codes of later tiles between its values' products, a slice to
+// a product, in an order that the compiler is kept from changing (8192 tokens of 32 heads of 128: 607 us for 621 of one kind after
+// the other; now 580 to 620). That is 880 to 950 TFLOP/s, three quarters of what the library's products of float16 reach.
+// 128 rows and two workgroups a CU: 256 rows in eight waves, one workgroup a CU, took as long (576 for 578 us).
 template <int D>
 struct Many {
     static constexpr int TT = D == 256 ? 32 : 64;   // tokens of a tile
@@ -626,8 +637,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
     h8 q[M::KS];
     const float up = take_q(a, static_cast<const T*>(a.q) + int64_t(s.first + row_t) * a.q_stride + int64_t(row_h) * D + 8 * c, 16, q,
                             [](uint32_t v) { return max(v, uint32_t(__shfl_xor(int(v), 32))); });
-    const Cap cap{2.0f * kLog2e / a.softcap, a.softcap * kLog2e};
-    const float upx = CAP ? 1.0f : up;
+    const Cap cap(a.softcap, up);
+    const float upx = CAP ? cap.out : up;
 
     float top = kLowest, sum = 0.0f;
     f16x o[M::NT] = {};
@@ -660,7 +671,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
     const auto look_over = [&](f16x (&x)[M::MT], bool fresh, int begin_at, int end_at) {
 #pragma unroll
         for (int i = begin_at; i < end_at; ++i) {
-            if (CAP && fresh) x[i / 16][i % 16] = cap(x[i / 16][i % 16] * up);
+            if (CAP && fresh) x[i / 16][i % 16] = cap(x[i / 16][i % 16]);
             most = fmaxf(most, x[i / 16][i % 16]);
         }
     };

@@ -228,7 +228,8 @@ struct AttendArgs {
     float* part_ml;             // and their maxima and sums of exponentials
     int splits, tiles, few;     // as in AttendPlan
 };
-// How an attention call is cut (numbers of the batch alone): see attend_plan in xl_attend.hip.
+// How an attention call is cut (numbers of the batch alone): see attend_plan in xl_attend.hip. With a window it never takes
+// more of the workspace than without.
 struct AttendPlan {
     int splits = 1, tiles = 1;                   // parts of the tokens; tiles of rows, of a sequence (few) or of all
     bool few = true;                             // which kernel
@@ -236,7 +237,6 @@ struct AttendPlan {
     uint64_t part = 0, part_ml = 0, bytes = 0;   // offsets in the workspace, and its bytes
 };
 AttendPlan attend_plan(int dim, int kv_heads, int q_heads, int n_seqs, int rows, int max_rows, int64_t max_tokens, int window);
-// The same with a window never takes more of the workspace.
 // Router over softmax or sigmoid scores (xl_score.hip).
 struct ScoreArgs {
     const void* logits;

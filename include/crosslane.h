@@ -553,15 +553,18 @@ int32_t xl_kv_write_async(xl_context* ctx, const xl_kv_batch* batch, const void*
                           int64_t v_stride, int32_t type, const xl_rotary* rotary_or_null, const void* d_q_or_null,
                           int64_t q_stride, int32_t q_heads, void* d_q_out_or_null, int64_t q_out_stride, void* stream,
                           xl_error* err);
-/* What the cache holds at the rows' positions, as floats (one rounding to `type`). */
+/* What the cache holds at the rows' positions, as floats (one rounding to `type`). k and v may be
+ * different columns of the same rows. */
 int32_t xl_kv_read_async(xl_context* ctx, const xl_kv_batch* batch, void* d_k, int64_t k_stride, void* d_v,
                          int64_t v_stride, int32_t type, void* stream, xl_error* err);
 /* Attention of the rows over the cache: for each row at position i and head h,
- *   score_j = scale * q . key_j, with softcap > 0: softcap * tanh(score_j / softcap)
+ *   score_j = scale * q . key_j, with softcap (1e-20 to 16384; 0: none): softcap * tanh(score_j / softcap)
  *   out = sum_j softmax(score)_j * value_j over j <= i, with window > 0 also j > i - window
  * keys and values of kv head h / (q_heads / kv_heads) (q_heads a multiple of kv_heads, at most 1024). q and out:
- * XL_F16 or XL_BF16. Scores, maxima and sums are float32. A token held as NaN makes
- * the outputs of the rows that see it NaN, of no others; so does a value of q that is not finite for its row and head. d_work: 256-byte aligned,
+ * XL_F16 or XL_BF16. Scores, maxima and sums are float32; keys, values and weights are rounded to float16
+ * once. A row that sees no token: zeros. A token held as NaN makes
+ * the outputs of the rows that see it NaN, of no others; so does a value of q that is not finite for its row and head.
+ * Outputs of rows that see a token whose page is out of range mean nothing. d_work: 256-byte aligned,
  * xl_attention_work_bytes(batch, q_heads) bytes, used during the call only (0 bytes:
  * may be null). The size goes by the batch's numbers, not by its pointers. out and work overlap nothing else. */
 uint64_t xl_attention_work_bytes(const xl_kv_batch* batch, int32_t q_heads);

@@ -96,6 +96,7 @@ BAD = [(n, c, m) for n in CALLS for c, m in BATCH_BAD] + [
     ("xl_attention_async", {"q_heads": 7}, "q_heads"), ("xl_attention_async", {"q_heads": 1026}, "q_heads"),
     ("xl_attention_async", {"scale": float("nan")}, "scale"), ("xl_attention_async", {"softcap": -1.0}, "softcap"),
     ("xl_attention_async", {"softcap": float("inf")}, "softcap"), ("xl_attention_async", {"softcap": 1e-21}, "softcap"),
+    ("xl_attention_async", {"softcap": 16385.0}, "softcap"),
     ("xl_kv_read_async", {"v": 7 * A + 4 * 256, "k_stride": 511, "v_stride": 511}, "overlaps"),
     ("xl_kv_read_async", {"v": 7 * A + 4 * 256, "k_stride": 512, "v_stride": 768}, "overlaps"), ("xl_attention_async", {"window": -1}, "window"),
     ("xl_attention_async", {"b_n_seqs": 65535, "b_rows": 1 << 23, "b_max_rows": 1 << 23, "b_kv_heads": 256, "q_heads": 1024,
