@@ -32,8 +32,12 @@ constexpr int few_rows(int dim) { return dim == 256 ? 192 : 64; }
 }  // namespace
 
 // Few rows: as many workgroups as the card holds at once (four a CU, two of heads of 256 values) where each has 256 tokens at
-// least, or four times as many for an even end where each has 1536. Many rows: the least of the rounds that 512 workgroups at a
-// time make, at 0.03 us a token and 5 us a workgroup, and the join's bytes at 4 TB/s.
+// least, or three times as many for an even end where each has 2048; up to 1280 tokens in one piece, which the join's launch
+// would cost more than it gives (48 sequences' last 1024 tokens 20 to 30 us, in two or three pieces 26 to 36; one sequence of
+// 1024 14.7 in one and in two). Over 77 calls, run with 1 to 128 splits each, 4 % above the best on average and 22 % at most.
+// Many rows: the least of the rounds that 512 workgroups at a
+// time make (256 of heads of 256), at 0.03 (0.05) us a token that the rows see on average and 5 us a workgroup, and the join's
+// bytes at 4 TB/s: over 62 calls of 60 to 2000 rows, run with 1 to 16 splits each, 2 % above the best on average and 18 % at most.
 AttendPlan attend_plan(int dim, int kv_heads, int q_heads, int n_seqs, int rows, int max_rows, int64_t max_tokens, int window) {
     AttendPlan p;
     const int64_t group = q_heads / kv_heads, most = max_rows * group;
@@ -44,17 +48,20 @@ AttendPlan attend_plan(int dim, int kv_heads, int q_heads, int n_seqs, int rows,
         p.tiles = int((most + 15) / 16);
         wgs = int64_t(n_seqs) * kv_heads * p.tiles;
         const int64_t held = dim < 256 ? 1024 : 512;
-        const auto splits = [&](int64_t groups, int64_t least) { return std::min((groups + wgs - 1) / wgs, (tokens + least - 1) / least); };
-        // (512 tokens: 11.4 us in one piece, 15.3 in two; 1024: 14.7 and 14.7)
-        if (tokens > 768) p.splits = int(std::min<int64_t>(128, std::max(splits(held, 256), splits(4 * held, 1536))));
+        const auto splits = [&](int64_t groups, int64_t least) {
+            return std::min(std::max<int64_t>(1, groups / wgs), (tokens + least - 1) / least);
+        };
+        if (tokens > 1280) p.splits = int(std::min<int64_t>(128, std::max(splits(held, 256), splits(3 * held, 2048))));
     } else {
         p.tiles = int((rows * group >> 7) + n_seqs);   // numbers for them; about half a tile of each sequence has rows
         wgs = int64_t(kv_heads) * p.tiles;
+        const int64_t held = dim < 256 ? 512 : 256;
+        const double seen = std::max(double(tokens) - 0.5 * max_rows, 0.5 * double(tokens)), us_token = dim < 256 ? 0.03 : 0.05;
         const int64_t real = kv_heads * (((rows * group + 127) >> 7) + (n_seqs - 1) / 2);
         double best = 1e30;
         for (int64_t k = 1; k <= 128 && (k == 1 || (real * k <= 2048 && tokens >= 256 * k)); ++k) {
-            const double rounds = double((real * k + 511) / 512), join = k == 1 ? 0.0 : 4.0 + double(rows) * q_heads * dim * double(k) * 1e-6;
-            const double us = rounds * (0.03 * double(tokens) / double(k) + 5.0) + join;
+            const double rounds = double((real * k + held - 1) / held), join = k == 1 ? 0.0 : 4.0 + double(rows) * q_heads * dim * double(k) * 1e-6;
+            const double us = rounds * (us_token * seen / double(k) + 5.0) + join;
             if (us < best) {
                 best = us;
                 p.splits = int(k);
