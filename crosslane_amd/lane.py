@@ -859,6 +859,8 @@ class Lane:
                 _refuse("work: a contiguous GPU buffer is wanted")
             wb = work.nbytes
             wp = work.data_ptr() if wb else None
+        if not 0 <= window < 2 ** 31:
+            _refuse("window: 0 to 2^31 - 1 is wanted")
         rc = lib().xl_attention_async(self._ctx, batch.ref, qp, qs, heads, kind, batch.scale if scale is None else scale, window,
                                       softcap, op, os_, wp, wb, None if stream is None else int(stream), self._errp)
         if rc:

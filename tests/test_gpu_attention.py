@@ -230,3 +230,61 @@ def test_wide_windows(lane, rows):  # noqa: F811
         lane.attention_async(b.kv, q, out, window=window, work=work)
         lane.sync()
         check(b, c, q32, out.double().cpu().numpy(), 2, "f16", 0.125, window, 0.0)
+
+
+@pytest.mark.parametrize("rows,length,D,H,kind", [(1, 9000, 64, 4, "f16"), (1, 12000, 128, 8, "bf16"), (2, 9000, 256, 2, "bf16"),
+                                                  (1, 40000, 64, 2, "bf16"), (70, 6000, 64, 1, "f16"), (70, 5000, 128, 1, "bf16"),
+                                                  (200, 4500, 256, 1, "f16")])
+def test_many_splits(lane, rows, length, D, H, kind):  # noqa: F811
+    """Tokens in more parts than one thread joins, next to a sequence that leaves most parts without tokens."""
+    step(f"attention, many splits {rows} {length} {D}")
+    b = Batch([(rows, length), (1, 2)], 64, 1, D)
+    c = filled(b, 7)
+    q, q32 = rand_rows(b.rows, H, D, kind, 5, 0, 0.5)
+    out = torch.full((b.rows, H, D), 7.0, dtype=TYPES[kind], device="cuda")
+    work = work_of(b, H)
+    torch.cuda.synchronize()
+    lane.attention_async(b.kv, q, out, work=work)
+    lane.sync()
+    check(b, c, q32, out.double().cpu().numpy(), H, kind, D ** -0.5, 0, 0.0)
+
+
+@pytest.mark.parametrize("KV,H,rows,D", [(1, 1024, 1, 64), (1, 63, 1, 128), (1, 65, 1, 128), (256, 256, 1, 64), (64, 1024, 2, 64),
+                                         (1, 192, 1, 256), (1, 97, 2, 256), (3, 1023, 1, 64)])
+def test_head_counts(lane, KV, H, rows, D):  # noqa: F811
+    """Groups around where the rows of one token are many, and the most heads of each kind."""
+    step(f"attention, heads {KV} {H} {rows} {D}")
+    b = Batch([(rows, 70), (rows, 9)], 1008, KV, D)
+    c = filled(b, 7, 0x7e)
+    q, q32 = rand_rows(b.rows, H, D, "f16", 5, 0, 0.5)
+    out = torch.full((b.rows, H, D), 7.0, dtype=torch.float16, device="cuda")
+    work = work_of(b, H)
+    torch.cuda.synchronize()
+    lane.attention_async(b.kv, q, out, work=work)
+    lane.sync()
+    check(b, c, q32, out.double().cpu().numpy(), H, "f16", D ** -0.5, 0, 0.0)
+
+
+@pytest.mark.parametrize("rows", [2, 70])
+@pytest.mark.parametrize("softcap", [1e-20, 1e-3, 16384.0])
+def test_softcap_ends(lane, rows, softcap):  # noqa: F811
+    """Caps at the ends of what a call takes, with scores far above the small ones and far below the large one."""
+    step(f"attention, softcap {rows} {softcap}")
+    b = Batch([(rows, 150)], 16, 1, 128)
+    c = filled(b, 7)
+    q, q32 = rand_rows(b.rows, 2, 128, "bf16", 5, 0, 0.5)
+    out = torch.full((b.rows, 2, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    work = work_of(b, 2)
+    torch.cuda.synchronize()
+    lane.attention_async(b.kv, q, out, softcap=softcap, work=work)
+    lane.sync()
+    check(b, c, q32, out.double().cpu().numpy(), 2, "bf16", 128 ** -0.5, 0, float(np.float32(softcap)))
+
+
+def test_window_refused(lane):  # noqa: F811
+    step("attention, windows refused")
+    b = Batch([(1, 5)], 16, 1, 64)
+    q = torch.zeros((1, 2, 64), dtype=torch.float16, device="cuda")
+    for window in (-1, 2 ** 31, 2 ** 32 + 5):
+        with pytest.raises(xl.XLError, match="window"):
+            lane.attention_async(b.kv, q, torch.zeros_like(q), window=window)
