@@ -7,11 +7,11 @@
 // instructions a pair (bits under an exponent, and that exponent's value off again) and their
 // scale and smallest value by one fused multiply-add. Scores, maxima, sums and outputs are
 // float32; what is rounded to float16, once each, by at most 2^-11 of itself:
-//   - keys and values, since the matrix cores take float16 operands. Exact ones would be two
-//     operands each (s * code has 15 bits, and m another exponent), so twice the products and
-//     the LDS. An eighth of what bfloat16 outputs round away; as much as float16 ones do, so that
-//     those are within two and a half of their own roundings (rms 5.3e-4 of the outputs' rms, 2.1e-4
-//     with exact operands), most of it by the keys.
+//   - keys and values, since the matrix cores take float16 operands: an eighth of what bfloat16 outputs round away, and as much
+//     as float16 ones do, which are so within two to three of their own roundings (rms 5.3e-4 of the outputs' rms, most of it by
+//     the keys, where exact operands have 2.1e-4). Keys as two operands each (s * code and what its rounding leaves, m by the sums
+//     of q over the groups) gave 3.0e-4 and took 10 to 12 % longer with few rows (637 MB 152 us for 137), and would take
+//     twice the LDS and the scores' products with many.
 //   - weights, for the second product. Their sum is of the weights before.
 #include <hip/hip_ext.h>
 
