@@ -222,7 +222,7 @@ __device__ __forceinline__ int scalar_load(const int32_t* p) {
 // Few rows (of one sequence and kv head: its tokens' rows, each with `group` heads): a workgroup has 16 of them and
 // one of `splits` parts of the tokens, its four waves every fourth tile of 32.
 //
-// Bound by the cache's bytes where each is read once (4.7 TB/s of 8 x 4096 tokens and of one
+// Bound by the cache's bytes where each is read once (4.8 to 5.0 TB/s of 64 sequences of up to 16384 tokens and of one
 // sequence of 131072, as a copy), else by the conversion, which each 16 rows do anew. A wave makes score^T = K q^T and out^T = V^T p^T with
 // v_mfma_f32_16x16x32_f16: keys and values go from memory to registers and from there into the matrix cores as the
 // first operand, with no LDS and no exchange between lanes; the scores come out in the lanes (row lane % 16, tokens
