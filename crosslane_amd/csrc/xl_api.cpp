@@ -2197,7 +2197,7 @@ int32_t xl_attention_async(xl_context* ctx, const xl_kv_batch* batch, const void
         check_rows(d_q, q_stride, width, 2, "q");
         check_rows(d_out, out_stride, width, 2, "out");
         const xl::AttendPlan plan = attend_plan_of(b, q_heads, window);
-        const uint64_t whole = attend_plan_of(b, q_heads, 0).bytes;
+        const uint64_t whole = std::max(plan.bytes, attend_plan_of(b, q_heads, 0).bytes);   // (a window's is never the larger one)
         // (a launch counts threads in 32 bits)
         need(plan.groups < 1 << 24, XL_E_ARG, "more workgroups than a launch takes: n_seqs * max_rows * q_heads too large");
         need(work_bytes >= whole && (d_work || whole == 0), XL_E_ARG,

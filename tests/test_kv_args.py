@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import random
 import shutil
 import subprocess
 
@@ -144,6 +145,27 @@ def test_work_is_checked():
         assert b"workspace smaller" in msg
         rc, msg = call("xl_attention_async", {**b, "work": 8 * A, "work_bytes": need})
         assert b"overlaps" in msg
+
+
+def test_work_covers_every_window():
+    """What xl_attention_work_bytes says is enough with any window."""
+    rng = random.Random(5)
+    split = 0
+    for _ in range(4000):
+        dim, kv, page = rng.choice((64, 128, 256)), rng.choice((1, 2, 8)), rng.choice((16, 64, 1024))
+        heads, seqs, most = kv * rng.choice((1, 4, 7)), rng.choice((1, 3, 40)), rng.choice((1, 2, 9, 40, 300, 1200))
+        rows, cols = rng.randint(most, seqs * most), int(rng.choice((1, 300, 3000, 40000, 400000)) * rng.random() / page) + 1
+        b = {"b_head_dim": dim, "b_kv_heads": kv, "b_page_tokens": page, "b_page_stride": kv * xl.kv_page_bytes(page, dim), "b_n_pages": 3,
+             "b_max_pages": cols, "b_table_stride": cols, "b_n_seqs": seqs, "b_rows": rows, "b_max_rows": most}
+        s = L._KVBatch(**{**BATCH, **{k[2:]: v for k, v in b.items()}})
+        need = L.lib().xl_attention_work_bytes(C.addressof(s), heads)
+        split += need > 0
+        at = [i << 40 for i in range(1, 9)]
+        b.update(b_pages=at[0], b_table=at[1], b_lens=at[2], b_starts=at[3])
+        rc, msg = call("xl_attention_async", {**b, "q": at[4], "out": at[5], "work": at[6], "q_heads": heads, "q_stride": heads * dim,
+                                              "out_stride": heads * dim, "work_bytes": need, "window": rng.choice((0, 1, 500, 2000, 9000, 100000))})
+        assert PAST in msg, (b, msg)
+    assert split > 1000
 
 
 def test_lane_refuses_host_tensors_and_wrong_shapes():
