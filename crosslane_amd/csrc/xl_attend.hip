@@ -13,7 +13,7 @@
 //     of q over the groups) gave 3.0e-4 and took 10 to 12 % longer with few rows (637 MB 152 us for 137), and would take
 //     twice the LDS and the scores' products with many.
 //   - weights, for the second product. Their sum is of the weights before.
-#include <hip/hip_ext.h>
+#include <hip/hip_runtime.h>
 
 #include <algorithm>
 
@@ -881,10 +881,10 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
 }
 
 template <class T, int D>
-hipError_t attend_go(const AttendArgs& a, hipStream_t s, hipEvent_t stop) {
+hipError_t attend_go(const AttendArgs& a, hipStream_t s) {
     const uint32_t grid = uint32_t(a.few ? a.b.n_seqs : 1) * uint32_t(a.tiles) * uint32_t(a.splits) * uint32_t(a.b.kv_heads);
     const auto go = [&](auto kernel) {
-        hipExtLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, s, nullptr, a.splits == 1 ? stop : nullptr, 0, a);
+        hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, s, a);
     };
     // bytes that one workgroup reads past the caches: decode_long 41.1 us -> 38.9, decode_batch 145.8 -> 136.4; not for heads of
     // 256, whose lanes take 32 bytes in two loads (56.5 us of drafted rows -> 57.9)
@@ -895,7 +895,7 @@ hipError_t attend_go(const AttendArgs& a, hipStream_t s, hipEvent_t stop) {
     if (a.splits > 1) {
         const int64_t heads = int64_t(a.b.rows) * a.q_heads;
         const auto join = [&](auto kernel, int64_t groups) {
-            hipExtLaunchKernelGGL(kernel, dim3(uint32_t(groups)), dim3(256), 0, s, nullptr, stop, 0, a);
+            hipLaunchKernelGGL(kernel, dim3(uint32_t(groups)), dim3(256), 0, s, a);
         };
         if (a.splits > 16) join(attend_join_kernel<T, D>, heads);
         else join(attend_join_few_kernel<T, D>, (heads * (D / 4) + 255) / 256);
@@ -903,21 +903,21 @@ hipError_t attend_go(const AttendArgs& a, hipStream_t s, hipEvent_t stop) {
     return hipGetLastError();
 }
 template <class T>
-hipError_t attend_type(const AttendArgs& a, hipStream_t s, hipEvent_t stop) {
+hipError_t attend_type(const AttendArgs& a, hipStream_t s) {
     switch (a.b.dim) {
-    case 64: return attend_go<T, 64>(a, s, stop);
-    case 128: return attend_go<T, 128>(a, s, stop);
-    case 256: return attend_go<T, 256>(a, s, stop);
+    case 64: return attend_go<T, 64>(a, s);
+    case 128: return attend_go<T, 128>(a, s);
+    case 256: return attend_go<T, 256>(a, s);
     default: return hipErrorInvalidValue;
     }
 }
 
 }  // namespace
 
-hipError_t launch_attend(const AttendArgs& a, hipStream_t s, hipEvent_t stop) {
+hipError_t launch_attend(const AttendArgs& a, hipStream_t s) {
     switch (a.type) {
-    case kActF16: return attend_type<f16>(a, s, stop);
-    case kActBF16: return attend_type<bf16>(a, s, stop);
+    case kActF16: return attend_type<f16>(a, s);
+    case kActBF16: return attend_type<bf16>(a, s);
     default: return hipErrorInvalidValue;
     }
 }

@@ -392,9 +392,9 @@ hipError_t launch_block_norm(const BlockNormArgs& a, int cus, hipStream_t s, hip
 hipError_t launch_quant_rows(const void* x, int type, int64_t x_stride, int T, int K, int8_t* q, int64_t q_stride,
                              float* scale, int* err, hipStream_t s, hipEvent_t stop);
 // The cache calls (xl_kv.hip) and the attention over the cache (xl_attend.hip).
-hipError_t launch_kv_write(const KvBatch& b, const KvRotary& r, const KvRows& x, hipStream_t s, hipEvent_t stop);
-hipError_t launch_kv_read(const KvBatch& b, const KvRows& x, hipStream_t s, hipEvent_t stop);
-hipError_t launch_attend(const AttendArgs& a, hipStream_t s, hipEvent_t stop);
+hipError_t launch_kv_write(const KvBatch& b, const KvRotary& r, const KvRows& x, hipStream_t s);
+hipError_t launch_kv_read(const KvBatch& b, const KvRows& x, hipStream_t s);
+hipError_t launch_attend(const AttendArgs& a, hipStream_t s);
 hipError_t launch_score_route(const ScoreArgs& a, hipStream_t s, hipEvent_t stop);
 hipError_t launch_lin8(const Lin8Args& a, int cus, hipStream_t s, hipEvent_t stop);
 // h = SwiGLU(g, u) elementwise over n values, with the limit (lim <= 0: none).

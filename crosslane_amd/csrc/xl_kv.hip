@@ -6,7 +6,7 @@
 // thread has eight consecutive values of a head, so a group is four threads and a row 8, 16 or
 // 32, joined by lane exchanges. Values are float32 between loads and codes; what is held is
 // rounded as crosslane.h says, to the bit.
-#include <hip/hip_ext.h>
+#include <hip/hip_runtime.h>
 
 #include <algorithm>
 
@@ -265,22 +265,22 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(KvBatch b, KvRows x) 
 int parts(int rows, int items) { return rows >= 512 ? 1 : std::min((items + kThreads - 1) / kThreads, std::max(1, 1024 / rows)); }
 
 template <class T, int D>
-hipError_t write_go(const KvBatch& b, const KvRotary& r, const KvRows& x, hipStream_t s, hipEvent_t stop) {
+hipError_t write_go(const KvBatch& b, const KvRotary& r, const KvRows& x, hipStream_t s) {
     const int items = ((x.q ? x.q_heads : 0) + 2 * b.kv_heads) * (D / 8);
-    hipExtLaunchKernelGGL((kv_write_kernel<T, D>), dim3(b.rows, parts(b.rows, items)), dim3(kThreads), 0, s, nullptr, stop, 0, b, r, x);
+    hipLaunchKernelGGL((kv_write_kernel<T, D>), dim3(b.rows, parts(b.rows, items)), dim3(kThreads), 0, s, b, r, x);
     return hipGetLastError();
 }
 template <class T, int D>
-hipError_t read_go(const KvBatch& b, const KvRows& x, hipStream_t s, hipEvent_t stop) {
+hipError_t read_go(const KvBatch& b, const KvRows& x, hipStream_t s) {
     if (b.max_rows >= 16) {
         const int64_t pairs = ((int64_t(b.rows) >> 4) + 2 * int64_t(b.n_seqs)) * b.kv_heads;
         if (pairs < int64_t(1) << 26) {   // (a launch counts threads in 32 bits)
-            hipExtLaunchKernelGGL((kv_read_runs_kernel<T, D>), dim3(uint32_t((pairs + 3) / 4)), dim3(kThreads), 0, s, nullptr, stop, 0, b, x);
+            hipLaunchKernelGGL((kv_read_runs_kernel<T, D>), dim3(uint32_t((pairs + 3) / 4)), dim3(kThreads), 0, s, b, x);
             return hipGetLastError();
         }
     }
     const int items = 2 * b.kv_heads * (D / 8);
-    hipExtLaunchKernelGGL((kv_read_kernel<T, D>), dim3(b.rows, parts(b.rows, items)), dim3(kThreads), 0, s, nullptr, stop, 0, b, x);
+    hipLaunchKernelGGL((kv_read_kernel<T, D>), dim3(b.rows, parts(b.rows, items)), dim3(kThreads), 0, s, b, x);
     return hipGetLastError();
 }
 template <class F>
@@ -304,12 +304,12 @@ hipError_t by_type_and_dim(int type, int dim, F&& f) {
 
 }  // namespace
 
-hipError_t launch_kv_write(const KvBatch& b, const KvRotary& r, const KvRows& x, hipStream_t s, hipEvent_t stop) {
+hipError_t launch_kv_write(const KvBatch& b, const KvRotary& r, const KvRows& x, hipStream_t s) {
     if (r.n > b.dim / 2) return hipErrorInvalidValue;
-    return by_type_and_dim(x.type, b.dim, [&]<class T, int D>() { return write_go<T, D>(b, r, x, s, stop); });
+    return by_type_and_dim(x.type, b.dim, [&]<class T, int D>() { return write_go<T, D>(b, r, x, s); });
 }
-hipError_t launch_kv_read(const KvBatch& b, const KvRows& x, hipStream_t s, hipEvent_t stop) {
-    return by_type_and_dim(x.type, b.dim, [&]<class T, int D>() { return read_go<T, D>(b, x, s, stop); });
+hipError_t launch_kv_read(const KvBatch& b, const KvRows& x, hipStream_t s) {
+    return by_type_and_dim(x.type, b.dim, [&]<class T, int D>() { return read_go<T, D>(b, x, s); });
 }
 
 }  // namespace xl::dev

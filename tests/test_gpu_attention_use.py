@@ -246,3 +246,88 @@ def test_many_sequences(lane, seqs, rows):  # noqa: F811
         want[:, t] = [x[p % 16] for x in c.values(b.table[i, p // 16], 0)] if p >= 0 else 0
     for x, w in zip((k, v), want):
         assert np.abs(x.cpu().numpy()[:, 0] - w).max() <= 2.0 ** -23 * 40
+
+
+def long_batch(seed=3):
+    """A sequence long enough that its attention is still running when the host enqueues the next call."""
+    P, KV, H, D, T = 64, 2, 8, 64, 200
+    b = Batch([(T, 20000)], P, KV, D)
+    filled(b, seed)
+    q, _ = rand_rows(T, H, D, "bf16", 3, 0, 0.5)
+    kv = [[rand_rows(T, KV, D, "bf16", 10 * i + j)[0] for j in range(2)] for i in range(3)]
+    return b, q, kv, work_of(b, H)
+
+
+def test_order_across_streams(lane):  # noqa: F811
+    """Writes on one stream and attention on another, in turn and without a wait by the caller: the results of one stream."""
+    step("attention half, order across streams")
+    b, q, kv, work = long_batch()
+    start = b.whole.clone()
+    s1, s2 = torch.cuda.Stream().cuda_stream, torch.cuda.Stream().cuda_stream
+    outs = [[torch.zeros_like(q) for _ in kv] for _ in range(2)]
+    backs = [[torch.zeros_like(kv[0][0]) for _ in range(2)] for _ in range(2)]
+    torch.cuda.synchronize()
+    for streams, o, back in (((s1, s1), outs[0], backs[0]), ((s1, s2), outs[1], backs[1])):
+        b.whole.copy_(start)
+        torch.cuda.synchronize()
+        for (k, v), out in zip(kv, o):
+            lane.kv_write_async(b.kv, k, v, stream=streams[1])
+            lane.attention_async(b.kv, q, out, work=work, stream=streams[0])
+        lane.kv_read_async(b.kv, *back, stream=streams[1])
+        lane.sync(streams[0])
+        lane.sync(streams[1])
+    assert all(torch.equal(x, y) for x, y in zip(outs[0] + backs[0], outs[1] + backs[1]))
+
+
+def test_sync_waits_for_another_stream(lane):  # noqa: F811
+    """A wait for the context's own stream waits for a call that named another one."""
+    step("attention half, sync of another stream")
+    b, q, kv, work = long_batch()
+    s1 = torch.cuda.Stream().cuda_stream
+    want, out = torch.zeros_like(q), torch.zeros_like(q)
+    torch.cuda.synchronize()
+    lane.attention_async(b.kv, q, want, work=work)
+    lane.sync()
+    lane.attention_async(b.kv, q, out, work=work, stream=s1)
+    lane.sync()
+    got = out.cpu()   # (torch's own stream does not wait for s1)
+    assert torch.equal(got, want.cpu())
+
+
+def test_order_around_a_capture():
+    """A call on another stream while the previous call's stream is captured is refused, unless it is captured too: then it
+    becomes part of the same graph, ordered."""
+    step("attention half, order around a capture")
+    b, q, kv, work = long_batch()
+    out, other = torch.zeros_like(q), torch.zeros_like(q)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    with open_lane() as ln:
+        torch.cuda.synchronize()
+        ln.attention_async(b.kv, q, out, work=work, stream=s1.cuda_stream)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s1):
+            ln.kv_write_async(b.kv, *kv[0], stream=s1.cuda_stream)
+            with pytest.raises(xl.XLError, match="being captured"):
+                ln.attention_async(b.kv, q, other, work=work, stream=s2.cuda_stream)
+            s2.wait_stream(s1)
+            ln.attention_async(b.kv, q, out, work=work, stream=s2.cuda_stream)
+            s1.wait_stream(s2)
+        start = b.whole.clone()
+        for turn in range(3):
+            b.whole.copy_(start)
+            torch.cuda.synchronize()
+            ln.kv_write_async(b.kv, *kv[turn], stream=s2.cuda_stream)
+            ln.attention_async(b.kv, q, other, work=work, stream=s2.cuda_stream)
+            ln.sync(s2.cuda_stream)
+            want = other.clone()
+            b.whole.copy_(start)
+            out.zero_()
+            for x, y in zip(kv[0], kv[turn]):
+                x.copy_(y)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(s1):
+                g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and (other == want).all()
+        ln.sync()
