@@ -777,7 +777,8 @@ void xl_close(xl_context* ctx) {
     (void)hipSetDevice(ctx->cfg.device);
     // The last call may have run on a caller stream: wait for it, then for the
     // context stream, before any memory goes back.
-    if (ctx->done) (void)wait_for_last(ctx);
+    if (ctx->pending) (void)hipDeviceSynchronize();   // (the stream itself may be gone)
+    else if (ctx->done && ctx->has_last) (void)hipEventSynchronize(ctx->done);
     if (ctx->stream) (void)hipStreamSynchronize(ctx->stream);
     for (auto& e : ctx->prof.ev)   // profiling left active (xl_profile_end never called)
         if (e) (void)hipEventDestroy(e);

@@ -481,7 +481,7 @@ int32_t xl_linear_i8_async(xl_context* ctx, const void* d_x, int32_t x_type, con
  * context's workspace; element types and strides as in the section above, a row's
  * heads consecutive (head_dim values each). What orders such a call before the context's
  * next one on another stream is recorded by that next call: it then waits for whatever was
- * enqueued on the first stream until there, which must live until then or until xl_sync, and
+ * enqueued on the first stream until there, which must live until then, xl_sync or xl_close, and
  * while that stream is captured (and the next call's is not) the next call is refused.
  *
  * A page holds page_tokens tokens: for each kv head xl_kv_page_bytes(page_tokens,
