@@ -275,3 +275,16 @@ def test_read_into_columns(lane, rows):
         for h in range(2):
             x, y = (z[p % 16] for z in ref.values(b.table[i, p // 16], h))
             assert np.abs(got[t, 3 + h] - x).max() <= 2.0 ** -23 * np.abs(x).max() and np.abs(got[t, h] - y).max() <= 2.0 ** -23 * np.abs(y).max()
+
+
+def test_sections_refused(lane):
+    step("cache write, sections refused")
+    b = Batch([(1, 5)], 16, 1, 64)
+    k = torch.zeros((1, 1, 64), dtype=torch.float16, device="cuda")
+    freqs = torch.ones(32, device="cuda")
+    torch.cuda.synchronize()
+    for sections in ((2 ** 32 + 32,), (32.0,), (33,), (-32,), (32, 0)):
+        with pytest.raises(xl.XLError, match="section"):
+            lane.kv_write_async(b.kv, k, k, freqs=freqs, sections=sections)
+    lane.kv_write_async(b.kv, k, k, freqs=freqs, sections=[32])
+    lane.sync()
