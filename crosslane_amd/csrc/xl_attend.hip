@@ -693,6 +693,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
     // Behind the last tile that is work on tokens that are there, not used.
     const auto tile = [&](f16x (&x)[M::MT], f16x (&y)[M::MT], int tl) {
         const int buf = (tl - begin) & 1;
+        // The stores of the tile before are done before the barrier hands them over. It is stated here: the wait of __syncthreads() is
+        // left out by the compiler round the loop, whose entry has nothing outstanding.
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __syncthreads();
         if (TT * tl < lo_most || TT * (tl + 1) > hi_least) {   // tokens that some rows do not see
 #pragma unroll
