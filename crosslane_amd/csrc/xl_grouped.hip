@@ -1003,6 +1003,9 @@ __global__ __launch_bounds__(NW * 64, 1) void grouped_kernel(GroupArgs a) {
                             : total >= 16 * NW * int(gridDim.x) ? NW : 4;
         uint8_t* wl = ti == 2 ? lds + kL_TAB1 + wv * kL_WAVE1 : lds + kL_TAB + wv * kL_WAVE;
         if (MASK == 7 || i == 0) {
+            // A wave that fetched the empty last bundle has stored s_bundle, which thread 0 stores anew behind the barrier: its store is done
+            // first. (__syncthreads() alone has the compiler leave the wait out round the loop, whose entry has nothing outstanding.)
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __syncthreads();   // every wave is done with the previous type's tables
             if (t == 0) {
                 s_open = total > 0 && (i == 0 || __hip_atomic_load(next + ti, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) * bs < total);

@@ -125,7 +125,7 @@ def with_far_branches(lines):
         yield text
 
 
-@pytest.mark.parametrize("src", ["xl_attend.hip"])
+@pytest.mark.parametrize("src", [s for s in _build.SOURCES if s.endswith(".hip")])
 def test_no_barrier_with_lds_outstanding(src, tmp_path):
     if not os.path.exists(os.path.join(TOOLS, "llvm-objdump")) or not shutil.which(_build.HIPCC):
         pytest.skip("no ROCm tools")
