@@ -259,17 +259,18 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
 
     const Slab<D> slab(b.page);
     const uint8_t* base = b.pages + int64_t(head) * slab.bytes();
-    const int last_run = (hi_all - 1) >> 4;
+    const int first_run = lo_all >> 4, last_run = (hi_all - 1) >> 4;
     TileLoads<D, ONCE> t(lane);
     const Codes codes;
-    // A tile's pages, by the table's entries, which are read a tile before they are used. Where a tile's second run lies
-    // behind the last token, it is the last run; where an entry is no page, the first page: such tokens are hidden.
+    // A tile's pages, by the table's entries, which are read a tile before they are used. A run before the first token that a row
+    // sees, or behind the last, is the first or last run with such a token (other pages may be gone); where an entry is no page,
+    // the first page: such tokens are hidden.
     const int32_t* row_of_table = b.table + int64_t(seq) * b.table_stride;
     int id[2], in[2];
-    const auto look = [&](int tl) {
+    const auto look = [&](int tl, int first = INT32_MIN) {   // (the first tile alone has a run before the first token)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint32_t run = uint32_t(min(2 * tl + i, last_run));
+            const uint32_t run = uint32_t(min(max(2 * tl + i, first), last_run));
             const uint32_t col = b.page_inv ? __umulhi(run, b.page_inv) : run;
             in[i] = int(run - col * uint32_t(b.page >> 4));
             id[i] = scalar_load(row_of_table + col);
@@ -287,7 +288,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
         }
     };
     if (begin < end) {
-        look(begin);
+        look(begin, first_run);
         turn_to();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -295,6 +296,14 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
             t.values(i, pg[i], slab, run[i]);
         }
         if (begin + 4 < end) look(begin + 4);
+        if (32 * begin < lo_all) {   // values before the first token that a row sees
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (32 * begin + 16 * (j >> 2) + 4 * c + (j & 3) < lo_all) {
+                    t.vs[j >> 2][(j & 3) >> 1] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+                    t.vs[j >> 2][2 + ((j & 3) >> 1)] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+                }
+        }
     }
 
     // q: the second operand, row lane % 16, dims 32g + 8c ..+7
@@ -518,8 +527,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
     const int begin = tile0 + split * per, end = tile0 + min(tiles, (split + 1) * per);
 
     // This thread's part of a tile: words of one token's keys, and eight dims of four (or two) tokens' values. A wave's lie in one run
-    // of 16 tokens, whose page is looked up a tile before it is used; a run behind the last token is the last one, an entry
-    // that is no page the first page. Keys are loaded a tile before the values of the same tokens.
+    // of 16 tokens, whose page is looked up a tile before it is used; a run before the first token that a row sees, or behind the
+    // last, is the first or last run with such a token (other pages may be gone), an entry that is no page the first page. Keys are
+    // loaded a tile before the values of the same tokens.
     const Slab<D> slab(b.page);
     const Codes codes;
     const uint8_t* base = b.pages + int64_t(head) * slab.bytes();
@@ -531,7 +541,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
     const uint32_t kv_at = slab.v_scales() + 2 * ((k_tok >> 2 & 3) * 8 * G + (k_tok & 3));   // the scale of the same token's values
     const uint32_t vc_at = slab.v_codes() + 2 * ((v_quad & 3) * D + v_chunk * 8) + 8 * v_pair;
     const uint32_t vs_at = slab.v_scales() + 16 * ((v_quad & 3) * G + v_chunk / 4) + 4 * v_pair;
-    const int last_run = (hi_all - 1) >> 4;
+    const int first_run = lo_all >> 4, last_run = (hi_all - 1) >> 4;
     struct Page {
         int id, in;
     };
@@ -539,8 +549,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
         const uint8_t *code, *scale;
         bool ok;
     };
-    const auto look = [&](int tl) {
-        const uint32_t run = uint32_t(min(TT == 64 ? 4 * tl + wave : 2 * tl + (wave >> 1), last_run));
+    const auto look = [&](int tl, int first = INT32_MIN) {   // (the first tile alone has runs before the first token)
+        const uint32_t run = uint32_t(min(max(TT == 64 ? 4 * tl + wave : 2 * tl + (wave >> 1), first), last_run));
         const uint32_t col = b.page_inv ? __umulhi(run, b.page_inv) : run;
         return Page{scalar_load(row_of_table + col), int(run - col * uint32_t(b.page >> 4))};
     };
@@ -751,7 +761,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
     };
     if (begin < end) {
         RawKeys next;
-        const Run r0 = run_of(look(begin)), r1 = run_of(look(begin + 1));
+        const Run r0 = run_of(look(begin, first_run)), r1 = run_of(look(begin + 1));
         fetch_keys(r0, k_raw);
         fetch_values(r0, v_raw);
         fetch_keys(r1, next);
@@ -760,6 +770,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
         page = look(begin + 4);
         check_keys(k_raw);
         check_values(v_raw, begin);
+        if (TT * begin < lo_all) {   // values before the first token that a row sees
+#pragma unroll
+            for (int i = 0; i < VP; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    if (TT * begin + 4 * v_quad + 2 * (v_pair + i) + j < lo_all) {
+                        v_raw.step[i] &= j ? 0x0000ffffu : 0xffff0000u;
+                        v_raw.small[i] &= j ? 0x0000ffffu : 0xffff0000u;
+                    }
+        }
 #pragma unroll
         for (int i = 0; i < KSLICES; ++i) stage_keys(k_raw, 0, i);
 #pragma unroll

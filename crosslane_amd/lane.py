@@ -852,7 +852,8 @@ class Lane:
     def attention_async(self, batch: KVBatch, q, out, scale: Optional[float] = None, window: int = 0, softcap: float = 0.0,
                         work=None, stream=None) -> None:
         """out [rows, q_heads, head_dim] = attention of the rows of q over the batch's cache (f16 or
-        bf16): tokens up to each row's own, with window > 0 the last `window` of them, softcap > 0 (up to 16384): scores
+        bf16): tokens up to each row's own, with window > 0 the last `window` of them (pages below every
+        row's window may be gone, their entries of the table anything), softcap > 0 (up to 16384): scores
         through softcap * tanh(score / softcap). scale: 1 / sqrt(head_dim) by default. work:
         attention_work_bytes(batch, q_heads) bytes (None where that is 0)."""
         shape = q.shape

@@ -567,6 +567,7 @@ int32_t xl_kv_read_async(xl_context* ctx, const xl_kv_batch* batch, void* d_k, i
  * XL_F16 or XL_BF16. Scores, maxima and sums are float32; keys, values and weights are rounded to float16
  * once. A row that sees no token: zeros. A token held as NaN makes
  * the outputs of the rows that see it NaN, of no others; so does a value of q that is not finite for its row and head.
+ * Tokens that no row of their sequence sees (below the window of its first row) need no page, and what lies in their places may be anything.
  * Outputs of rows that see a token whose page is out of range mean nothing. d_work: 256-byte aligned,
  * xl_attention_work_bytes(batch, q_heads) bytes, used during the call only (0 bytes:
  * may be null). The size goes by the batch's numbers, not by its pointers. out and work overlap nothing else. */
