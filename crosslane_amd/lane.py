@@ -384,7 +384,8 @@ class Lane:
     """One context: a resident bank of n_layers x n_experts experts on one GPU.
 
     The *_async calls enqueue on `stream` (a raw HIP stream handle), by default
-    on the context's own non-blocking stream. Tensors passed to them must stay
+    on the context's own non-blocking stream, which does not wait for what PyTorch has
+    enqueued on its streams (a fill of an output, say). Tensors passed to them must stay
     alive until that stream has run the call (`sync(stream)`): PyTorch's caching
     allocator hands a freed tensor's memory to the next allocation on its own
     current stream at once, so a temporary such as `torch.tensor(...).cuda()`

