@@ -13,6 +13,8 @@
 //     of q over the groups) gave 3.0e-4 and took 10 to 12 % longer with few rows (637 MB 152 us for 137), and would take
 //     twice the LDS and the scores' products with many.
 //   - weights, for the second product. Their sum is of the weights before.
+// A row before its sequence's first token sees none, and its outputs are zeros. Of every other row the sum of the weights is 1 at
+// least, but where its scores pass what float32 holds: then it is 0 or a NaN, and the outputs are NaN.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -447,7 +449,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
     for (int n = 0; n < N; ++n) y[n] = (part[0][r][d + n] + part[1][r][d + n]) + (part[2][r][d + n] + part[3][r][d + n]);
     const int t_out = (row0 + r) / a.group, h_out = head * a.group + (row0 + r) - t_out * a.group;
     if (a.splits == 1) {
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        const float inv = before + t_out < 0 ? 0.0f : 1.0f / total;
         T v[N];
 #pragma unroll
         for (int n = 0; n < N; ++n) v[n] = T(y[n] * inv);
@@ -803,7 +805,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
     if (32 * wave + (lane & 31) >= rows) return;
     // the lane has chunks 8u + 4c + i of its row, whose eight dims lie in as many registers (of row j * C + chunk of the products)
     const int64_t out_row = int64_t(s.first + row_t), part = (out_row * a.q_heads + row_h) * a.splits + split;
-    const float inv = a.splits > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = a.splits > 1 ? 1.0f : hi <= 0 ? 0.0f : 1.0f / sum;
 #pragma unroll
     for (int u = 0; u < C / 8; ++u)
 #pragma unroll
@@ -844,7 +846,7 @@ __global__ __launch_bounds__(256) void attend_join_few_kernel(AttendArgs a) {
         total += ml[i][1] * f;
         y += *reinterpret_cast<const f4*>(p + i * D) * f;
     }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    const float inv = s.len - s.n + t - s.first < 0 ? 0.0f : 1.0f / total;
     T v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = T(y[i] * inv);
@@ -896,7 +898,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
     if (threadIdx.x >= L) return;
 #pragma unroll
     for (int i = 1; i < 4; ++i) y += sums[i][lane];
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    const float inv = s.len - s.n + t - s.first < 0 ? 0.0f : 1.0f / total;
     T o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = T(y[i] * inv);

@@ -565,7 +565,8 @@ int32_t xl_kv_read_async(xl_context* ctx, const xl_kv_batch* batch, void* d_k, i
  *   out = sum_j softmax(score)_j * value_j over j <= i, with window > 0 also j > i - window
  * keys and values of kv head h / (q_heads / kv_heads) (q_heads a multiple of kv_heads, at most 1024). q and out:
  * XL_F16 or XL_BF16. Scores, maxima and sums are float32; keys, values and weights are rounded to float16
- * once. A row that sees no token: zeros. A token held as NaN makes
+ * once. A row that sees no token: zeros. Scores (times log2(e)) past what float32 holds: NaN where
+ * they are a row's largest. A token held as NaN makes
  * the outputs of the rows that see it NaN, of no others; so does a value of q that is not finite for its row and head.
  * Tokens that no row of their sequence sees (below the window of its first row) need no page, and what lies in their places may be anything.
  * Outputs of rows that see a token whose page is out of range mean nothing. d_work: 256-byte aligned,
