@@ -211,6 +211,8 @@ struct xl_context {
     hipStream_t last_stream = nullptr;
     bool has_last = false;
     bool pending = false;                // the last call left `done` to be recorded when it is needed
+    int steady = kSteady;                // calls since one named another stream than the call before it, up to kSteady
+    static constexpr int kSteady = 64;
     // Layer calls by the way they ran (XL_LAUNCH_*), for xl_debug_launch_counts.
     int64_t launches[XL_LAUNCH_KINDS] = {};
 };
@@ -289,7 +291,9 @@ struct Ordered {
     bool carried = false;   // the call's last launch already carries `done` as its stop event
     bool later = false;     // `done` is recorded by the next call on another stream, should there be one
     Ordered(xl_context* c, hipStream_t st) : ctx(c), s(st) {
-        if (!ctx->has_last || ctx->last_stream == s) return;
+        const bool other = ctx->has_last && ctx->last_stream != s;
+        ctx->steady = other ? 0 : std::min(ctx->steady + 1, xl_context::kSteady);
+        if (!other) return;
         if (ctx->pending && !record_now()) return;
         hip_check(hipStreamWaitEvent(s, ctx->done, 0), "order after the previous call");
     }
@@ -317,8 +321,14 @@ struct Ordered {
     hipEvent_t stop() const { return ctx->done; }
     void carried_by_launch(bool yes) { carried = yes; }
     // Short calls: a launch that carries an event costs the host 0.2 us more than one that does not, and after some thousand of
-    // them, on most hosts, 3.5 more (7.2 for 3.7); a record of its own costs 5.
-    void recorded_later() { later = true; }
+    // them, on most hosts, 3.5 more (7.2 for 3.7); a record of its own costs 5. But a record made later covers whatever else was
+    // enqueued on the stream by then, so a caller that changes streams has it with the call: the next call on another stream
+    // waits for no more than it must. (Not in a capture, which may end before that next call.)
+    void recorded_later() {
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+        later = ctx->steady >= xl_context::kSteady ||
+                (hipStreamIsCapturing(s, &capture) == hipSuccess && capture != hipStreamCaptureStatusNone);
+    }
     ~Ordered() {
         if (later || carried || hipEventRecord(ctx->done, s) == hipSuccess) {
             ctx->last_stream = s;

@@ -482,7 +482,9 @@ int32_t xl_linear_i8_async(xl_context* ctx, const void* d_x, int32_t x_type, con
  * heads consecutive (head_dim values each). What orders such a call before the context's
  * next one on another stream is recorded by that next call: it then waits for whatever was
  * enqueued on the first stream until there, which must live until then, xl_sync or xl_close, and
- * while that stream is captured (and the next call's is not) the next call is refused.
+ * while that stream is captured (and the next call's is not) the next call is refused. Where
+ * one of the context's last 64 calls named another stream than the call before it, it is recorded
+ * with the call (5 us of host time; not while the stream is captured), and the next call waits for that call alone.
  *
  * A page holds page_tokens tokens: for each kv head xl_kv_page_bytes(page_tokens,
  * head_dim) bytes, the heads' parts consecutive. A group of 32 values of a head is
