@@ -339,6 +339,8 @@ class KVBatch:
     the tensors are kept alive with it. A layer with a cache of its own has a batch of its own."""
 
     def __init__(self, cache, table, lens, starts, rows: int, head_dim: int, max_rows: Optional[int] = None):
+        if not (1 <= rows < 2 ** 31 and (max_rows is None or 1 <= max_rows < 2 ** 31)):   # (a field of the struct drops higher bits)
+            _refuse("rows and max_rows: 1 to 2^31 - 1 is wanted")
         sh, st = cache.shape, cache.stride()
         if len(sh) != 3 or str(cache.dtype) != "torch.uint8" or st[2] != 1 or (st[1] != sh[2] and sh[1] != 1):
             _refuse("cache: uint8 [n_pages, kv_heads, bytes] with a page's heads consecutive is wanted")
