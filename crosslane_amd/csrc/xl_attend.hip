@@ -8,8 +8,8 @@
 // scale and smallest value by one fused multiply-add. Scores, maxima, sums and outputs are
 // float32; what is rounded to float16, once each, by at most 2^-11 of itself:
 //   - keys and values, since the matrix cores take float16 operands: an eighth of what bfloat16 outputs round away, and as much
-//     as float16 ones do, which are so within two to three of their own roundings (rms 5.3e-4 of the outputs' rms, most of it by
-//     the keys, where exact operands have 2.1e-4). Keys as two operands each (s * code and what its rounding leaves, m by the sums
+//     as float16 ones do, which are so within two to four of their own roundings (rms 3.0e-4 to 7.5e-4 of the outputs' rms over
+//     the measured calls, most of it by the keys, where exact operands have 2.1e-4). Keys as two operands each (s * code and what its rounding leaves, m by the sums
 //     of q over the groups) gave 3.0e-4 and took 10 to 12 % longer with few rows (637 MB 152 us for 137), and would take
 //     twice the LDS and the scores' products with many.
 //   - weights, for the second product. Their sum is of the weights before.
@@ -135,7 +135,7 @@ __device__ __forceinline__ float rows_sum(float v) {
 // Scores through softcap * tanh(score / softcap), of a row's products x: tanh y = 2 / (1 + exp(-2 y)) - 1. A row's scores may all be off
 // by the same, so the -1 is left out: 1 / (1 + exp(-2 y)) of each, and twice softcap (times log2(e)) as the row's factor. What this
 // rounds is 2^-23 of softcap, so the host takes softcap up to 2^14 only (0.003 of a score). (Written with the -1: the largest prefill
-// with a softcap 837 instead of 760 us.)
+// with a softcap 837 instead of 760 us; 710 to 760 by card, 580 to 660 without a cap: 8,350 more vector instructions a wave on 19,440.)
 struct Cap {
     float in, out;   // (a factor that would be infinite makes 0 of no product NaN)
     __device__ __forceinline__ Cap(float softcap, float up) : in(fmaxf(-2.0f * kLog2e / softcap * up, -3.4e38f)), out(2.0f * softcap * kLog2e) {}
@@ -473,7 +473,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void attend_few_kernel(Atten
 // as above (values' tokens lie in LDS in the order in which the scores come out), and both kinds of instructions go side by side:
 // a tile's exponentials between the next tile's scores, and the codes of later tiles between its values' products, a slice to
 // a product, in an order that the compiler is kept from changing (8192 tokens of 32 heads of 128: 607 us for 621 of one kind after
-// the other; now 580 to 620). That is 880 to 950 TFLOP/s, three quarters of what the library's products of float16 reach.
+// the other; now 580 to 660 by card). That is 830 to 950 TFLOP/s, 70 to 80 % of what the library's products of float16 reach.
 // 128 rows and two workgroups a CU: 256 rows in eight waves, one workgroup a CU, took as long (576 for 578 us).
 template <int D>
 struct Many {

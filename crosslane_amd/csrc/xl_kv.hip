@@ -116,7 +116,7 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(KvBatch b, KvRotary 
             hi = fmaxf(hi, v[e]);
         }
         // the lanes of this row (a wave has whole rows)
-        const uint64_t row = (C == 64 ? ~0ull : (1ull << C) - 1) << (threadIdx.x & 63 & ~(C - 1));
+        const uint64_t row = ((1ull << C) - 1) << (threadIdx.x & 63 & ~(C - 1));
         fine = (__ballot(!fine) & row) == 0;
         const f16 m = f16(quad_min(lo));
         const f16 step = rounded<f16>(fmaxf((quad_max(hi) - float(m)) * (1.0f / 15.0f), 0.0f));   // (m may have been rounded up)

@@ -500,7 +500,8 @@ int32_t xl_linear_i8_async(xl_context* ctx, const void* d_x, int32_t x_type, con
  *                   of token 2b + e of the four, in order
  *   values' scales  P/4 x [G][2][4] float16: s of the four tokens, then m
  * A kernel of the caller's own may fill it too, if scales are >= 0 and a row's
- * scales are either all finite or all the NaN 0x7e00 with m NaN.
+ * scales are either all finite or all the NaN 0x7e00 with m NaN. (Attention reads values as
+ * float16: 15 * s + m and m lie within +-65504 for it.)
  *
  * A batch: sequence b has d_lens[b] tokens, token j in page d_table[b * table_stride
  * + j / page_tokens] at j % page_tokens. Its rows are d_starts[b] .. d_starts[b + 1] - 1
