@@ -10,6 +10,7 @@ import os
 import re
 import shutil
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 
@@ -76,14 +77,30 @@ def test_the_walk_finds_what_it_looks_for():
     assert outstanding(["s_cbranch_execz L1", "ds_write_b32 v0, v1", "s_branch L2", "L1:", wait, "L2:", barrier]) == [(True, False)]
 
 
-def kernels(src, tmp):
-    """Names and instructions of a source's kernels, as they are built: from the library's object, or, where that is
-    older than the source, from a new one."""
-    obj = os.path.join(_build.OBJDIR, src.replace(".hip", ".o"))
-    inputs = [os.path.join(_build.CSRC, f) for f in (src, *_build.HEADERS)]
-    if not os.path.exists(obj) or os.path.getmtime(obj) < max(map(os.path.getmtime, inputs)):
-        obj = str(tmp / "new.o")
-        subprocess.run([_build.HIPCC, *_build.CFLAGS, "-w", "-c", inputs[0], "-o", obj], check=True, capture_output=True)
+SOURCES = [s for s in _build.SOURCES if s.endswith(".hip")]
+
+
+@pytest.fixture(scope="module")
+def objects(tmp_path_factory):
+    """Each source's object: the library's, or, where that is older than the source, a new one."""
+    if not os.path.exists(os.path.join(TOOLS, "llvm-objdump")) or not shutil.which(_build.HIPCC):
+        pytest.skip("no ROCm tools")
+    tmp = tmp_path_factory.mktemp("objects")
+
+    def of(src):
+        obj = os.path.join(_build.OBJDIR, src.replace(".hip", ".o"))
+        inputs = [os.path.join(_build.CSRC, f) for f in (src, *_build.HEADERS)]
+        if not os.path.exists(obj) or os.path.getmtime(obj) < max(map(os.path.getmtime, inputs)):
+            obj = str(tmp / os.path.basename(obj))
+            subprocess.run([_build.HIPCC, *_build.CFLAGS, "-w", "-c", inputs[0], "-o", obj], check=True, capture_output=True)
+        return obj
+
+    with ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:
+        return dict(zip(SOURCES, pool.map(of, SOURCES)))
+
+
+def kernels(obj, tmp):
+    """Names and instructions of an object's kernels."""
     run = lambda tool, *args: subprocess.run([os.path.join(TOOLS, tool), *map(str, args)], check=True, capture_output=True, text=True)  # noqa: E731
     run("llvm-objcopy", f"--dump-section=.hip_fatbin={tmp / 'fat'}", obj, tmp / "copy.o")
     run("clang-offload-bundler", "--unbundle", "--type=o", f"--input={tmp / 'fat'}", f"--targets=hipv4-amdgcn-amd-amdhsa--{_build.ARCH}",
@@ -125,12 +142,10 @@ def with_far_branches(lines):
         yield text
 
 
-@pytest.mark.parametrize("src", [s for s in _build.SOURCES if s.endswith(".hip")])
-def test_no_barrier_with_lds_outstanding(src, tmp_path):
-    if not os.path.exists(os.path.join(TOOLS, "llvm-objdump")) or not shutil.which(_build.HIPCC):
-        pytest.skip("no ROCm tools")
+@pytest.mark.parametrize("src", SOURCES)
+def test_no_barrier_with_lds_outstanding(src, objects, tmp_path):
     barriers, bad = 0, []
-    for name, lines in kernels(src, tmp_path):
+    for name, lines in kernels(objects[src], tmp_path):
         found = outstanding(list(lines))
         barriers += len(found)
         bad += [name] * sum(any(f) for f in found)
